@@ -101,6 +101,25 @@ def _bind() -> None:
         "b2_rope_kv_store_typed": (_i, [_vp, _i, _i, _i, _i, _i, _vp, _vp, _vp, _vp, _vp, _i, _vp, _i, _i, _vp]),
         "b2_attn_decode_typed": (_i, [_vp, _vp, _i, _vp, _i, _vp, _vp, _i, _i, _i, _i, _i, _i, _vp, _vp]),
         "b2_kv_shift_k_typed": (_i, [_vp, _i, _i, _i, _i, _i, _i, _i, _i, _f, _vp]),
+        "b2_page_cache_bytes": (_i, [_vp, _vp, _vp]),
+        "b2_page_rope_store": (_i, [_vp, ctypes.c_int32, _vp, ctypes.c_int32, _vp, _i, _vp, _i, _vp, ctypes.c_int32,
+                                    _vp, _vp, ctypes.c_int32, ctypes.c_int32, _i, _vp]),
+        "b2_rope_sections": (_i, [_vp, ctypes.c_int32, ctypes.c_int32, _i, _vp]),
+        "b2_page_attn_workspace_bytes": (_i, [_vp, _vp, ctypes.c_int32, _i, _vp]),
+        "b2_page_attn": (_i, [_vp, ctypes.c_int32, _vp, ctypes.c_int32, _vp, _vp, _i, _f, ctypes.c_int32, _vp, _sz,
+                              _vp, _vp]),
+        "b2_page_copy": (_i, [_vp, _vp, _vp, ctypes.c_int32, _vp]),
+        "b2_page_gather": (_i, [_vp, ctypes.c_int32, _vp, _vp, ctypes.c_int32, _vp, _vp, ctypes.c_int32, _vp]),
+        "b2_page_pool_create": (_i, [ctypes.c_int32, ctypes.c_int32, ctypes.c_int32, ctypes.c_int32, _vp]),
+        "b2_page_pool_destroy": (_i, [_vp]),
+        "b2_page_pool_extend": (_i, [_vp, ctypes.c_int32, ctypes.c_int32, _vp, _vp]),
+        "b2_page_pool_fork": (_i, [_vp, ctypes.c_int32, ctypes.c_int32, ctypes.c_int32]),
+        "b2_page_pool_truncate": (_i, [_vp, ctypes.c_int32, ctypes.c_int32]),
+        "b2_page_pool_keep": (_i, [_vp, ctypes.c_int32, _vp, ctypes.c_int32, _vp]),
+        "b2_page_pool_settle": (_i, [_vp]),
+        "b2_page_pool_defrag": (_i, [_vp, _vp, _vp, ctypes.c_int32, _vp]),
+        "b2_page_pool_table": (_i, [_vp, ctypes.c_int32, _vp, _vp]),
+        "b2_page_pool_free_pages": (_i, [_vp, _vp]),
         "b2_model_default_params": (None, [_vp]),
         "b2_nccl_unique_id": (_i, [_vp]),
         "b2_model_load": (_i, [ctypes.c_char_p, _vp, _vp]),
@@ -416,6 +435,184 @@ def quantize_act(act_type: int, x: np.ndarray) -> np.ndarray:
     out = DeviceBuffer(n_tok * row_bytes(act_type, k))
     check(lib.b2_quantize_act(act_type, xd.ptr, n_tok, k, out.ptr, None), "quantize_act")
     return out.download(np.uint8).reshape(n_tok, -1)
+
+
+# ---- paged K/V cache ----------------------------------------------------------------------------
+ROPE_ADJACENT, ROPE_HALVES = 0, 1
+
+
+def _addr(x):
+    """A device address: a DeviceBuffer's, or the number itself (another library's pointer)."""
+    return x.ptr if isinstance(x, DeviceBuffer) else x
+
+
+class _PageCacheC(ctypes.Structure):
+    _fields_ = [("k", ctypes.c_void_p), ("v", ctypes.c_void_p), ("n_layer", ctypes.c_int32),
+                ("n_pages", ctypes.c_int32), ("page_size", ctypes.c_int32), ("n_kv", ctypes.c_int32),
+                ("head_dim", ctypes.c_int32), ("type_k", ctypes.c_int32), ("type_v", ctypes.c_int32)]
+
+
+class _PageBatchC(ctypes.Structure):
+    _fields_ = [("q_start", ctypes.c_void_p), ("kv_len", ctypes.c_void_p), ("table", ctypes.c_void_p),
+                ("n_seq", ctypes.c_int32), ("max_pages", ctypes.c_int32), ("n_tok", ctypes.c_int32),
+                ("max_q", ctypes.c_int32)]
+
+
+class PageCache:
+    """The pools of a paged K/V cache: [n_layer][n_pages][n_kv][page_size]
+    rows of K and of V.  Without k and v the pools are allocated here (and
+    start undefined); k and v may be DeviceBuffers or device addresses, which
+    the caller keeps alive."""
+
+    def __init__(self, n_layer: int, n_pages: int, page_size: int, n_kv: int, head_dim: int, type_k: int = F16,
+                 type_v: int = F16, k=None, v=None):
+        self.c = _PageCacheC(None, None, n_layer, n_pages, page_size, n_kv, head_dim, type_k, type_v)
+        self.ref = ctypes.byref(self.c)
+        bk, bv = ctypes.c_size_t(), ctypes.c_size_t()
+        check(lib.b2_page_cache_bytes(self.ref, ctypes.byref(bk), ctypes.byref(bv)), "page_cache_bytes")
+        self.bytes_k, self.bytes_v = bk.value, bv.value
+        self.k = DeviceBuffer(self.bytes_k) if k is None else k
+        self.v = DeviceBuffer(self.bytes_v) if v is None else v
+        self.c.k, self.c.v = _addr(self.k), _addr(self.v)
+
+
+class PageBatch:
+    """One step's sequences: q_start [n_seq+1], kv_len [n_seq] and table
+    [n_seq][max_pages], as numpy arrays (uploaded here, sizes taken from
+    them) or as device addresses with the sizes given."""
+
+    def __init__(self, q_start, kv_len, table, n_seq: int | None = None, max_pages: int | None = None,
+                 n_tok: int | None = None, max_q: int | None = None):
+        if isinstance(q_start, np.ndarray):
+            n_seq, max_pages = table.shape
+            n_tok = int(q_start[-1]) if n_tok is None else n_tok
+            max_q = max(1, int(np.diff(q_start).max())) if max_q is None else max_q
+            q_start, kv_len, table = (DeviceBuffer.from_array(np.ascontiguousarray(a, np.int32))
+                                      for a in (q_start, kv_len, table))
+        self.q_start, self.kv_len, self.table = q_start, kv_len, table
+        self.c = _PageBatchC(_addr(q_start), _addr(kv_len), _addr(table), n_seq, max_pages, n_tok, max_q)
+        self.ref = ctypes.byref(self.c)
+
+
+def rope_sections(sections, interleave: bool = False) -> np.ndarray:
+    """The axis of each rotary pair, from the number of pairs of each axis."""
+    sec = np.ascontiguousarray(sections, np.int32)
+    out = np.empty(int(sec.sum()), np.uint8)
+    check(lib.b2_rope_sections(ptr(sec), sec.size, out.size, 1 if interleave else 0, ptr(out)), "rope_sections")
+    return out
+
+
+def page_rope_store(cache: PageCache, layer: int, batch: PageBatch, n_head: int, qkv, type_x: int, q_out, type_q: int,
+                    pos, n_axes: int, axis, rope, n_pos: int, n_rot: int, style: int = ROPE_ADJACENT,
+                    stream: int | None = None) -> None:
+    """Rotary positions (one or several axes) on q and k, q to q_out, k and v to their pages."""
+    rc = lib.b2_page_rope_store(cache.ref, layer, batch.ref, n_head, _addr(qkv), type_x, _addr(q_out), type_q,
+                                _addr(pos), n_axes, _addr(axis), _addr(rope), n_pos, n_rot, style, stream)
+    if rc:
+        check(rc, "page_rope_store")
+
+
+def page_attn_workspace_bytes(cache: PageCache, batch: PageBatch, n_head: int, type_q: int) -> int:
+    v = ctypes.c_size_t()
+    check(lib.b2_page_attn_workspace_bytes(cache.ref, batch.ref, n_head, type_q, ctypes.byref(v)),
+          "page_attn_workspace_bytes")
+    return v.value
+
+
+def page_attn(cache: PageCache, layer: int, batch: PageBatch, n_head: int, q, out, type_q: int,
+              scale: float | None = None, window: int = 0, workspace: DeviceBuffer | None = None,
+              status: DeviceBuffer | None = None, stream: int | None = None) -> None:
+    """Attention of each sequence's new tokens over its pages; scale defaults to 1/sqrt(head_dim)."""
+    if scale is None:
+        scale = cache.c.head_dim ** -0.5
+    rc = lib.b2_page_attn(cache.ref, layer, batch.ref, n_head, _addr(q), _addr(out), type_q, scale, window,
+                          workspace.ptr if workspace else None, workspace.nbytes if workspace else 0,
+                          status.ptr if status else None, stream)
+    if rc:
+        check(rc, "page_attn")
+
+
+def page_copy(cache: PageCache, src, dst, stream: int | None = None) -> None:
+    """Pages src[i] -> dst[i] (host lists) in every layer."""
+    src, dst = np.ascontiguousarray(src, np.int32), np.ascontiguousarray(dst, np.int32)
+    assert src.size == dst.size
+    rc = lib.b2_page_copy(cache.ref, src.ctypes.data, dst.ctypes.data, src.size, stream)
+    if rc:
+        check(rc, "page_copy")
+
+
+def page_gather(cache: PageCache, n_seq: int, keep_start, keep, n_keep: int, old_table, new_table, max_pages: int,
+                stream: int | None = None) -> None:
+    """Kept positions of the old tables' pages gathered into the new tables' pages, in every layer."""
+    rc = lib.b2_page_gather(cache.ref, n_seq, _addr(keep_start), _addr(keep), n_keep, _addr(old_table),
+                            _addr(new_table), max_pages, stream)
+    if rc:
+        check(rc, "page_gather")
+
+
+class PagePool:
+    """Host-side bookkeeping of pages (b2_page_pool_*): which pages a
+    sequence holds and which are shared."""
+
+    def __init__(self, n_pages: int, page_size: int, n_seq: int, max_pages: int):
+        h = ctypes.c_void_p()
+        check(lib.b2_page_pool_create(n_pages, page_size, n_seq, max_pages, ctypes.byref(h)), "page_pool_create")
+        self.h = h.value
+        self.n_pages, self.page_size, self.n_seq, self.max_pages = n_pages, page_size, n_seq, max_pages
+
+    def extend(self, seq: int, n: int):
+        """Room for n more positions: (status, the page copy to make as (src, dst) or None)."""
+        a, b = ctypes.c_int32(), ctypes.c_int32()
+        rc = check(lib.b2_page_pool_extend(self.h, seq, n, ctypes.byref(a), ctypes.byref(b)), "page_pool_extend")
+        return rc, ((a.value, b.value) if a.value >= 0 else None)
+
+    def fork(self, src: int, dst: int, n: int | None = None) -> None:
+        check(lib.b2_page_pool_fork(self.h, src, dst, self.length(src) if n is None else n), "page_pool_fork")
+
+    def truncate(self, seq: int, n: int = 0) -> None:
+        check(lib.b2_page_pool_truncate(self.h, seq, n), "page_pool_truncate")
+
+    def keep(self, seq: int, keep):
+        """Keeps the given positions: (status, the table row before)."""
+        k = np.ascontiguousarray(keep, np.int32)
+        old = np.empty(self.max_pages, np.int32)
+        return check(lib.b2_page_pool_keep(self.h, seq, ptr(k), k.size, ptr(old)), "page_pool_keep"), old
+
+    def settle(self) -> None:
+        check(lib.b2_page_pool_settle(self.h), "page_pool_settle")
+
+    def defrag(self):
+        """Page copies (src, dst) that make the used pages the pool's first ones."""
+        src, dst, n = np.empty(self.n_pages, np.int32), np.empty(self.n_pages, np.int32), ctypes.c_int32()
+        check(lib.b2_page_pool_defrag(self.h, ptr(src), ptr(dst), self.n_pages, ctypes.byref(n)), "page_pool_defrag")
+        return src[:n.value].copy(), dst[:n.value].copy()
+
+    def table(self, seqs) -> np.ndarray:
+        out = np.empty((len(seqs), self.max_pages), np.int32)
+        for i, s in enumerate(seqs):
+            check(lib.b2_page_pool_table(self.h, int(s), out[i].ctypes.data, None), "page_pool_table")
+        return out
+
+    def length(self, seq: int) -> int:
+        v = ctypes.c_int32()
+        check(lib.b2_page_pool_table(self.h, seq, None, ctypes.byref(v)), "page_pool_table")
+        return v.value
+
+    def free_pages(self) -> int:
+        v = ctypes.c_int32()
+        check(lib.b2_page_pool_free_pages(self.h, ctypes.byref(v)), "page_pool_free_pages")
+        return v.value
+
+    def batch(self, seqs, new_tokens) -> PageBatch:
+        """The step in which sequence seqs[i] brings new_tokens[i] tokens (its
+        length, extended beforehand, counts them)."""
+        q_start = np.concatenate([[0], np.cumsum(new_tokens)]).astype(np.int32)
+        return PageBatch(q_start, np.array([self.length(s) for s in seqs], np.int32), self.table(seqs))
+
+    def __del__(self):
+        if getattr(self, "h", None):
+            lib.b2_page_pool_destroy(self.h)
+            self.h = None
 
 
 # ---- GGUF models and the engine -------------------------------------------------------------

@@ -3,6 +3,7 @@
 // status code with a message for b2_last_error().
 #include <string.h>
 
+#include <memory>
 #include <new>
 #include <thread>
 #include <vector>
@@ -11,6 +12,7 @@
 
 #include "b2_common.cuh"
 #include "b2_layers.hpp"
+#include "b2_pages.hpp"
 
 struct b2_qmatrix {
   b2::QMatrix m;
@@ -559,6 +561,233 @@ int b2_flag_wait(const uint64_t* flags, int n, uint64_t target, int* status, voi
   B2_CHECK_ARG(flags && status && n > 0, "flag_wait arguments");
   return launch_flag_wait(reinterpret_cast<const unsigned long long*>(flags), n, (unsigned long long)target, status,
                           as_stream(stream));
+}
+
+}  // extern "C"
+
+namespace b2 {
+namespace {
+
+int page_check(const b2_page_cache* c, bool pools = true) {
+  B2_CHECK_ARG(c && (!pools || (c->k && c->v)), "page cache pools");
+  B2_CHECK_ARG(c->n_layer > 0 && c->n_pages > 0 && c->n_kv > 0, "page cache sizes");
+  B2_CHECK_ARG(c->page_size >= 1 && c->page_size <= 256 && (c->page_size & (c->page_size - 1)) == 0,
+               "page_size must be a power of two up to 256");
+  B2_CHECK_ARG(c->head_dim > 0 && c->head_dim % 32 == 0 && c->head_dim <= 256,
+               "head_dim must be a multiple of 32 up to 256");
+  B2_CHECK_ARG(kv_type_ok(c->type_k) && kv_type_ok(c->type_v), "KV cache types must be B2_F16, B2_Q8_0 or B2_Q4_0");
+  B2_CHECK_ARG((reinterpret_cast<uintptr_t>(c->k) | reinterpret_cast<uintptr_t>(c->v)) % 16 == 0,
+               "page cache pools must be 16-byte aligned");
+  return B2_OK;
+}
+int64_t page_bytes(const b2_page_cache* c, int type) {
+  return (int64_t)c->n_kv * c->page_size * kv_row_bytes(type, c->head_dim);
+}
+PageView page_view(const b2_page_cache* c, int layer) {
+  PageView v;
+  v.k = static_cast<uint8_t*>(c->k) + layer * (c->n_pages * page_bytes(c, c->type_k));
+  v.v = static_cast<uint8_t*>(c->v) + layer * (c->n_pages * page_bytes(c, c->type_v));
+  v.n_pages = c->n_pages;
+  while ((1 << v.ps_log2) < c->page_size) ++v.ps_log2;
+  v.n_kv = c->n_kv;
+  v.type_k = c->type_k;
+  v.type_v = c->type_v;
+  v.rb_k = (int32_t)kv_row_bytes(c->type_k, c->head_dim);
+  v.rb_v = (int32_t)kv_row_bytes(c->type_v, c->head_dim);
+  return v;
+}
+int batch_check(const b2_page_cache* c, const b2_page_batch* b) {
+  B2_CHECK_ARG(b && b->q_start && b->kv_len && b->table, "page batch arrays");
+  B2_CHECK_ARG(b->n_seq > 0 && b->n_seq <= kPageMaxSeq, "a page batch holds 1..1024 sequences");
+  B2_CHECK_ARG(b->max_pages > 0 && (int64_t)b->max_pages * c->page_size <= (1 << 30), "page batch max_pages");
+  B2_CHECK_ARG(b->n_tok > 0 && b->max_q > 0 && b->max_q <= b->n_tok, "page batch tokens (1 <= max_q <= n_tok)");
+  return B2_OK;
+}
+PageSeqs page_seqs(const b2_page_batch* b) {
+  PageSeqs s;
+  s.q_start = b->q_start;
+  s.kv_len = b->kv_len;
+  s.table = b->table;
+  s.n_seq = b->n_seq;
+  s.max_pages = b->max_pages;
+  s.n_tok = b->n_tok;
+  s.max_q = b->max_q;
+  return s;
+}
+bool aligned16(const void* p) { return reinterpret_cast<uintptr_t>(p) % 16 == 0; }
+bool act_type_ok(int t) { return t == B2_F32 || t == B2_F16; }
+
+int page_attn_args(const b2_page_cache* c, const b2_page_batch* b, int32_t n_head, int type_q, PageAttnArgs* a) {
+  int rc = page_check(c);
+  if (rc == B2_OK) rc = batch_check(c, b);
+  if (rc != B2_OK) return rc;
+  B2_CHECK_ARG(n_head > 0 && n_head % c->n_kv == 0, "n_head must be a multiple of n_kv");
+  B2_CHECK_ARG(act_type_ok(type_q), "page_attn: q and out are B2_F32 or B2_F16");
+  B2_CHECK_ARG((int64_t)b->n_tok * n_head < (1 << 30), "page_attn: n_tok·n_head below 2^30");
+  if (c->head_dim != 64 && c->head_dim != 96 && c->head_dim != 128 && c->head_dim != 256) {
+    set_error("page_attn: head_dim %d (64, 96, 128 and 256 are supported)", c->head_dim);
+    return B2_ERR_UNSUPPORTED;
+  }
+  a->b = page_seqs(b);
+  a->n_head = n_head;
+  a->hd = c->head_dim;
+  a->type_q = type_q;
+  return B2_OK;
+}
+
+}  // namespace
+}  // namespace b2
+
+extern "C" {
+
+int b2_page_cache_bytes(const b2_page_cache* c, size_t* bytes_k, size_t* bytes_v) {
+  B2_CHECK_ARG(c && bytes_k && bytes_v, "page_cache_bytes arguments");
+  const int rc = page_check(c, false);   // the pools need not exist yet
+  if (rc != B2_OK) return rc;
+  *bytes_k = (size_t)c->n_layer * c->n_pages * page_bytes(c, c->type_k);
+  *bytes_v = (size_t)c->n_layer * c->n_pages * page_bytes(c, c->type_v);
+  return B2_OK;
+}
+
+int b2_page_rope_store(const b2_page_cache* cache, int32_t layer, const b2_page_batch* batch, int32_t n_head,
+                       const void* qkv, int type_x, void* q_out, int type_q, const int32_t* pos, int32_t n_axes,
+                       const uint8_t* axis, const float* rope, int32_t n_pos, int32_t n_rot, int style, void* stream) {
+  int rc = page_check(cache);
+  if (rc == B2_OK) rc = batch_check(cache, batch);
+  if (rc != B2_OK) return rc;
+  B2_CHECK_ARG(layer >= 0 && layer < cache->n_layer, "layer");
+  B2_CHECK_ARG(qkv && q_out && pos && rope && n_head > 0, "page_rope_store arguments");
+  B2_CHECK_ARG(aligned16(qkv) && aligned16(q_out) && aligned16(rope), "page_rope_store arrays must be 16-byte aligned");
+  B2_CHECK_ARG(act_type_ok(type_x) && act_type_ok(type_q), "page_rope_store: qkv and q_out are B2_F32 or B2_F16");
+  B2_CHECK_ARG(n_axes >= 1 && n_axes <= 8 && (axis || n_axes == 1), "page_rope_store: 1..8 axes, with an axis map");
+  B2_CHECK_ARG(n_pos > 0 && n_rot > 0 && n_rot % 8 == 0 && n_rot <= cache->head_dim,
+               "page_rope_store: n_rot a multiple of 8 up to head_dim");
+  B2_CHECK_ARG(style == B2_ROPE_ADJACENT || style == B2_ROPE_HALVES, "page_rope_store: style");
+  RopeStoreArgs a;
+  a.c = page_view(cache, layer);
+  a.b = page_seqs(batch);
+  a.x = qkv;
+  a.q = q_out;
+  a.pos = pos;
+  a.axis = axis;
+  a.rope = rope;
+  a.n_head = n_head;
+  a.hd = cache->head_dim;
+  a.n_axes = n_axes;
+  a.n_pos = n_pos;
+  a.rot = n_rot;
+  a.style = style;
+  a.type_x = type_x;
+  a.type_q = type_q;
+  return launch_page_rope_store(a, as_stream(stream));
+}
+
+int b2_rope_sections(const int32_t* sections, int32_t n_axes, int32_t n_pairs, int interleave, uint8_t* out) {
+  B2_CHECK_ARG(sections && out && n_axes >= 1 && n_axes <= 8 && n_pairs >= 1, "rope_sections arguments");
+  int64_t sum = 0;
+  int32_t left[8];
+  for (int a = 0; a < n_axes; ++a) {
+    B2_CHECK_ARG(sections[a] >= 0, "rope_sections: negative section");
+    sum += left[a] = sections[a];
+  }
+  B2_CHECK_ARG(sum == n_pairs, "rope_sections: the sections must add up to n_pairs");
+  int n = 0;
+  if (interleave) {
+    for (int a = 0; n < n_pairs; a = (a + 1) % n_axes)
+      if (left[a] > 0) {
+        --left[a];
+        out[n++] = (uint8_t)a;
+      }
+  } else {
+    for (int a = 0; a < n_axes; ++a)
+      for (int i = 0; i < sections[a]; ++i) out[n++] = (uint8_t)a;
+  }
+  return B2_OK;
+}
+
+int b2_page_attn_workspace_bytes(const b2_page_cache* cache, const b2_page_batch* batch, int32_t n_head, int type_q,
+                                 size_t* bytes) {
+  B2_CHECK_ARG(bytes, "bytes");
+  PageAttnArgs a;
+  const int rc = page_attn_args(cache, batch, n_head, type_q, &a);
+  if (rc != B2_OK) return rc;
+  a.c = page_view(cache, 0);
+  *bytes = page_attn_workspace(a);
+  return B2_OK;
+}
+
+int b2_page_attn(const b2_page_cache* cache, int32_t layer, const b2_page_batch* batch, int32_t n_head, const void* q,
+                 void* out, int type_q, float scale, int32_t window, void* workspace, size_t workspace_bytes,
+                 int* status, void* stream) {
+  PageAttnArgs a;
+  int rc = page_attn_args(cache, batch, n_head, type_q, &a);
+  if (rc != B2_OK) return rc;
+  B2_CHECK_ARG(layer >= 0 && layer < cache->n_layer, "layer");
+  B2_CHECK_ARG(q && out && aligned16(q) && aligned16(out) && aligned16(workspace),
+               "page_attn: q, out and workspace 16-byte aligned");
+  B2_CHECK_ARG(scale == scale && scale - scale == 0.0f, "page_attn: scale must be finite");
+  a.c = page_view(cache, layer);
+  a.q = q;
+  a.out = out;
+  a.scale = scale;
+  a.window = window > 0 ? window : 0;
+  a.status = status;
+  const size_t need = page_attn_workspace(a);
+  B2_CHECK_ARG(!workspace || workspace_bytes >= need, "page_attn: workspace below b2_page_attn_workspace_bytes");
+  cudaStream_t s = as_stream(stream);
+  a.ws = static_cast<uint8_t*>(workspace);
+  if (!workspace) {
+    void* scratch = nullptr;
+    B2_CUDA_TRY(cudaMallocAsync(&scratch, need, s));
+    a.ws = static_cast<uint8_t*>(scratch);
+  }
+  rc = launch_page_attn(a, s);
+  if (!workspace) cudaFreeAsync(a.ws, s);
+  return rc;
+}
+
+int b2_page_copy(const b2_page_cache* cache, const int32_t* src, const int32_t* dst, int32_t n, void* stream) {
+  int rc = page_check(cache);
+  if (rc != B2_OK) return rc;
+  B2_CHECK_ARG(n >= 0 && (n == 0 || (src && dst)), "page_copy arguments");
+  if (n == 0) return B2_OK;
+  B2_CHECK_ARG(n <= cache->n_pages, "page_copy: more copies than pages");
+  B2_CHECK_ARG(cache->n_layer <= 32767, "page_copy: layers");
+  std::unique_ptr<uint8_t[]> seen(new (std::nothrow) uint8_t[cache->n_pages]());
+  if (!seen) {
+    set_error("page_copy: out of host memory");
+    return B2_ERR_OOM;
+  }
+  for (int i = 0; i < n; ++i) {
+    B2_CHECK_ARG(src[i] >= 0 && src[i] < cache->n_pages && dst[i] >= 0 && dst[i] < cache->n_pages,
+                 "page_copy: page outside the pool");
+    B2_CHECK_ARG(!(seen[dst[i]] & 1), "page_copy: a page is written twice");
+    seen[dst[i]] |= 1;
+    seen[src[i]] |= 2;
+  }
+  for (int i = 0; i < n; ++i) B2_CHECK_ARG(seen[dst[i]] != 3, "page_copy: a page is both read and written");
+  return launch_page_copy(static_cast<uint8_t*>(cache->k), static_cast<uint8_t*>(cache->v), cache->n_layer,
+                          cache->n_pages, page_bytes(cache, cache->type_k), page_bytes(cache, cache->type_v), src, dst,
+                          n, as_stream(stream));
+}
+
+int b2_page_gather(const b2_page_cache* cache, int32_t n_seq, const int32_t* keep_start, const int32_t* keep,
+                   int32_t n_keep, const int32_t* old_table, const int32_t* new_table, int32_t max_pages,
+                   void* stream) {
+  int rc = page_check(cache);
+  if (rc != B2_OK) return rc;
+  B2_CHECK_ARG(n_keep >= 0 && n_seq > 0 && keep_start && old_table && new_table && (n_keep == 0 || keep),
+               "page_gather arguments");
+  B2_CHECK_ARG(max_pages > 0 && (int64_t)max_pages * cache->page_size <= (1 << 30), "page_gather: max_pages");
+  B2_CHECK_ARG(cache->n_layer <= 32767, "page_gather: layers");
+  if (n_keep == 0) return B2_OK;
+  PageSeqs d;
+  d.q_start = keep_start;
+  d.table = new_table;
+  d.n_seq = n_seq;
+  d.max_pages = max_pages;
+  d.n_tok = n_keep;
+  return launch_page_gather(page_view(cache, 0), cache->n_layer, d, keep, old_table, as_stream(stream));
 }
 
 }  // extern "C"

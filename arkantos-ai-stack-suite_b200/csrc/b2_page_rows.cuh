@@ -1,0 +1,654 @@
+// Attention of few rows over the paged cache: single tokens, short chunks,
+// and every cache type and head size (b2_page_rows_*.cu instantiate it).
+//
+//   o_r = Σ_t e^{s_rt − m_r} v_t / Σ_t e^{s_rt − m_r},   s_rt = scale · q_r·k_t
+//
+// in one pass over the positions with the running maximum m and sum of each
+// row.  What bounds a decode step is the read of K and V; the rows of one kv
+// head (its G query heads) share that read, and their products go to the
+// tensor pipe through mma.sync m16n8k16: with at most 16 rows per kv head a
+// tcgen05 tile of 128 rows would be 90 % padding and its operands would still
+// pass through shared memory.
+//
+// Exactness.  Cache values enter the products exactly: fp16 as they are,
+// Q8_0 / Q4_0 as their integer codes in fp16, the block scale applied in fp32
+// to K's block sums and to p for V (a row of K or V is never rounded to
+// fp16).  In the SPLIT form a row of the 16-row operand is a pair: rows 0-7
+// hold the high fp16 part of q (scaled in fp32), rows 8-15 the remainder, and
+// likewise for p, so fp32 queries keep 22 bits and the output is good to
+// fp32 accuracy at no further cost while a tile has 8 rows or fewer.  The
+// FULL form (fp16 queries and outputs) rounds p once to fp16, the size of
+// error the fp16 output has by itself.  Accumulators, maxima and sums are
+// fp32.
+//
+// Layout.  A unit is 64 positions.  cp.async brings its K and V rows into a
+// ring of stages, 16 bytes a thread, row by row through the page table, so a
+// page may end anywhere; positions the tile does not attend to and table
+// entries outside the pool are filled with zeros.  Quantized rows land as stored and
+// are unpacked to fp16 codes by the CTA.  WM = 1: the 4 warps take 16
+// positions each of the one 16-row operand and their results are joined at
+// the end of a tile; WM = 4: each warp has its own 16-row operand and runs
+// over all 64 positions.
+#pragma once
+
+#include <atomic>
+
+#include "b2_page_work.cuh"
+
+namespace b2 {
+
+struct PageRowsArgs {
+  PageView c;
+  PageWork w;
+  const void* q;
+  void* out;
+  int n_head, q_f32;
+  float scale_log2;          // scale · log2(e)
+  SplitTile* split;
+  float* slots;
+};
+
+constexpr int kRowsThreads = 128, kRowsBk = 64, kMaxDevices = 64;
+
+__device__ __forceinline__ void cp_async16(uint32_t dst, const void* src, bool on) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(on ? 16 : 0) : "memory");
+}
+__device__ __forceinline__ void cp_async_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+template <int N>
+__device__ __forceinline__ void cp_async_wait() {
+  asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory");
+}
+__device__ __forceinline__ void ldsm4(uint32_t a, uint32_t (&r)[4]) {
+  asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0,%1,%2,%3}, [%4];"
+               : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3])
+               : "r"(a)
+               : "memory");
+}
+__device__ __forceinline__ void ldsm4_t(uint32_t a, uint32_t (&r)[4]) {
+  asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0,%1,%2,%3}, [%4];"
+               : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3])
+               : "r"(a)
+               : "memory");
+}
+__device__ __forceinline__ void mma16816(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+  asm volatile(
+      "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+      : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+      : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+__device__ __forceinline__ float ex2(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+__device__ __forceinline__ uint32_t h2(float lo, float hi) {
+  const __half2 v = __floats2half2_rn(lo, hi);
+  return *reinterpret_cast<const uint32_t*>(&v);
+}
+// (lo, hi) as fp16 pairs: the rounded values and what the rounding left.
+__device__ __forceinline__ void h2_split(float lo, float hi, uint32_t& head, uint32_t& rest) {
+  const __half2 v = __floats2half2_rn(lo, hi);
+  const float2 f = __half22float2(v);
+  head = *reinterpret_cast<const uint32_t*>(&v);
+  rest = h2(lo - f.x, hi - f.y);
+}
+
+// Bytes 0-3 of w (signed codes) as four exact fp16 values: a byte b + 128 in
+// the low bits of 0x6400 is 1024 + b + 128.
+__device__ __forceinline__ void s8x4_to_h2(uint32_t w, uint32_t& a, uint32_t& b) {
+  w ^= 0x80808080u;
+  const uint32_t x = __byte_perm(w, 0x64646464u, 0x4140), y = __byte_perm(w, 0x64646464u, 0x4342);
+  const __half2 off = __halves2half2(__ushort_as_half(0x6480), __ushort_as_half(0x6480));   // 1152
+  const __half2 p = __hsub2(*reinterpret_cast<const __half2*>(&x), off);
+  const __half2 q = __hsub2(*reinterpret_cast<const __half2*>(&y), off);
+  a = *reinterpret_cast<const uint32_t*>(&p);
+  b = *reinterpret_cast<const uint32_t*>(&q);
+}
+
+// p is carried times 2^offset so that its fp16 parts stay normal; the sum
+// carries the same factor.  With a quantized V the operand is p·d, d the
+// block scale: |v| <= 65504 bounds d by 516 (Q8_0) and 8188 (Q4_0), which
+// leaves room for 2^6 and 2^3.
+__host__ __device__ inline float p_offset(int type_v) { return type_v == B2_F16 ? 10.f : type_v == B2_Q8_0 ? 6.f : 3.f; }
+
+template <int HD>
+struct RowsSmem {
+  static constexpr int pitch = HD * 2 + 16;                  // ldmatrix rows 16 bytes apart modulo 128
+  static constexpr int tile = kRowsBk * pitch;               // an fp16 (or unpacked) operand
+  static constexpr int scales = (HD / 32) * kRowsBk * 4;
+  __host__ __device__ static int raw(int rb) { return kRowsBk * rb; }
+};
+template <int HD, bool KQ, bool VQ>
+__host__ __device__ inline int rows_stage_bytes(int rb_k, int rb_v) {
+  return (KQ ? RowsSmem<HD>::raw(rb_k) : RowsSmem<HD>::tile) + (VQ ? RowsSmem<HD>::raw(rb_v) : RowsSmem<HD>::tile);
+}
+template <int HD, bool KQ, bool VQ>
+__host__ __device__ inline int rows_conv_bytes() {
+  return (KQ ? RowsSmem<HD>::tile + RowsSmem<HD>::scales : 0) + (VQ ? RowsSmem<HD>::tile + RowsSmem<HD>::scales : 0);
+}
+
+template <int HD, bool KQ, bool VQ, bool SPLIT, int WM>
+__global__ void __launch_bounds__(kRowsThreads) page_rows_kernel(const PageRowsArgs a, int stages) {
+  constexpr int WK = 4 / WM;                   // warps along the positions
+  constexpr int KEYS = kRowsBk / WK;           // positions of a warp in a unit
+  constexpr int NC = WM == 1 ? 16 : 32;        // positions per softmax step
+  constexpr int NT = NC / 8, KS = HD / 16, NB = HD / 32, DT = HD / 8;
+  constexpr int WROWS = SPLIT ? 8 : 16;        // rows of a warp's operand
+  constexpr int PITCH = RowsSmem<HD>::pitch;
+  extern __shared__ __align__(128) uint8_t smem[];
+  pdl_wait();
+  pdl_launch_dependents();
+
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  const int wm = WM == 1 ? 0 : warp, wk = WM == 1 ? warp : 0;
+  const int g = lane >> 2, j = lane & 3;
+  const PageView& c = a.c;
+  const PageWork& w = a.w;
+
+  Share sh;
+  int* sums = reinterpret_cast<int*>(smem);
+  const bool have = find_share(w, blockIdx.x, gridDim.x, sums, sh);
+  SplitTile rec = {};
+  rec.last = -1;
+  if (!have) {
+    if (tid == 0) a.split[blockIdx.x] = rec;
+    return;
+  }
+  __syncthreads();   // sums are read; the stages take their place
+
+  const int stage_bytes = rows_stage_bytes<HD, KQ, VQ>(c.rb_k, c.rb_v);
+  const int k_bytes = KQ ? RowsSmem<HD>::raw(c.rb_k) : RowsSmem<HD>::tile;
+  uint8_t* ring = smem;
+  uint8_t* conv = smem + stages * stage_bytes;
+  uint8_t* conv_k = conv;
+  float* scale_k = reinterpret_cast<float*>(conv + RowsSmem<HD>::tile);
+  uint8_t* conv_v = conv + (KQ ? RowsSmem<HD>::tile + RowsSmem<HD>::scales : 0);
+  float* scale_v = reinterpret_cast<float*>(conv_v + RowsSmem<HD>::tile);
+  const float off = p_offset(c.type_v);
+
+  bool first_tile = true;
+  while (sh.u < sh.u_end) {
+    const TileAt at = sh.at;
+    const int u_lo = sh.off, u_hi = (int)(sh.u_end - sh.u < at.units - u_lo ? u_lo + (sh.u_end - sh.u) : at.units);
+    const int row0 = at.t * w.rows;
+    const int rows = min(w.rows, at.rows_total - row0);
+
+    // ---- queries: registers, scaled in fp32 and split, or as they are ----
+    uint32_t qf[KS][4];
+    int p0 = -1, p1 = -1;   // positions of rows g and g + 8 (-1: sees nothing)
+    {
+      const int r = wm * WROWS + g, r1 = r + 8;
+      const bool on0 = r < rows, on1 = !SPLIT && r1 < rows;
+      const int rr0 = row0 + (on0 ? r : 0), rr1 = row0 + (on1 ? r1 : 0);
+      if (on0) p0 = at.first + rr0 / w.G;
+      if (on1) p1 = at.first + rr1 / w.G;
+      const int64_t e0 = ((int64_t)(at.q0 + rr0 / w.G) * a.n_head + at.h * w.G + rr0 % w.G) * HD;
+      const int64_t e1 = ((int64_t)(at.q0 + rr1 / w.G) * a.n_head + at.h * w.G + rr1 % w.G) * HD;
+#pragma unroll
+      for (int ks = 0; ks < KS; ++ks) {
+        const int d0 = ks * 16 + 2 * j, d1 = d0 + 8;
+        if constexpr (SPLIT) {
+          float2 x = make_float2(0.f, 0.f), y = x;
+          if (on0) {
+            if (a.q_f32) {
+              const float* q = static_cast<const float*>(a.q) + e0;
+              x = *reinterpret_cast<const float2*>(q + d0);
+              y = *reinterpret_cast<const float2*>(q + d1);
+            } else {
+              const __half* q = static_cast<const __half*>(a.q) + e0;
+              x = __half22float2(*reinterpret_cast<const __half2*>(q + d0));
+              y = __half22float2(*reinterpret_cast<const __half2*>(q + d1));
+            }
+          }
+          h2_split(x.x * a.scale_log2, x.y * a.scale_log2, qf[ks][0], qf[ks][1]);
+          h2_split(y.x * a.scale_log2, y.y * a.scale_log2, qf[ks][2], qf[ks][3]);
+        } else {
+          const __half* q = static_cast<const __half*>(a.q);
+          qf[ks][0] = on0 ? *reinterpret_cast<const uint32_t*>(q + e0 + d0) : 0u;
+          qf[ks][1] = on1 ? *reinterpret_cast<const uint32_t*>(q + e1 + d0) : 0u;
+          qf[ks][2] = on0 ? *reinterpret_cast<const uint32_t*>(q + e0 + d1) : 0u;
+          qf[ks][3] = on1 ? *reinterpret_cast<const uint32_t*>(q + e1 + d1) : 0u;
+        }
+      }
+    }
+
+    float o[DT][4];
+#pragma unroll
+    for (int d = 0; d < DT; ++d)
+#pragma unroll
+      for (int e = 0; e < 4; ++e) o[d][e] = 0.f;
+    float m0 = -INFINITY, m1 = -INFINITY, l0 = 0.f, l1 = 0.f;   // rows g and g + 8 (SPLIT: row g)
+
+    // ---- staging ----
+    auto stage_in = [&](int u) {
+      const int key0 = (at.lo_unit + u) * kRowsBk;
+      uint8_t* st = ring + (u % stages) * stage_bytes;
+      const uint32_t sk = smem_u32(st), sv = smem_u32(st + k_bytes);
+      auto rows_in = [&](uint32_t dst, const uint8_t* pool, int rb, int pitch) {
+        const int cpr = rb >> 4;
+        for (int i = tid; i < kRowsBk * cpr; i += kRowsThreads) {
+          const int key = i / cpr, ch = i - key * cpr, p = key0 + key;
+          const int64_t row = p >= at.lo && p < at.hi ? page_row(w.b, c, at.s, at.h, p) : -1;
+          cp_async16(dst + key * pitch + ch * 16, pool + (row < 0 ? 0 : row * rb + ch * 16), row >= 0);
+        }
+      };
+      rows_in(sk, c.k, c.rb_k, KQ ? c.rb_k : PITCH);
+      rows_in(sv, c.v, c.rb_v, VQ ? c.rb_v : PITCH);
+    };
+    // Quantized rows of a stage -> fp16 codes and fp32 scales [block][position].
+    auto unpack = [&](const uint8_t* raw, int type, int rb, uint8_t* dst, float* sc) {
+      const int cb = type == B2_Q8_0 ? HD : HD / 2, cpr = cb / 16;
+      for (int i = tid; i < kRowsBk * cpr; i += kRowsThreads) {
+        const int key = i / cpr, ch = i - key * cpr;
+        const uint4 x = *reinterpret_cast<const uint4*>(raw + key * rb + ch * 16);
+        uint32_t h[8];
+        if (type == B2_Q8_0) {
+          s8x4_to_h2(x.x, h[0], h[1]);
+          s8x4_to_h2(x.y, h[2], h[3]);
+          s8x4_to_h2(x.z, h[4], h[5]);
+          s8x4_to_h2(x.w, h[6], h[7]);
+          uint4* t = reinterpret_cast<uint4*>(dst + key * PITCH + ch * 32);
+          t[0] = make_uint4(h[0], h[1], h[2], h[3]);
+          t[1] = make_uint4(h[4], h[5], h[6], h[7]);
+        } else {
+          uint4* t = reinterpret_cast<uint4*>(dst + key * PITCH + ch * 64);
+          const uint32_t lo[4] = {(uint32_t)nib_lo_s8(x.x), (uint32_t)nib_lo_s8(x.y), (uint32_t)nib_lo_s8(x.z),
+                                  (uint32_t)nib_lo_s8(x.w)};
+          const uint32_t hi[4] = {(uint32_t)nib_hi_s8(x.x), (uint32_t)nib_hi_s8(x.y), (uint32_t)nib_hi_s8(x.z),
+                                  (uint32_t)nib_hi_s8(x.w)};
+          s8x4_to_h2(lo[0], h[0], h[1]);
+          s8x4_to_h2(lo[1], h[2], h[3]);
+          s8x4_to_h2(lo[2], h[4], h[5]);
+          s8x4_to_h2(lo[3], h[6], h[7]);
+          t[0] = make_uint4(h[0], h[1], h[2], h[3]);
+          t[1] = make_uint4(h[4], h[5], h[6], h[7]);
+          s8x4_to_h2(hi[0], h[0], h[1]);
+          s8x4_to_h2(hi[1], h[2], h[3]);
+          s8x4_to_h2(hi[2], h[4], h[5]);
+          s8x4_to_h2(hi[3], h[6], h[7]);
+          t[2] = make_uint4(h[0], h[1], h[2], h[3]);
+          t[3] = make_uint4(h[4], h[5], h[6], h[7]);
+        }
+      }
+      for (int i = tid; i < kRowsBk * NB; i += kRowsThreads) {
+        const int b = i / kRowsBk, key = i - b * kRowsBk;
+        sc[i] = h2f(*reinterpret_cast<const uint16_t*>(raw + key * rb + cb + 2 * b));
+      }
+    };
+
+    for (int n = 0; n < stages - 1; ++n) {
+      if (u_lo + n < u_hi) stage_in(u_lo + n);
+      cp_async_commit();
+    }
+    // positions every live row sees need no mask
+    const int p_min = at.first + row0 / w.G, p_max = at.first + (row0 + rows - 1) / w.G;
+    for (int u = u_lo; u < u_hi; ++u) {
+      // all but the newest stages - 2 groups have landed
+      if (stages == 4) cp_async_wait<2>(); else if (stages == 3) cp_async_wait<1>(); else cp_async_wait<0>();
+      __syncthreads();   // unit u is here; everyone is done with unit u - 1, whose stage the next copy takes
+      if (u + stages - 1 < u_hi) stage_in(u + stages - 1);
+      cp_async_commit();
+      uint8_t* st = ring + (u % stages) * stage_bytes;
+      const int key0 = (at.lo_unit + u) * kRowsBk;
+      const bool edge = key0 + kRowsBk > at.hi || key0 + kRowsBk - 1 > p_min ||
+                        (w.window > 0 && key0 <= p_max - w.window);
+      if constexpr (KQ) unpack(st, c.type_k, c.rb_k, conv_k, scale_k);
+      if constexpr (VQ) unpack(st + k_bytes, c.type_v, c.rb_v, conv_v, scale_v);
+      uint8_t* Vt = VQ ? conv_v : st + k_bytes;
+      const uint32_t ks_base = smem_u32(KQ ? conv_k : st), vs_base = smem_u32(Vt);
+      bool bad = false;
+      if (edge && p_max > p_min) {
+        // A value that some row must not see can still reach it as 0·v when v
+        // is infinite or NaN.  Such values are taken out of the operand here
+        // and added below to the rows that do see them.
+        if constexpr (VQ) __syncthreads();   // the scales are written
+        int found = 0;
+        if constexpr (VQ) {
+          for (int i = tid; i < kRowsBk * NB; i += kRowsThreads)
+            if (!(fabsf(scale_v[i]) <= 65504.f)) {
+              scale_v[i] = 0.f;
+              found = 1;
+            }
+        } else {
+          for (int i = tid; i < kRowsBk * (HD / 2); i += kRowsThreads) {
+            const int key = i / (HD / 2), x = i - key * (HD / 2);
+            uint32_t* p = reinterpret_cast<uint32_t*>(Vt + key * PITCH) + x;
+            uint32_t v = *p;
+            if ((v & 0x7C00u) == 0x7C00u) v &= 0xFFFF0000u;
+            if ((v & 0x7C000000u) == 0x7C000000u) v &= 0xFFFFu;
+            if (v != *p) {
+              *p = v;
+              found = 1;
+            }
+          }
+        }
+        bad = __syncthreads_or(found);
+      } else if constexpr (KQ || VQ) {
+        __syncthreads();
+      }
+
+      for (int c0 = 0; c0 < KEYS; c0 += NC) {
+        const int kw = wk * KEYS + c0;   // first position of this step within the unit
+        // ---- S = Q·K^T ----
+        float s[NT][4];
+#pragma unroll
+        for (int n = 0; n < NT; ++n) {
+          float acc[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+          for (int b = 0; b < NB; ++b) {
+            uint32_t kf[4];   // 8 positions x 32 dims
+            ldsm4(ks_base + (kw + n * 8 + (lane & 7)) * PITCH + b * 64 + (lane >> 3) * 16, kf);
+            if constexpr (KQ) {
+              float t[4] = {0.f, 0.f, 0.f, 0.f};
+              mma16816(t, qf[2 * b], kf[0], kf[1]);
+              mma16816(t, qf[2 * b + 1], kf[2], kf[3]);
+              const float2 d = *reinterpret_cast<const float2*>(scale_k + b * kRowsBk + kw + n * 8 + 2 * j);
+              acc[0] = fmaf(t[0], d.x, acc[0]);
+              acc[1] = fmaf(t[1], d.y, acc[1]);
+              acc[2] = fmaf(t[2], d.x, acc[2]);
+              acc[3] = fmaf(t[3], d.y, acc[3]);
+            } else {
+              mma16816(acc, qf[2 * b], kf[0], kf[1]);
+              mma16816(acc, qf[2 * b + 1], kf[2], kf[3]);
+            }
+          }
+          if constexpr (SPLIT) {
+            s[n][0] = acc[0] + acc[2];
+            s[n][1] = acc[1] + acc[3];
+            s[n][2] = s[n][3] = 0.f;
+          } else {
+#pragma unroll
+            for (int e = 0; e < 4; ++e) s[n][e] = acc[e] * a.scale_log2;
+          }
+          if (edge) {
+            const int t0 = key0 + kw + n * 8 + 2 * j;
+#pragma unroll
+            for (int e = 0; e < (SPLIT ? 2 : 4); ++e) {
+              const int t = t0 + (e & 1), p = e < 2 ? p0 : p1;
+              if (t > p || t >= at.hi || (w.window > 0 && t <= p - w.window)) s[n][e] = -INFINITY;
+            }
+          }
+        }
+        // ---- running maximum and sum ----
+        float n0 = m0, n1 = m1;
+#pragma unroll
+        for (int n = 0; n < NT; ++n) {
+          n0 = fmaxf(n0, fmaxf(s[n][0], s[n][1]));
+          if constexpr (!SPLIT) n1 = fmaxf(n1, fmaxf(s[n][2], s[n][3]));
+        }
+#pragma unroll
+        for (int x = 1; x < 4; x <<= 1) {
+          n0 = fmaxf(n0, __shfl_xor_sync(0xffffffffu, n0, x));
+          if constexpr (!SPLIT) n1 = fmaxf(n1, __shfl_xor_sync(0xffffffffu, n1, x));
+        }
+        // a row that has seen nothing keeps m = -inf; its exponents are taken from 0
+        const float r0 = (n0 == -INFINITY ? 0.f : n0) - off, r1 = (n1 == -INFINITY ? 0.f : n1) - off;
+        if (n0 != m0 || (!SPLIT && n1 != m1)) {
+          const float f0 = m0 == -INFINITY ? 0.f : ex2(m0 - n0), f1 = m1 == -INFINITY ? 0.f : ex2(m1 - n1);
+          l0 *= f0;
+          l1 *= f1;
+#pragma unroll
+          for (int d = 0; d < DT; ++d) {
+            o[d][0] *= f0;
+            o[d][1] *= f0;
+            o[d][2] *= SPLIT ? f0 : f1;
+            o[d][3] *= SPLIT ? f0 : f1;
+          }
+          m0 = n0;
+          m1 = n1;
+        }
+#pragma unroll
+        for (int n = 0; n < NT; ++n) {
+          s[n][0] = ex2(s[n][0] - r0);
+          s[n][1] = ex2(s[n][1] - r0);
+          l0 += s[n][0] + s[n][1];
+          if constexpr (!SPLIT) {
+            s[n][2] = ex2(s[n][2] - r1);
+            s[n][3] = ex2(s[n][3] - r1);
+            l1 += s[n][2] + s[n][3];
+          }
+        }
+        // ---- O += P·V ----
+#pragma unroll
+        for (int k = 0; k < NC / 16; ++k) {
+          uint32_t pf[4];
+          const float* x = s[2 * k];
+          const float* y = s[2 * k + 1];
+          auto operand = [&](float a0, float a1, float b0, float b1) {   // scales of positions 2j, 2j+1, 2j+8, 2j+9
+            if constexpr (SPLIT) {
+              h2_split(x[0] * a0, x[1] * a1, pf[0], pf[1]);
+              h2_split(y[0] * b0, y[1] * b1, pf[2], pf[3]);
+            } else {
+              pf[0] = h2(x[0] * a0, x[1] * a1);
+              pf[1] = h2(x[2] * a0, x[3] * a1);
+              pf[2] = h2(y[0] * b0, y[1] * b1);
+              pf[3] = h2(y[2] * b0, y[3] * b1);
+            }
+          };
+          if constexpr (!VQ) operand(1.f, 1.f, 1.f, 1.f);
+#pragma unroll
+          for (int b = 0; b < NB; ++b) {
+            if constexpr (VQ) {
+              const float* sc = scale_v + b * kRowsBk + kw + k * 16 + 2 * j;
+              const float2 da = *reinterpret_cast<const float2*>(sc), db = *reinterpret_cast<const float2*>(sc + 8);
+              operand(da.x, da.y, db.x, db.y);
+            }
+#pragma unroll
+            for (int d = 0; d < 2; ++d) {
+              uint32_t vf[4];   // 16 positions x 16 dims
+              ldsm4_t(vs_base + (kw + k * 16 + (lane & 15)) * PITCH + (b * 32 + d * 16 + (lane >> 4) * 8) * 2, vf);
+              mma16816(o[b * 4 + 2 * d], pf, vf[0], vf[1]);
+              mma16816(o[b * 4 + 2 * d + 1], pf, vf[2], vf[3]);
+            }
+          }
+        }
+      }
+      if (bad) {
+        // infinite and NaN values of V, to the rows that see them (their
+        // weight is positive, so the value itself decides the sum)
+        for (int key = wk * KEYS; key < (wk + 1) * KEYS; ++key) {
+          const int t = key0 + key;
+          if (t < at.lo || t >= at.hi) continue;
+          const int64_t row = page_row(w.b, c, at.s, at.h, t);
+          if (row < 0) continue;
+          const uint8_t* vr = c.v + row * c.rb_v;
+          const bool see0 = t <= p0 && !(w.window > 0 && t <= p0 - w.window);
+          const bool see1 = !SPLIT && t <= p1 && !(w.window > 0 && t <= p1 - w.window);
+#pragma unroll
+          for (int d = 0; d < DT; ++d)
+#pragma unroll
+            for (int e = 0; e < 2; ++e) {
+              const int i = d * 8 + 2 * j + e;
+              float v;
+              if constexpr (VQ) {
+                const float sc = h2f(*reinterpret_cast<const uint16_t*>(
+                    vr + (c.type_v == B2_Q8_0 ? HD : HD / 2) + 2 * (i >> 5)));
+                const int code = c.type_v == B2_Q8_0
+                                     ? (int)(int8_t)vr[i]
+                                     : ((vr[(i >> 5) * 16 + (i & 15)] >> ((i & 16) ? 4 : 0)) & 15) - 8;
+                v = (float)code * sc;
+              } else {
+                v = h2f(reinterpret_cast<const uint16_t*>(vr)[i]);
+              }
+              if (fabsf(v) <= 3.4e38f) continue;
+              if (see0) o[d][e] += v;
+              if (see1) o[d][2 + e] += v;
+            }
+        }
+      }
+    }
+    cp_async_wait<0>();
+
+    // ---- join the lanes' sums, and for WM = 1 the warps ----
+#pragma unroll
+    for (int x = 1; x < 4; x <<= 1) {
+      l0 += __shfl_xor_sync(0xffffffffu, l0, x);
+      if constexpr (!SPLIT) l1 += __shfl_xor_sync(0xffffffffu, l1, x);
+    }
+    if constexpr (SPLIT) {
+#pragma unroll
+      for (int d = 0; d < DT; ++d) {
+        o[d][0] += o[d][2];
+        o[d][1] += o[d][3];
+      }
+    }
+    const bool whole = u_lo == 0 && u_hi == at.units;
+    const int slot = u_lo == 0 && !first_tile ? 2 * blockIdx.x + 1 : 2 * blockIdx.x;
+    float* part = a.slots + (int64_t)slot * slot_floats(w.rows, HD);
+    float* part_ml = part + w.rows * HD;
+
+    auto out_ptr = [&](int r) -> int64_t {
+      const int rr = row0 + r;
+      return ((int64_t)(at.q0 + rr / w.G) * a.n_head + at.h * w.G + rr % w.G) * HD;
+    };
+    auto put2 = [&](int r, int d, float x, float y) {   // values d, d + 1 of row r, normalized, or a partial result
+      if (!whole) {
+        *reinterpret_cast<float2*>(part + r * HD + d) = make_float2(x, y);
+      } else if (a.q_f32) {
+        *reinterpret_cast<float2*>(static_cast<float*>(a.out) + out_ptr(r) + d) = make_float2(x, y);
+      } else {
+        *reinterpret_cast<uint32_t*>(static_cast<__half*>(a.out) + out_ptr(r) + d) = h2(x, y);
+      }
+    };
+
+    if constexpr (WM == 1) {
+      // [4 warps][16] (m, l), then [4 warps][WROWS][HD] sums, over the stages
+      __syncthreads();
+      float2* ml = reinterpret_cast<float2*>(smem);
+      float* so = reinterpret_cast<float*>(smem + 4 * 16 * 8);
+      if (j == 0) {
+        ml[warp * 16 + g] = make_float2(m0, l0);
+        if constexpr (!SPLIT) ml[warp * 16 + g + 8] = make_float2(m1, l1);
+      }
+      __syncthreads();
+      auto top = [&](int r) {
+        return fmaxf(fmaxf(ml[r].x, ml[16 + r].x), fmaxf(ml[32 + r].x, ml[48 + r].x));
+      };
+      const float t0 = top(g), f0 = m0 == -INFINITY ? 0.f : ex2(m0 - t0);
+      float f1 = 0.f;
+      if constexpr (!SPLIT) f1 = m1 == -INFINITY ? 0.f : ex2(m1 - top(g + 8));
+      // a warp that saw nothing of a row contributes nothing, not 0·NaN
+#pragma unroll
+      for (int d = 0; d < DT; ++d) {
+        const int i = d * 8 + 2 * j;
+        *reinterpret_cast<float2*>(so + (warp * WROWS + g) * HD + i) =
+            l0 != 0.f ? make_float2(o[d][0] * f0, o[d][1] * f0) : make_float2(0.f, 0.f);
+        if constexpr (!SPLIT)
+          *reinterpret_cast<float2*>(so + (warp * WROWS + g + 8) * HD + i) =
+              l1 != 0.f ? make_float2(o[d][2] * f1, o[d][3] * f1) : make_float2(0.f, 0.f);
+      }
+      __syncthreads();
+      for (int i = tid; i < rows * (HD / 2); i += kRowsThreads) {
+        const int r = i / (HD / 2), d = 2 * (i - r * (HD / 2));
+        const float t = top(r);
+        float x = 0.f, y = 0.f, l = 0.f;
+#pragma unroll
+        for (int q = 0; q < 4; ++q) {
+          const float2 v = *reinterpret_cast<const float2*>(so + (q * WROWS + r) * HD + d);
+          const float2 e = ml[q * 16 + r];
+          x += v.x;
+          y += v.y;
+          l += e.x == -INFINITY ? e.y : e.y * ex2(e.x - t);
+        }
+        if (whole) {
+          const float inv = l != 0.f ? 1.f / l : 0.f;
+          x *= inv;
+          y *= inv;
+        } else if (d == 0) {
+          *reinterpret_cast<float2*>(part_ml + 2 * r) = make_float2(t, l);
+        }
+        put2(r, d, x, y);
+      }
+      __syncthreads();   // the stages are free for the next tile
+    } else {
+      const float i0 = !whole ? 1.f : l0 != 0.f ? 1.f / l0 : 0.f, i1 = !whole ? 1.f : l1 != 0.f ? 1.f / l1 : 0.f;
+      const int r = wm * WROWS + g;
+#pragma unroll
+      for (int d = 0; d < DT; ++d) {
+        const int i = d * 8 + 2 * j;
+        if (r < rows) put2(r, i, o[d][0] * i0, o[d][1] * i0);
+        if constexpr (!SPLIT)
+          if (r + 8 < rows) put2(r + 8, i, o[d][2] * i1, o[d][3] * i1);
+      }
+      if (!whole && j == 0) {
+        if (r < rows) *reinterpret_cast<float2*>(part_ml + 2 * r) = make_float2(m0, l0);
+        if constexpr (!SPLIT)
+          if (r + 8 < rows) *reinterpret_cast<float2*>(part_ml + 2 * (r + 8)) = make_float2(m1, l1);
+      }
+      __syncthreads();
+    }
+
+    if (u_lo == 0 && u_hi < at.units) {   // starts here, ends elsewhere
+      rec.h = at.h;
+      rec.s = at.s;
+      rec.t = at.t;
+      rec.rows = rows;
+      rec.q0 = at.q0;
+      rec.slot = slot;
+      rec.last = cta_of_unit(sh.u + at.units - 1, sh.total, sh.n);
+    }
+    sh.u += u_hi - u_lo;
+    sh.off = 0;
+    first_tile = false;
+    if (sh.u < sh.u_end) next_tile(w, sh.at);
+  }
+  if (tid == 0) a.split[blockIdx.x] = rec;
+}
+
+int launch_page_rows_64(const PageRowsArgs& a, bool split, int wm, cudaStream_t s);
+int launch_page_rows_96(const PageRowsArgs& a, bool split, int wm, cudaStream_t s);
+int launch_page_rows_128(const PageRowsArgs& a, bool split, int wm, cudaStream_t s);
+int launch_page_rows_256(const PageRowsArgs& a, bool split, int wm, cudaStream_t s);
+
+// Stages of the ring and the CTAs that fit on an SM with them.
+template <int HD, bool KQ, bool VQ>
+inline int rows_smem_bytes(const PageRowsArgs& a, int stages) {
+  const int ring = stages * rows_stage_bytes<HD, KQ, VQ>(a.c.rb_k, a.c.rb_v) + rows_conv_bytes<HD, KQ, VQ>();
+  const int join = 4 * 16 * 8 + 4 * 16 * HD * 4, sums = kPageMaxSeq * 4;
+  return std::max(ring, std::max(join, sums));
+}
+
+template <int HD, bool KQ, bool VQ, bool SPLIT, int WM>
+int launch_page_rows_one(const PageRowsArgs& a, cudaStream_t s) {
+  // As deep a ring as leaves two CTAs on an SM (one at head_dim 256 with fp16 rows).
+  const int stages = HD == 256 && !(KQ && VQ) ? 2 : 3;
+  const int smem = rows_smem_bytes<HD, KQ, VQ>(a, stages);
+  auto kern = page_rows_kernel<HD, KQ, VQ, SPLIT, WM>;
+  // looked up once per device and cache type pair
+  static std::atomic<int> resident[kMaxDevices][2][2];
+  int dev = 0;
+  B2_CUDA_TRY(cudaGetDevice(&dev));
+  B2_CHECK_ARG(dev < kMaxDevices, "device index");
+  std::atomic<int>& known = resident[dev][a.c.type_k == B2_Q4_0][a.c.type_v == B2_Q4_0];
+  int per_sm = known.load(std::memory_order_relaxed);
+  if (per_sm == 0) {
+    B2_CUDA_TRY(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, 227 * 1024));
+    B2_CUDA_TRY(cudaOccupancyMaxActiveBlocksPerMultiprocessor(&per_sm, kern, kRowsThreads, smem));
+    per_sm = std::max(1, std::min(per_sm, kPageMaxCtasPerSm));
+    known.store(per_sm, std::memory_order_relaxed);
+  }
+  const int ctas = per_sm * sm_count();
+  const int rc = launch_pdl(kern, dim3(ctas), dim3(kRowsThreads), (size_t)smem, s, a, stages);
+  if (rc != B2_OK) return rc;
+  return launch_page_join(a.w, a.split, a.slots, ctas, HD, a.n_head, a.out, a.q_f32 != 0, s);
+}
+
+template <int HD>
+int launch_page_rows_hd(const PageRowsArgs& a, bool split, int wm, cudaStream_t s) {
+  const bool kq = a.c.type_k != B2_F16, vq = a.c.type_v != B2_F16;
+#define B2_ROWS(KQ, VQ)                                                                             \
+  if (kq == KQ && vq == VQ) {                                                                       \
+    if (split) return wm == 1 ? launch_page_rows_one<HD, KQ, VQ, true, 1>(a, s)                     \
+                              : launch_page_rows_one<HD, KQ, VQ, true, 4>(a, s);                    \
+    return wm == 1 ? launch_page_rows_one<HD, KQ, VQ, false, 1>(a, s)                               \
+                   : launch_page_rows_one<HD, KQ, VQ, false, 4>(a, s);                              \
+  }
+  B2_ROWS(false, false)
+  B2_ROWS(true, false)
+  B2_ROWS(false, true)
+  B2_ROWS(true, true)
+#undef B2_ROWS
+  return B2_ERR_UNSUPPORTED;
+}
+
+}  // namespace b2

@@ -337,6 +337,145 @@ B2_API int b2_kv_shift_k(uint16_t* k_cache, int seq, int n_kv, int head_dim, int
 B2_API int b2_flag_wait(const uint64_t* flags, int n, uint64_t target, int* status, void* stream);
 
 /* ------------------------------------------------------------------------ */
+/* Paged K/V cache                                                            */
+/* ------------------------------------------------------------------------ */
+
+/* A cache whose positions live in pages of page_size positions that any
+ * sequence may hold, and several may share: no n_ctx is reserved per
+ * sequence, and a shared prefix is kept once.  The reference leaves its cache
+ * to llama.cpp, whose unified cache shares cells among sequences
+ * (llama_memory_seq_cp); these operators are this library's form of it.
+ *
+ * k and v are device pools of b2_page_cache_bytes bytes each (16-byte
+ * aligned): [n_layer][n_pages][n_kv][page_size] rows of
+ * b2_kv_row_bytes(type, head_dim) bytes, in the storage of the typed caches
+ * above.  page_size a power of two, 1..256; head_dim a multiple of 32 up to
+ * 256 (attention: 64, 96, 128 and 256). */
+typedef struct b2_page_cache {
+    void*   k;
+    void*   v;
+    int32_t n_layer, n_pages, page_size, n_kv, head_dim;
+    int32_t type_k, type_v;     /* B2_F16, B2_Q8_0 or B2_Q4_0, each on its own */
+} b2_page_cache;
+
+/* One step's sequences.  Sequence s brings the new tokens at rows
+ * [q_start[s], q_start[s+1]) of the token arrays; they are the last ones of
+ * its kv_len[s] positions, which count them.  Position p of sequence s is slot
+ * p % page_size of page table[s·max_pages + p / page_size].  The three arrays
+ * are device int32 and are read when the call runs, so a captured call follows
+ * them.  q_start[0] = 0 and ascending; n_tok is q_start[n_seq] or more, rows
+ * past it are not touched; max_q is at least every sequence's new tokens.
+ * Lengths outside the arrays are clamped into them; a table entry outside
+ * [0, n_pages) that a position needs reads as a row of zeros and stores
+ * nothing.  n_seq <= 1024, max_pages·page_size <= 2^30. */
+typedef struct b2_page_batch {
+    const int32_t* q_start;     /* [n_seq + 1] */
+    const int32_t* kv_len;      /* [n_seq] */
+    const int32_t* table;       /* [n_seq][max_pages] */
+    int32_t n_seq, max_pages, n_tok, max_q;
+} b2_page_batch;
+
+B2_API int b2_page_cache_bytes(const b2_page_cache* cache, size_t* bytes_k, size_t* bytes_v);
+
+/* Rotary positions with several axes, and the store.  qkv [n_tok][(n_head +
+ * 2·n_kv)·head_dim] of type_x (B2_F32 or B2_F16) holds q, k and v heads.  Pair
+ * j of the first n_rot values of every q and k head turns by the angle of one
+ * of the token's n_axes positions (time, height, width of a picture's or
+ * video's token; 1 for text): pos device int32 [n_axes][n_tok], axis device
+ * uint8 [n_rot/2] naming the axis of each pair (NULL: axis 0; see
+ * b2_rope_sections), rope device fp32 [n_pos][n_rot] from b2_rope_table(theta,
+ * n_rot, ...).  style B2_ROPE_ADJACENT pairs values (2j, 2j+1),
+ * B2_ROPE_HALVES (j, j + n_rot/2).  Values past n_rot and the v heads pass
+ * unchanged.  q_out [n_tok][n_head][head_dim] of type_q (B2_F32 or B2_F16); k
+ * and v go to their positions of `layer`, quantized as the typed caches
+ * quantize.  With B2_F32 and one axis the results are bit-identical to
+ * b2_rope_kv_store_typed.  A token with a rotary position or axis outside the
+ * table, or no place in the cache, gets a zero q row and stores nothing.
+ * n_rot a multiple of 8 up to head_dim.  Every device array 16-byte aligned
+ * (pos, axis and the batch: their own type). */
+#define B2_ROPE_ADJACENT 0
+#define B2_ROPE_HALVES 1
+B2_API int b2_page_rope_store(const b2_page_cache* cache, int32_t layer, const b2_page_batch* batch, int32_t n_head,
+                              const void* qkv, int type_x, void* q_out, int type_q, const int32_t* pos,
+                              int32_t n_axes, const uint8_t* axis, const float* rope, int32_t n_pos, int32_t n_rot,
+                              int style, void* stream);
+/* The axis of each of n_pairs rotary pairs (host, out [n_pairs]) from the
+ * number of pairs of each of n_axes (1..8) axes, whose sum is n_pairs:
+ * consecutive sections, or with interleave != 0 dealt in turn (axis 0, 1, 2,
+ * 0, 1, 2, ...) while an axis has pairs left. */
+B2_API int b2_rope_sections(const int32_t* sections, int32_t n_axes, int32_t n_pairs, int interleave, uint8_t* out);
+
+/* Attention of each sequence's new tokens over its pages of `layer`, one
+ * token or many per sequence: the token at position p attends to positions
+ * (p - window, p], window <= 0 meaning all up to p, with n_head/n_kv query
+ * heads per kv head and scores scale·q·k.  q and out [n_tok][n_head][head_dim]
+ * of type_q: B2_F32 is computed to fp32 accuracy, B2_F16 rounds the softmax
+ * weights to fp16.  A token that sees no position gets a zero row; no value
+ * outside the positions a token sees reaches its row, infinite and NaN ones
+ * included.  Results do not depend on timing: the same call gives the same
+ * bits.  Unlike b2_attn_decode the sums are not in the reference's sequential
+ * order.  |scale·q| and |v| up to 65504 (fp16's range).
+ * workspace: device, 16-byte aligned, b2_page_attn_workspace_bytes for this
+ * batch's n_tok, max_q and n_seq or larger ones; one call at a time may use
+ * it.  NULL: the call allocates stream-ordered scratch.  status (device int,
+ * may be NULL) receives a nonzero code if a pipeline wait expired. */
+B2_API int b2_page_attn_workspace_bytes(const b2_page_cache* cache, const b2_page_batch* batch, int32_t n_head,
+                                        int type_q, size_t* bytes);
+B2_API int b2_page_attn(const b2_page_cache* cache, int32_t layer, const b2_page_batch* batch, int32_t n_head,
+                        const void* q, void* out, int type_q, float scale, int32_t window, void* workspace,
+                        size_t workspace_bytes, int* status, void* stream);
+
+/* Whole pages src[i] -> dst[i] (host int32 [n]) in every layer, K and V.  No
+ * page may be written twice, or be both written and read. */
+B2_API int b2_page_copy(const b2_page_cache* cache, const int32_t* src, const int32_t* dst, int32_t n, void* stream);
+
+/* Kept positions gathered, in every layer, K and V: entry i of sequence s's
+ * list (device int32, entries keep_start[s] .. keep_start[s+1] of keep, n_keep
+ * in all) names a position of its old table that becomes position i of its new
+ * one ([n_seq][max_pages] both, device int32).  Rows are moved as they are: K
+ * keeps the rotary positions it was stored with.  A new page must not be an
+ * old page of the call, except where the position keeps its page and slot
+ * (nothing is moved then). */
+B2_API int b2_page_gather(const b2_page_cache* cache, int32_t n_seq, const int32_t* keep_start, const int32_t* keep,
+                          int32_t n_keep, const int32_t* old_table, const int32_t* new_table, int32_t max_pages,
+                          void* stream);
+
+/* Host-side page bookkeeping (CPU only): which pages each sequence holds, in
+ * order, its length, and how many sequences share a page.  Not thread-safe.
+ * The pool decides, b2_page_copy and b2_page_gather move the bytes; calls on
+ * one stream in the order of the decisions keep a page's old readers ahead of
+ * its new writers. */
+typedef struct b2_page_pool b2_page_pool;
+B2_API int b2_page_pool_create(int32_t n_pages, int32_t page_size, int32_t n_seq, int32_t max_pages,
+                               b2_page_pool** out);
+B2_API int b2_page_pool_destroy(b2_page_pool* p);
+/* Room for n more positions of a sequence.  If its last page is partly filled
+ * and shared, the sequence gets a copy of its own: *copy_src and *copy_dst
+ * name the page copy to make before the positions are written (-1 when there
+ * is none).  B2_NO_KV_SLOT, with nothing changed, when the pool has too few
+ * pages or the sequence would pass max_pages. */
+B2_API int b2_page_pool_extend(b2_page_pool* p, int32_t seq, int32_t n, int32_t* copy_src, int32_t* copy_dst);
+/* dst (empty) shares the first n positions of src. */
+B2_API int b2_page_pool_fork(b2_page_pool* p, int32_t src, int32_t dst, int32_t n);
+/* Keeps the first n positions (0: frees the sequence). */
+B2_API int b2_page_pool_truncate(b2_page_pool* p, int32_t seq, int32_t n);
+/* Keeps the n positions keep[] (ascending): whole leading pages that do not
+ * change stay, the others become fresh pages for b2_page_gather; old_table
+ * [max_pages] receives the pages as they were (-1 past the end).  The old
+ * pages stay taken until b2_page_pool_settle, called once the gather has been
+ * issued.  B2_NO_KV_SLOT, with nothing changed, when pages are short. */
+B2_API int b2_page_pool_keep(b2_page_pool* p, int32_t seq, const int32_t* keep, int32_t n, int32_t* old_table);
+B2_API int b2_page_pool_settle(b2_page_pool* p);
+/* Moves used pages down so that they are the first ones of the pool: *n pairs
+ * for b2_page_copy in src / dst (room for `room` pairs; never more than half
+ * the pages).  Held pages must be settled first. */
+B2_API int b2_page_pool_defrag(b2_page_pool* p, int32_t* src, int32_t* dst, int32_t room, int32_t* n);
+/* The table row of a sequence (out [max_pages], -1 past the end) and its
+ * length in positions; either may be NULL. */
+B2_API int b2_page_pool_table(const b2_page_pool* p, int32_t seq, int32_t* out, int32_t* length);
+B2_API int b2_page_pool_free_pages(const b2_page_pool* p, int32_t* n);
+
+/* ------------------------------------------------------------------------ */
 /* GGUF model files                                                           */
 /* ------------------------------------------------------------------------ */
 
