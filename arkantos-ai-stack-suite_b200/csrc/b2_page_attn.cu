@@ -2,8 +2,7 @@
 // split over several CTAs.
 #include <math.h>
 
-#include "b2_page_rows.cuh"
-#include "b2_page_work.cuh"
+#include "b2_page_tc.cuh"
 
 namespace b2 {
 namespace {
@@ -67,17 +66,26 @@ __global__ void __launch_bounds__(kJoinThreads)
 
 // Which kernel takes a call, by the most rows a sequence has per kv head.
 struct Plan {
-  bool split;
-  int wm, rows, bk;
+  bool tc, split;
+  int wm, rows, bk, max_ctas;
 };
 Plan plan_of(const PageAttnArgs& a) {
   const int64_t rows = (int64_t)a.b.max_q * (a.n_head / a.c.n_kv);
   const bool f32 = a.type_q == B2_F32;
   Plan p;
-  p.split = f32 || rows <= 8;
-  p.wm = rows <= (p.split ? 8 : 16) ? 1 : 4;
-  p.rows = (p.split ? 8 : 16) * p.wm;
-  p.bk = kRowsBk;
+  p.tc = rows > 32 && page_tc_ok(a.c, a.hd);
+  p.split = f32 || (!p.tc && rows <= 8);
+  if (p.tc) {
+    p.wm = 0;
+    p.rows = kTcRows;
+    p.bk = kTcBk;
+    p.max_ctas = sm_count();
+  } else {
+    p.wm = rows <= (p.split ? 8 : 16) ? 1 : 4;
+    p.rows = (p.split ? 8 : 16) * p.wm;
+    p.bk = kRowsBk;
+    p.max_ctas = kPageMaxCtasPerSm * sm_count();
+  }
   return p;
 }
 PageWork work_of(const PageAttnArgs& a, const Plan& p) {
@@ -110,12 +118,27 @@ int launch_page_join(const PageWork& w, const SplitTile* split, const float* slo
 
 size_t page_attn_workspace(const PageAttnArgs& a) {
   const Plan p = plan_of(a);
-  const int ctas = kPageMaxCtasPerSm * sm_count();
-  return split_bytes(ctas) + 2 * (size_t)ctas * slot_floats(p.rows, a.hd) * 4;
+  return split_bytes(p.max_ctas) + 2 * (size_t)p.max_ctas * slot_floats(p.rows, a.hd) * 4;
 }
 
 int launch_page_attn(const PageAttnArgs& a, cudaStream_t s) {
   const Plan p = plan_of(a);
+  const float scale_log2 = (float)((double)a.scale * 1.4426950408889634);
+  SplitTile* split = reinterpret_cast<SplitTile*>(a.ws);
+  float* slots = reinterpret_cast<float*>(a.ws + split_bytes(p.max_ctas));
+  if (p.tc) {
+    PageTcArgs t;
+    t.c = a.c;
+    t.w = work_of(a, p);
+    t.q = a.q;
+    t.out = a.out;
+    t.n_head = a.n_head;
+    t.scale_log2 = scale_log2;
+    t.split = split;
+    t.slots = slots;
+    t.status = a.status;
+    return launch_page_tc(t, a.hd, p.split, 1 << a.c.ps_log2, s);
+  }
   PageRowsArgs r;
   r.c = a.c;
   r.w = work_of(a, p);
@@ -123,9 +146,9 @@ int launch_page_attn(const PageAttnArgs& a, cudaStream_t s) {
   r.out = a.out;
   r.n_head = a.n_head;
   r.q_f32 = a.type_q == B2_F32;
-  r.scale_log2 = a.scale * 1.44269504088896340736f;
-  r.split = reinterpret_cast<SplitTile*>(a.ws);
-  r.slots = reinterpret_cast<float*>(a.ws + split_bytes(kPageMaxCtasPerSm * sm_count()));
+  r.scale_log2 = scale_log2;
+  r.split = split;
+  r.slots = slots;
   switch (a.hd) {
     case 64: return launch_page_rows_64(r, p.split, p.wm, s);
     case 96: return launch_page_rows_96(r, p.split, p.wm, s);

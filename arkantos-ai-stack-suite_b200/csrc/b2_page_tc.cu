@@ -1,0 +1,67 @@
+// Launch of the tensor-core page attention (see b2_page_tc.cuh).
+#include "b2_page_tc.cuh"
+
+namespace b2 {
+namespace {
+
+// One layer's pool as [rows][hd] fp16, copied in boxes of one page (at most
+// 128 rows) x 64 dims, 128-byte swizzled.
+int pool_map(const void* base, int hd, int64_t rows, int box_rows, CUtensorMap* map) {
+  static std::atomic<PFN_cuTensorMapEncodeTiled> encode{nullptr};
+  PFN_cuTensorMapEncodeTiled fn = encode.load(std::memory_order_relaxed);
+  if (!fn) {
+    void* p = nullptr;
+    cudaDriverEntryPointQueryResult qr;
+    if (cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &p, cudaEnableDefault, &qr) != cudaSuccess || !p) {
+      set_error("page_attn: cuTensorMapEncodeTiled unavailable");
+      return B2_ERR_CUDA;
+    }
+    fn = reinterpret_cast<PFN_cuTensorMapEncodeTiled>(p);
+    encode.store(fn, std::memory_order_relaxed);
+  }
+  const cuuint64_t dims[2] = {(cuuint64_t)hd, (cuuint64_t)rows};
+  const cuuint64_t strides[1] = {(cuuint64_t)hd * 2};
+  const cuuint32_t box[2] = {64, (cuuint32_t)box_rows}, step[2] = {1, 1};
+  const CUresult r = fn(map, CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 2, const_cast<void*>(base), dims, strides, box, step,
+                        CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+                        CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  if (r != CUDA_SUCCESS) {
+    set_error("page_attn: tensor map of the pool rejected (CUresult %d)", (int)r);
+    return B2_ERR_CUDA;
+  }
+  return B2_OK;
+}
+
+template <int HD, bool SPLIT>
+int launch(const PageTcArgs& a, const CUtensorMap& km, const CUtensorMap& vm, cudaStream_t s) {
+  auto kern = page_tc_kernel<HD, SPLIT>;
+  static std::atomic<int> ready[kMaxDevices];
+  int dev = 0;
+  B2_CUDA_TRY(cudaGetDevice(&dev));
+  B2_CHECK_ARG(dev < kMaxDevices, "device index");
+  if (!ready[dev].load(std::memory_order_relaxed)) {
+    B2_CUDA_TRY(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, TcSmem<HD, SPLIT>::bytes));
+    ready[dev].store(1, std::memory_order_relaxed);
+  }
+  const int ctas = sm_count();   // one per SM: the kernel takes all of TMEM
+  const int rc = launch_pdl(kern, dim3(ctas), dim3(kTcThreads), (size_t)TcSmem<HD, SPLIT>::bytes, s, a, km, vm);
+  if (rc != B2_OK) return rc;
+  return launch_page_join(a.w, a.split, a.slots, ctas, HD, a.n_head, a.out, SPLIT, s);
+}
+
+}  // namespace
+
+int launch_page_tc(PageTcArgs a, int hd, bool split, int page_size, cudaStream_t s) {
+  const int box = std::min(page_size, kTcBk);
+  a.box_rows_log2 = 0;
+  while ((1 << a.box_rows_log2) < box) ++a.box_rows_log2;
+  a.pool_rows = (int64_t)a.c.n_pages * a.c.n_kv * page_size;
+  CUtensorMap km, vm;
+  int rc = pool_map(a.c.k, hd, a.pool_rows, box, &km);
+  if (rc == B2_OK) rc = pool_map(a.c.v, hd, a.pool_rows, box, &vm);
+  if (rc != B2_OK) return rc;
+  if (hd == 128) return split ? launch<128, true>(a, km, vm, s) : launch<128, false>(a, km, vm, s);
+  return split ? launch<64, true>(a, km, vm, s) : launch<64, false>(a, km, vm, s);
+}
+
+}  // namespace b2
