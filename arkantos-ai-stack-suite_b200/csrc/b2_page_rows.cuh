@@ -147,7 +147,9 @@ __global__ void __launch_bounds__(kRowsThreads) page_rows_kernel(const PageRowsA
 
   Share sh;
   int* sums = reinterpret_cast<int*>(smem);
-  const bool have = find_share(w, blockIdx.x, gridDim.x, sums, sh);
+  sum_units(w, sums);
+  __syncthreads();
+  const bool have = find_share(w, blockIdx.x, gridDim.x, sums, sh);   // every warp finds the same place
   SplitTile rec = {};
   rec.last = -1;
   if (!have) {

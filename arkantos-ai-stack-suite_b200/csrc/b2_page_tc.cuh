@@ -14,13 +14,23 @@
 // many cycles of the special-function pipe, so the two bound the kernel
 // together.
 //
-//   warps 0-3, 4-7  softmax of halves 0, 1; they also bring their rows of Q
-//                   into shared memory and write the result
+//   warps 0-3, 4-7  softmax of halves 0, 1, and their results
 //   warp 8          issues the products from one thread
 //   warp 9          brings K and V: one tensor copy per page and 64 dims, the
 //                   lanes issuing side by side; pages past the tile's
 //                   positions and table entries outside the pool are sent out
 //                   of the map's range, which fills zeros
+//   warp 10         walks the tiles of the CTA's share and hands them to the
+//                   other warps through a short ring in shared memory; brings
+//                   the next tile's Q as soon as the last product of this
+//                   one's has read it (SPLIT: the softmax warps do, after
+//                   their results: both parts need the whole of that space)
+//   warp 11         looks over V of units that not every row sees whole
+//
+// The next tile's first product is issued before this tile's results are out,
+// and results leave through shared memory so that a warp writes whole
+// segments of rows: with a few units per tile (a prompt of 2000 tokens has 7
+// on average) the change of tiles costs as much as the units otherwise.
 //
 // The running maximum of a row is raised only when it grew by more than 2^8
 // (the weights are relative to the old one until then: at most 2^15 with
@@ -30,10 +40,17 @@
 // two products instead of one; both parts of p take exactly S's columns.
 // FULL rounds p once to fp16, the error of the fp16 output itself.
 //
-// V rows that a tile must not see are zeroed in shared memory by half 0's
-// threads before the unit's product, and infinite or NaN values of units that
-// only some rows see wholly are taken out and added to the rows that see
-// them at the end, so nothing masked reaches a row as 0·NaN.
+// V rows that a tile must not see are zeroed in shared memory before the
+// unit's product, and infinite or NaN values of units that only some rows see
+// whole are taken out and added to the rows that see them at the end, so
+// nothing masked reaches a row as 0·NaN.
+//
+// The product warp stays converged and elects a lane at each issue, so that
+// descriptors live in uniform registers: issued from a branch of one lane, a
+// tcgen05.mma took about 100 cycles to issue and the issue bounded the kernel
+// (5700 cycles a unit).  For the same reason the tile walk exists once and the
+// waits are short: with everything inlined in every role the code was 160 KB
+// and its fetches showed at every change of tiles.
 //
 // Every wait is bounded: an expired one records a code in *status and ends
 // the other waits.
@@ -62,47 +79,55 @@ struct PageTcArgs {
 
 constexpr int kTcRows = 256, kTcBk = 128, kTcThreads = 384;
 constexpr float kTcOffset = 7.f, kTcRaise = 8.f;
+constexpr int kTcPolls = 1 << 22;   // polls of a wait, each suspended by the hardware for a while
+constexpr int kTcFmaEvery = 8;   // one pair of weights in four is formed on the FMA pipe
 
 template <int HD, bool SPLIT>
 struct TcSmem {
   static constexpr int half_q = 128 * HD * 2;                        // one fp16 part of a half's queries
   static constexpr int q = 2 * half_q * (SPLIT ? 2 : 1);
   static constexpr int tile = kTcBk * HD * 2;
-  static constexpr int stages = HD == 128 ? (SPLIT ? 3 : 5) : 8;
+  static constexpr int stages = HD == 128 ? (SPLIT ? 3 : 4) : 7;
   static constexpr int ctrl = 1024;
-  static constexpr int bytes = ctrl + q + stages * tile + 1024;      // the last for alignment
+  // Results on their way out, 32 rows x 32 columns of fp32 a warp; SPLIT uses
+  // the space of the warp's own queries, which are done by then.
+  static constexpr int out = SPLIT ? 0 : 8 * 32 * 128;
+  static constexpr int bytes = ctrl + q + stages * tile + out + 1024;   // the last for alignment
 };
 
 // ---- tcgen05 -------------------------------------------------------------------------------
-// K-major, 128-byte swizzle: rows of 64 fp16, 8-row groups 1024 bytes apart.
-__device__ __forceinline__ uint64_t tc_desc_k(uint32_t saddr) {
-  return (uint64_t)((saddr >> 4) & 0x3FFF) | ((uint64_t)1 << 16) | ((uint64_t)(1024 >> 4) << 32) | ((uint64_t)1 << 46) |
-         ((uint64_t)2 << 61);
-}
-// N-major (V: rows are positions, the k of P·V; 64 dims of a row contiguous):
-// 64-dim blocks 128 rows apart, 8-row groups 1024 bytes apart.
-__device__ __forceinline__ uint64_t tc_desc_n(uint32_t saddr) {
-  return (uint64_t)((saddr >> 4) & 0x3FFF) | ((uint64_t)((kTcBk * 128) >> 4) << 16) | ((uint64_t)(1024 >> 4) << 32) |
-         ((uint64_t)1 << 46) | ((uint64_t)2 << 61);
-}
+// Shared-memory descriptors, 128-byte swizzle, 8-row groups 1024 bytes apart.
+// The high word is the same for all; the low one is the address in 16-byte
+// steps and the distance of 64-value blocks along M or N, which only N-major
+// operands use (V: rows are positions, the k of P·V, 64 dims of a row
+// contiguous; blocks of 64 dims are 128 rows apart).
+constexpr uint32_t kDescHi = (1024 >> 4) | (1u << 14) | (2u << 29);
+__device__ __forceinline__ uint32_t desc_k(uint32_t saddr) { return (saddr >> 4) | (1u << 16); }
+__device__ __forceinline__ uint32_t desc_n(uint32_t saddr) { return (saddr >> 4) | ((uint32_t)((kTcBk * 128) >> 4) << 16); }
 // fp16 operands, fp32 accumulators, M = 128.
 constexpr uint32_t tc_idesc(int n, bool b_n_major) {
   return (1u << 4) | ((b_n_major ? 1u : 0u) << 16) | ((uint32_t)(n >> 3) << 17) | ((uint32_t)(128 >> 4) << 24);
 }
-__device__ __forceinline__ void tc_mma_ss(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, bool acc) {
+__device__ __forceinline__ void tc_mma_ss(uint32_t d, uint32_t a, uint32_t b, uint32_t idesc, uint32_t acc) {
   asm volatile(
-      "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
-      "tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}\n" ::"r"(d),
-      "l"(a), "l"(b), "r"(idesc), "r"((uint32_t)acc)
+      "{\n\t.reg .pred p;\n\t.reg .b64 x, y;\n\tmov.b64 x, {%1, %3};\n\tmov.b64 y, {%2, %3};\n\tsetp.ne.b32 p, %5, 0;\n\t"
+      "tcgen05.mma.cta_group::1.kind::f16 [%0], x, y, %4, p;\n\t}\n" ::"r"(d),
+      "r"(a), "r"(b), "r"(kDescHi), "r"(idesc), "r"(acc)
       : "memory");
 }
-__device__ __forceinline__ void tc_mma_ts(uint32_t d, uint32_t a, uint64_t b, uint32_t idesc, bool acc) {
+__device__ __forceinline__ void tc_mma_ts(uint32_t d, uint32_t a, uint32_t b, uint32_t idesc, uint32_t acc) {
   asm volatile(
-      "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
-      "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}\n" ::"r"(d),
-      "r"(a), "l"(b), "r"(idesc), "r"((uint32_t)acc)
+      "{\n\t.reg .pred p;\n\t.reg .b64 y;\n\tmov.b64 y, {%2, %3};\n\tsetp.ne.b32 p, %5, 0;\n\t"
+      "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], y, %4, p;\n\t}\n" ::"r"(d),
+      "r"(a), "r"(b), "r"(kDescHi), "r"(idesc), "r"(acc)
       : "memory");
 }
+__device__ __forceinline__ bool elect_one() {
+  uint32_t p;
+  asm volatile("{\n\t.reg .pred p;\n\telect.sync _|p, 0xffffffff;\n\tselp.u32 %0, 1, 0, p;\n\t}\n" : "=r"(p));
+  return p != 0;
+}
+__device__ __forceinline__ uint32_t uniform(uint32_t x) { return __shfl_sync(0xffffffffu, x, 0); }
 __device__ __forceinline__ void tc_commit(uint64_t* bar) {
   asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(smem_u32(bar))
                : "memory");
@@ -127,11 +152,14 @@ __device__ __forceinline__ void tmem_ld32(uint32_t t, float* r) {
       : "r"(t)
       : "memory");
 }
-__device__ __forceinline__ void tmem_ld64(uint32_t t, float* r) {
+__device__ __forceinline__ void tmem_ld128(uint32_t t, float* r) {
   uint32_t* u = reinterpret_cast<uint32_t*>(r);
   asm volatile(
-      "tcgen05.ld.sync.aligned.32x32b.x64.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31,"
-      "%32,%33,%34,%35,%36,%37,%38,%39,%40,%41,%42,%43,%44,%45,%46,%47,%48,%49,%50,%51,%52,%53,%54,%55,%56,%57,%58,%59,%60,%61,%62,%63}, [%64];\n\t"
+      "tcgen05.ld.sync.aligned.32x32b.x128.b32 {"
+      "%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31,"
+      "%32,%33,%34,%35,%36,%37,%38,%39,%40,%41,%42,%43,%44,%45,%46,%47,%48,%49,%50,%51,%52,%53,%54,%55,%56,%57,%58,%59,%60,%61,%62,%63,"
+      "%64,%65,%66,%67,%68,%69,%70,%71,%72,%73,%74,%75,%76,%77,%78,%79,%80,%81,%82,%83,%84,%85,%86,%87,%88,%89,%90,%91,%92,%93,%94,%95,"
+      "%96,%97,%98,%99,%100,%101,%102,%103,%104,%105,%106,%107,%108,%109,%110,%111,%112,%113,%114,%115,%116,%117,%118,%119,%120,%121,%122,%123,%124,%125,%126,%127}, [%128];\n\t"
       "tcgen05.wait::ld.sync.aligned;"
       : "=r"(u[0]), "=r"(u[1]), "=r"(u[2]), "=r"(u[3]), "=r"(u[4]), "=r"(u[5]), "=r"(u[6]), "=r"(u[7]), "=r"(u[8]),
         "=r"(u[9]), "=r"(u[10]), "=r"(u[11]), "=r"(u[12]), "=r"(u[13]), "=r"(u[14]), "=r"(u[15]), "=r"(u[16]),
@@ -140,7 +168,15 @@ __device__ __forceinline__ void tmem_ld64(uint32_t t, float* r) {
         "=r"(u[33]), "=r"(u[34]), "=r"(u[35]), "=r"(u[36]), "=r"(u[37]), "=r"(u[38]), "=r"(u[39]), "=r"(u[40]),
         "=r"(u[41]), "=r"(u[42]), "=r"(u[43]), "=r"(u[44]), "=r"(u[45]), "=r"(u[46]), "=r"(u[47]), "=r"(u[48]),
         "=r"(u[49]), "=r"(u[50]), "=r"(u[51]), "=r"(u[52]), "=r"(u[53]), "=r"(u[54]), "=r"(u[55]), "=r"(u[56]),
-        "=r"(u[57]), "=r"(u[58]), "=r"(u[59]), "=r"(u[60]), "=r"(u[61]), "=r"(u[62]), "=r"(u[63])
+        "=r"(u[57]), "=r"(u[58]), "=r"(u[59]), "=r"(u[60]), "=r"(u[61]), "=r"(u[62]), "=r"(u[63]), "=r"(u[64]),
+        "=r"(u[65]), "=r"(u[66]), "=r"(u[67]), "=r"(u[68]), "=r"(u[69]), "=r"(u[70]), "=r"(u[71]), "=r"(u[72]),
+        "=r"(u[73]), "=r"(u[74]), "=r"(u[75]), "=r"(u[76]), "=r"(u[77]), "=r"(u[78]), "=r"(u[79]), "=r"(u[80]),
+        "=r"(u[81]), "=r"(u[82]), "=r"(u[83]), "=r"(u[84]), "=r"(u[85]), "=r"(u[86]), "=r"(u[87]), "=r"(u[88]),
+        "=r"(u[89]), "=r"(u[90]), "=r"(u[91]), "=r"(u[92]), "=r"(u[93]), "=r"(u[94]), "=r"(u[95]), "=r"(u[96]),
+        "=r"(u[97]), "=r"(u[98]), "=r"(u[99]), "=r"(u[100]), "=r"(u[101]), "=r"(u[102]), "=r"(u[103]), "=r"(u[104]),
+        "=r"(u[105]), "=r"(u[106]), "=r"(u[107]), "=r"(u[108]), "=r"(u[109]), "=r"(u[110]), "=r"(u[111]), "=r"(u[112]),
+        "=r"(u[113]), "=r"(u[114]), "=r"(u[115]), "=r"(u[116]), "=r"(u[117]), "=r"(u[118]), "=r"(u[119]), "=r"(u[120]),
+        "=r"(u[121]), "=r"(u[122]), "=r"(u[123]), "=r"(u[124]), "=r"(u[125]), "=r"(u[126]), "=r"(u[127])
       : "r"(t)
       : "memory");
 }
@@ -163,6 +199,51 @@ __device__ __forceinline__ void tmem_st16(uint32_t t, const uint32_t* u) {
 }
 __device__ __forceinline__ void tmem_wait_st() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
 
+// Two fp32 operations in one instruction.
+__device__ __forceinline__ float2 fma2(float2 a, float2 b, float2 c) {
+  float2 d;
+  asm("{\n\t.reg .b64 x, y, z, r;\n\tmov.b64 x, {%2, %3};\n\tmov.b64 y, {%4, %5};\n\tmov.b64 z, {%6, %7};\n\t"
+      "fma.rn.f32x2 r, x, y, z;\n\tmov.b64 {%0, %1}, r;\n\t}"
+      : "=f"(d.x), "=f"(d.y)
+      : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y), "f"(c.x), "f"(c.y));
+  return d;
+}
+__device__ __forceinline__ float2 add2(float2 a, float2 b) {
+  float2 d;
+  asm("{\n\t.reg .b64 x, y, r;\n\tmov.b64 x, {%2, %3};\n\tmov.b64 y, {%4, %5};\n\t"
+      "add.rn.f32x2 r, x, y;\n\tmov.b64 {%0, %1}, r;\n\t}"
+      : "=f"(d.x), "=f"(d.y)
+      : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y));
+  return d;
+}
+// Maxima that keep a NaN, so that a row with a NaN score becomes NaN whole.
+__device__ __forceinline__ float max_nan(float a, float b) {
+  float d;
+  asm("max.NaN.f32 %0, %1, %2;" : "=f"(d) : "f"(a), "f"(b));
+  return d;
+}
+__device__ __forceinline__ float max3_nan(float a, float b, float c) {
+  float d;
+  asm("max.NaN.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
+  return d;
+}
+// 2^x of two values on the FMA pipe: x = n + f with |f| <= 1/2, 2^f by the
+// cubic of least relative error (7.5e-5, fitted by exchange, a quarter of
+// what the rounding of a weight to fp16 costs), n added to the exponent.
+// Arguments below -125 count as -125.
+__device__ __forceinline__ float2 ex2_fma(float2 x) {
+  x = make_float2(max_nan(x.x, -125.f), max_nan(x.y, -125.f));
+  const float2 big = make_float2(12582912.f, 12582912.f);   // 1.5·2^23: the sum's low bits are n
+  const float2 t = add2(x, big);
+  const float2 n = add2(t, make_float2(-12582912.f, -12582912.f));
+  const float2 f = fma2(n, make_float2(-1.f, -1.f), x);
+  float2 p = fma2(f, make_float2(0.0551716685f, 0.0551716685f), make_float2(0.242611125f, 0.242611125f));
+  p = fma2(p, f, make_float2(0.693260968f, 0.693260968f));
+  p = fma2(p, f, make_float2(0.999928057f, 0.999928057f));
+  return make_float2(__int_as_float(__float_as_int(p.x) + (__float_as_int(t.x) << 23)),
+                     __int_as_float(__float_as_int(p.y) + (__float_as_int(t.y) << 23)));
+}
+
 __device__ __forceinline__ void tma_2d(uint32_t dst, const CUtensorMap* map, int x, int y, uint64_t* bar) {
   asm volatile(
       "cp.async.bulk.tensor.2d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4}], [%2];" ::"r"(
@@ -171,38 +252,73 @@ __device__ __forceinline__ void tma_2d(uint32_t dst, const CUtensorMap* map, int
       : "memory");
 }
 
+// A tile of the CTA's share as the warps see it.
+struct TcTile {
+  int h, s, q0, first;            // kv head, sequence; its first new token's row and position
+  int row0, rows;                 // first row (of the sequence's) and rows of the tile
+  int key0, units;                // first position and units of this CTA's part; units = 0: no more tiles
+  int lo, hi, p_min, p_max;       // positions attended to; those of the first and last row
+  int whole, slot;                // whether the part is the whole tile; the slot of a partial result
+  int pad[2];
+};
+static_assert(sizeof(TcTile) == 64, "four 16-byte words");
+constexpr int kTcTiles = 4;       // ring of tiles
+
+// Whether some row of the tile does not see the unit at key0 whole.
+__device__ __forceinline__ bool tc_edge(const TcTile& t, int key0, int window) {
+  return key0 + kTcBk > t.hi || key0 + kTcBk - 1 > t.p_min || (window > 0 && key0 <= t.p_max - window);
+}
+
 template <int HD, bool SPLIT>
 __global__ void __launch_bounds__(kTcThreads, 1)
     page_tc_kernel(const PageTcArgs a, const __grid_constant__ CUtensorMap k_map,
                    const __grid_constant__ CUtensorMap v_map) {
   using L = TcSmem<HD, SPLIT>;
-  constexpr int NS = L::stages;
+  constexpr int NS = L::stages, PARTS = SPLIT ? 2 : 1;
   extern __shared__ __align__(1024) uint8_t smem_raw[];
   uint8_t* smem = smem_raw + ((1024 - (smem_u32(smem_raw) & 1023)) & 1023);
-  uint64_t* kv_full = reinterpret_cast<uint64_t*>(smem);   // [NS]
-  uint64_t* kv_empty = kv_full + NS;                       // [NS]
-  uint64_t* q_full = kv_empty + NS;                        // [2]
+  // The ring's stages hold K and V of the units in turn; a stage's release is
+  // counted by stage, an arrival by unit and operand, so that warp 11, which
+  // waits for V alone, meets every phase of the barriers it waits on.
+  uint64_t* k_full = reinterpret_cast<uint64_t*>(smem);    // [NS]
+  uint64_t* v_full = k_full + NS;                          // [NS]
+  uint64_t* kv_empty = v_full + NS;                        // [NS]
+  uint64_t* v_ok = kv_empty + NS;                          // [NS], by unit: V has been looked over
+  uint64_t* q_full = v_ok + NS;                            // [2]
   uint64_t* s_full = q_full + 2;                           // [2]
-  uint64_t* p_full = s_full + 2;                           // [2]
-  uint64_t* o_full = p_full + 2;                           // [2]
-  uint64_t* done = o_full + 2;                             // [1]
+  uint64_t* p_full = s_full + 2;                           // [2] first 64 positions, [2] the others
+  uint64_t* o_full = p_full + 4;                           // [2]
+  uint64_t* q_empty = o_full + 2;                          // [2]
+  uint64_t* t_full = q_empty + 2;                          // [kTcTiles]
+  uint64_t* t_empty = t_full + kTcTiles;                   // [kTcTiles]
+  uint64_t* done = t_empty + kTcTiles;                     // [1]
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(smem + 512);
   int* abort_flag = reinterpret_cast<int*>(smem + 516);
-  int* bad_seen = reinterpret_cast<int*>(smem + 520);      // 1 + the last segment with values taken out of V
+  int* bad_seen = reinterpret_cast<int*>(smem + 520);      // 1 + the last tile with values taken out of V
+  TcTile* tiles = reinterpret_cast<TcTile*>(smem + 640);   // [kTcTiles]
   uint8_t* Qs = smem + L::ctrl;                            // [half][part][hd/64][128 rows][128 B]
   uint8_t* Ts = Qs + L::q;                                 // ring of K and V tiles [hd/64][128 rows][128 B]
+  static_assert(8 * (4 * NS + 15 + 2 * kTcTiles) <= 512 && 640 + kTcTiles * 64 <= L::ctrl, "control block");
 
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   if (tid == 0) {
     for (int i = 0; i < NS; ++i) {
-      mbar_init(&kv_full[i], 1);
+      mbar_init(&k_full[i], 1);
+      mbar_init(&v_full[i], 1);
+      mbar_init(&v_ok[i], 32);
       mbar_init(&kv_empty[i], 1);
     }
     for (int i = 0; i < 2; ++i) {
-      mbar_init(&q_full[i], 128);
+      mbar_init(&q_full[i], SPLIT ? 128 : 32);
+      mbar_init(&q_empty[i], 1);
       mbar_init(&s_full[i], 1);
       mbar_init(&p_full[i], 128);
+      mbar_init(&p_full[2 + i], 128);
       mbar_init(&o_full[i], 1);
+    }
+    for (int i = 0; i < kTcTiles; ++i) {
+      mbar_init(&t_full[i], 1);
+      mbar_init(&t_empty[i], 11 * 32);   // warps 0-9 and 11
     }
     mbar_init(done, 1);
     *abort_flag = 0;
@@ -216,385 +332,535 @@ __global__ void __launch_bounds__(kTcThreads, 1)
     asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
   }
   pdl_wait();
-  Share sh;
   const PageWork& w = a.w;
-  const bool have = find_share(w, blockIdx.x, gridDim.x, reinterpret_cast<int*>(Qs), sh);
+  sum_units(w, reinterpret_cast<int*>(Ts));
   tc_before();
-  __syncthreads();   // barriers, the TMEM address; the sums in the queries' place are read
+  __syncthreads();   // barriers, the TMEM address, the sums
   tc_after();
   const uint32_t tmem = *reinterpret_cast<volatile uint32_t*>(tmem_slot);
   pdl_launch_dependents();   // only now: a later kernel must not take the TMEM before this CTA has it
 
+  // A wait of one thread; after one in the CTA has expired all others return.
   auto wait = [&](uint64_t* bar, uint32_t parity, int code) -> bool {
-    if (*reinterpret_cast<volatile int*>(abort_flag)) return false;
-    if (mbar_wait_bounded(bar, parity, a.status, code)) return true;
-    *reinterpret_cast<volatile int*>(abort_flag) = 1;
-    return false;
+    for (int i = 0; !mbar_try_wait(bar, parity); ++i)
+      if (i == kTcPolls || *reinterpret_cast<volatile int*>(abort_flag)) {
+        *reinterpret_cast<volatile int*>(abort_flag) = 1;
+        if (a.status) atomicExch(a.status, code);
+        return false;
+      }
+    return true;
   };
-  // the units [lo, hi) of the current tile that fall into the share
-  auto seg_end = [&]() {
-    return sh.u_end - sh.u < sh.at.units - sh.off ? sh.off + (int)(sh.u_end - sh.u) : sh.at.units;
-  };
-  auto advance = [&](int u_hi) {
-    sh.u += u_hi - sh.off;
-    sh.off = 0;
-    if (sh.u < sh.u_end) next_tile(w, sh.at);
-  };
-  auto unit_edge = [&](const TileAt& at, int key0) {
-    const int row0 = at.t * kTcRows, last = min(row0 + kTcRows, at.rows_total) - 1;
-    return key0 + kTcBk > at.hi || key0 + kTcBk - 1 > at.first + row0 / w.G ||
-           (w.window > 0 && key0 <= at.first + last / w.G - w.window);
+  // The n-th tile of the share, copied out of the ring.
+  auto take_tile = [&](int n, TcTile& t) -> bool {
+    if (!wait(&t_full[n % kTcTiles], (n / kTcTiles) & 1, 90)) return false;
+    const int4* src = reinterpret_cast<const int4*>(&tiles[n % kTcTiles]);
+    int4* dst = reinterpret_cast<int4*>(&t);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) dst[i] = src[i];
+    mbar_arrive(&t_empty[n % kTcTiles]);
+    return t.units > 0;
   };
 
-  // Registers move from the last four warps to the softmax warps: 2 x 184 + 136
+  // Registers move from the last four warps to the softmax warps: 2 x 200 + 104
   // a lane of each scheduler, the 3 x 168 of the launch.
-  if (!have && tid == 0) {
-    SplitTile rec = {};
-    rec.last = -1;
-    a.split[blockIdx.x] = rec;
-  }
-  if (!have) sh.u = sh.u_end = 0;
   if (warp >= 8) {
-    asm volatile("setmaxnreg.dec.sync.aligned.u32 136;");
-  if (warp == 9) {
-    // ---------------- K and V ----------------
-    const int per = 128 >> a.box_rows_log2;              // copies of 64 dims per tile
-    const int rows_box = 1 << a.box_rows_log2;
-    const int bx = lane % per, bh = lane / per;          // this lane's copy: rows bx·rows_box, dims 64·bh
-    int n = 0;
-    bool ok = true;
-    while (ok && sh.u < sh.u_end) {
-      const TileAt& at = sh.at;
-      const int u_hi = seg_end();
-      for (int u = sh.off; ok && u < u_hi; ++u) {
-        const int p = (at.lo_unit + u) * kTcBk + bx * rows_box;
-        int64_t row = -1;
-        if (bh < HD / 64 && p < at.hi && p + rows_box > at.lo) row = page_row(w.b, a.c, at.s, at.h, p);
-        const int y = (int)(row < 0 ? a.pool_rows : row);
-#pragma unroll
-        for (int kv = 0; kv < 2 && ok; ++kv, ++n) {
-          const int st = n % NS;
-          if (n >= NS) ok = wait(&kv_empty[st], ((n / NS) - 1) & 1, 50);
-          ok = __all_sync(0xffffffffu, ok);
-          if (!ok) break;
-          if (lane == 0) mbar_arrive_expect_tx(&kv_full[st], L::tile);
-          __syncwarp();
-          if (bh < HD / 64)
-            tma_2d(smem_u32(Ts + st * L::tile + bh * (kTcBk * 128) + bx * rows_box * 128), kv ? &v_map : &k_map, bh * 64,
-                   y, &kv_full[st]);
-        }
-      }
-      advance(u_hi);
-    }
-    // every copy issued has landed before the CTA may end
-    for (int i = max(0, n - NS); i < n; ++i) mbar_wait_bounded(&kv_full[i % NS], (i / NS) & 1, a.status, 51);
-  } else if (warp == 8) {
-    // ---------------- products ----------------
-    if (lane == 0) {
-      constexpr uint32_t id_s = tc_idesc(128, false), id_o = tc_idesc(HD, true);
-      int n = 0, seg[2] = {0, 0}, pn[2] = {0, 0};   // ring position, segments and P tiles of each half so far
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 104;");
+    if (warp == 9) {
+      // ---------------- K and V ----------------
+      // the sums gave way to the ring once warp 10 has its share, which the
+      // first tile tells
+      const int per = 128 >> a.box_rows_log2;              // copies of 64 dims per operand
+      const int rows_box = 1 << a.box_rows_log2;
+      const int bx = lane % per, bh = lane / per;          // this lane's copy: rows bx·rows_box, dims 64·bh
+      int n = 0;
       bool ok = true;
-      auto qk = [&](int i, int st) {
+      TcTile t;
+      for (int nt = 0; ok && take_tile(nt, t); ++nt) {
+        if (nt == 0) fence_async_proxy();
+        for (int u = 0; ok && u < t.units; ++u) {
+          const int p = t.key0 + u * kTcBk + bx * rows_box;
+          int64_t row = -1;
+          if (bh < HD / 64 && p < t.hi && p + rows_box > t.lo) row = page_row(w.b, a.c, t.s, t.h, p);
+          const int y = (int)(row < 0 ? a.pool_rows : row);
 #pragma unroll
-        for (int part = 0; part < (SPLIT ? 2 : 1); ++part)
-#pragma unroll
-          for (int ks = 0; ks < HD / 16; ++ks) {
-            const uint32_t off = (ks / 4) * (128 * 128) + (ks % 4) * 32;
-            const uint32_t q = smem_u32(Qs) + (i * (SPLIT ? 2 : 1) + part) * L::half_q + off;
-            tc_mma_ss(tmem + i * 128, tc_desc_k(q), tc_desc_k(smem_u32(Ts) + st * L::tile + off), id_s, (part | ks) != 0);
-          }
-        tc_commit(&s_full[i]);
-      };
-      auto pv = [&](int i, int st, bool acc) {
-#pragma unroll
-        for (int part = 0; part < (SPLIT ? 2 : 1); ++part)
-#pragma unroll
-          for (int ks = 0; ks < kTcBk / 16; ++ks)
-            tc_mma_ts(tmem + 256 + i * 128, tmem + i * 128 + (SPLIT ? (ks / 2) * 32 + part * 16 + (ks & 1) * 8 : ks * 8),
-                      tc_desc_n(smem_u32(Ts) + st * L::tile + ks * 2048), id_o, acc || (part | ks) != 0);
-      };
-      while (ok && sh.u < sh.u_end) {
-        const int u_lo = sh.off, u_hi = seg_end();
-        const int halves = min(kTcRows, sh.at.rows_total - sh.at.t * kTcRows) > 128 ? 2 : 1;
-        ok = wait(&kv_full[n % NS], (n / NS) & 1, 60);
-        for (int i = 0; i < halves && ok; ++i) {
-          ok = wait(&q_full[i], seg[i] & 1, 61);
-          tc_after();
-          if (ok) qk(i, n % NS);
-          ++seg[i];
-        }
-        if (ok) tc_commit(&kv_empty[n % NS]);
-        ++n;
-        for (int u = u_lo; ok && u < u_hi; ++u) {
-          const int sv = n % NS, sk = (n + 1) % NS;
-          const bool more = u + 1 < u_hi;
-          ok = wait(&kv_full[sv], (n / NS) & 1, 62);
-          for (int i = 0; i < halves && ok; ++i) {
-            ok = wait(&p_full[i], pn[i] & 1, 63);
-            ++pn[i];
-            tc_after();
+          for (int kv = 0; kv < 2; ++kv, ++n) {
+            const int st = n % NS;
+            uint64_t* full = (kv ? v_full : k_full) + (n / 2) % NS;
+            if (n >= NS) ok = ok && wait(&kv_empty[st], ((n / NS) - 1) & 1, 50);
+            ok = __all_sync(0xffffffffu, ok);
             if (!ok) break;
-            pv(i, sv, u > u_lo);
-            if (i == halves - 1) tc_commit(&kv_empty[sv]);
-            if (more) {
-              if (i == 0) ok = wait(&kv_full[sk], ((n + 1) / NS) & 1, 64);
-              if (!ok) break;
-              qk(i, sk);
-              if (i == halves - 1) tc_commit(&kv_empty[sk]);
-            } else {
-              tc_commit(&o_full[i]);
-            }
+            if (lane == 0) mbar_arrive_expect_tx(full, L::tile);
+            __syncwarp();
+            if (bh < HD / 64)
+              tma_2d(smem_u32(Ts + st * L::tile + bh * (kTcBk * 128) + bx * rows_box * 128), kv ? &v_map : &k_map,
+                     bh * 64, y, full);
           }
-          n += more ? 2 : 1;
         }
-        advance(u_hi);
+        __syncwarp();
       }
-      tc_commit(done);   // every product has completed before TMEM is given back
-      mbar_wait_bounded(done, 0, a.status, 65);
-    }
-  }
-  } else {
-    asm volatile("setmaxnreg.inc.sync.aligned.u32 184;");
-    // ---------------- softmax: a thread owns row 128·half + its lane of TMEM ----------------
-    const int half = warp >> 2, r_in = tid & 127;
-    const uint32_t tm = tmem + ((uint32_t)((warp & 3) * 32) << 16);
-    const uint32_t ts = tm + half * 128, to = tm + 256 + half * 128;
-    const float c = SPLIT ? 1.f : fmaxf(fabsf(a.scale_log2), 1e-30f);   // the sign went into the queries
-    int n_seg = 0, n_s = 0, n_kv = 0, seg_id = 0;   // segments and S tiles of this half; units and segments of all
-    bool ok = true, first_tile = true;
-    SplitTile rec = {};
-    rec.last = -1;
-    while (ok && sh.u < sh.u_end) {
-      const TileAt& at = sh.at;
-      const int u_lo = sh.off, u_hi = seg_end();
-      const int row0 = at.t * kTcRows, rows = min(kTcRows, at.rows_total - row0);
-      const bool whole = u_lo == 0 && u_hi == at.units;
-      const int slot = u_lo == 0 && !first_tile ? 2 * blockIdx.x + 1 : 2 * blockIdx.x;
-      if (half * 128 < rows) {
-        const int r = half * 128 + r_in;
-        const bool on = r < rows;
-        const int rr = row0 + (on ? r : 0), tok = rr / w.G;
-        const int p = on ? at.first + tok : -1;
-        const int64_t e0 = ((int64_t)(at.q0 + tok) * a.n_head + at.h * w.G + (rr - tok * w.G)) * HD;
-        // ---- this row of Q, swizzled for the products ----
-        {
-          uint8_t* qd = Qs + half * (SPLIT ? 2 : 1) * L::half_q;
-          const uint32_t sign = !SPLIT && a.scale_log2 < 0.f ? 0x80008000u : 0u;
-#pragma unroll 4
-          for (int ch = 0; ch < HD / 8; ++ch) {
-            const uint32_t at_q = (ch / 8) * (128 * 128) + r_in * 128 + (((ch & 7) ^ (r_in & 7)) << 4);
-            if constexpr (SPLIT) {
-              float4 x = make_float4(0.f, 0.f, 0.f, 0.f), y = x;
-              if (on) {
-                const float4* q = reinterpret_cast<const float4*>(static_cast<const float*>(a.q) + e0 + ch * 8);
-                x = __ldg(q);
-                y = __ldg(q + 1);
-              }
-              uint4 hi, lo;
-              const float f = a.scale_log2;
-              h2_split(x.x * f, x.y * f, hi.x, lo.x);
-              h2_split(x.z * f, x.w * f, hi.y, lo.y);
-              h2_split(y.x * f, y.y * f, hi.z, lo.z);
-              h2_split(y.z * f, y.w * f, hi.w, lo.w);
-              *reinterpret_cast<uint4*>(qd + at_q) = hi;
-              *reinterpret_cast<uint4*>(qd + L::half_q + at_q) = lo;
-            } else {
-              uint4 x = make_uint4(0, 0, 0, 0);
-              if (on) x = __ldg(reinterpret_cast<const uint4*>(static_cast<const __half*>(a.q) + e0 + ch * 8));
-              x.x ^= sign;
-              x.y ^= sign;
-              x.z ^= sign;
-              x.w ^= sign;
-              *reinterpret_cast<uint4*>(qd + at_q) = x;
-            }
+      // every copy issued has landed before the CTA may end
+      for (int i = max(0, n - NS); i < n; ++i)
+        mbar_wait_bounded(((i & 1) ? v_full : k_full) + (i / 2) % NS, (i / 2 / NS) & 1, a.status, 51);
+    } else if (warp == 10) {
+      // ---------------- tiles, Q (FULL) ----------------
+      Share sh;
+      SplitTile rec = {};
+      rec.last = -1;
+      const bool have = find_share(w, blockIdx.x, gridDim.x, reinterpret_cast<const int*>(Ts), sh);
+      if (!have) sh.u = sh.u_end = 0;
+      __syncwarp();   // the sums are read: the ring may take their place
+      constexpr int LR = HD / 8, RI = 32 / LR;   // lanes per row of Q, rows per step
+      const int ch = lane % LR, rl = lane / LR;
+      const int step_tok = RI / w.G, step_g = RI % w.G;
+      int fills[2] = {0, 0};
+      bool ok = true;
+      for (int nt = 0; ok; ++nt) {
+        if (nt >= kTcTiles) ok = __all_sync(0xffffffffu, wait(&t_empty[nt % kTcTiles], (nt / kTcTiles - 1) & 1, 91));
+        if (!ok) break;
+        TcTile t = {};
+        const bool more = sh.u < sh.u_end;
+        if (more) {
+          const TileAt& at = sh.at;
+          const int u_hi = sh.u_end - sh.u < at.units - sh.off ? sh.off + (int)(sh.u_end - sh.u) : at.units;
+          t.h = at.h;
+          t.s = at.s;
+          t.q0 = at.q0;
+          t.first = at.first;
+          t.row0 = at.t * kTcRows;
+          t.rows = min(kTcRows, at.rows_total - t.row0);
+          t.key0 = (at.lo_unit + sh.off) * kTcBk;
+          t.units = u_hi - sh.off;
+          t.lo = at.lo;
+          t.hi = at.hi;
+          t.p_min = at.first + t.row0 / w.G;
+          t.p_max = at.first + (t.row0 + t.rows - 1) / w.G;
+          t.whole = sh.off == 0 && u_hi == at.units;
+          t.slot = sh.off == 0 && nt > 0 ? 2 * blockIdx.x + 1 : 2 * blockIdx.x;
+          if (sh.off == 0 && u_hi < at.units) {
+            rec.h = at.h;
+            rec.s = at.s;
+            rec.t = at.t;
+            rec.rows = t.rows;
+            rec.q0 = at.q0;
+            rec.slot = t.slot;
+            rec.last = cta_of_unit(sh.u + at.units - 1, sh.total, sh.n);
           }
-          fence_async_proxy();
-          mbar_arrive(&q_full[half]);
+          sh.u += t.units;
+          sh.off = 0;
         }
-        float m = -INFINITY, l = 0.f;
-        for (int u = u_lo; u < u_hi && ok; ++u) {
-          const int key0 = (at.lo_unit + u) * kTcBk;
-          const bool edge = unit_edge(at, key0);
-          ok = wait(&s_full[half], n_s & 1, 70);
-          ++n_s;
-          ok = __all_sync(0xffffffffu, ok);
-          if (!ok) break;
-          tc_after();
-          // The columns past 63 give their maximum, then the first 64 stay in
-          // registers: their weights go where they came from before the others
-          // are read again.
-          float s[64];
-          // this row sees columns [lo, hi)
-          const int hi = min(p + 1, at.hi) - key0, lo = w.window > 0 ? p - w.window + 1 - key0 : 0;
-          auto load = [&](int h) {
-            tmem_ld64(ts + h * 64, s);
-            if (edge) {
-#pragma unroll
-              for (int i = 0; i < 64; ++i)
-                if (i + h * 64 >= hi || i + h * 64 < lo) s[i] = -INFINITY;
-            }
-          };
-          float top = -INFINITY, top1 = -INFINITY;
-          load(1);
-#pragma unroll
-          for (int i = 0; i < 64; i += 2) {
-            top = fmaxf(top, s[i]);
-            top1 = fmaxf(top1, s[i + 1]);
-          }
-          load(0);
-#pragma unroll
-          for (int i = 0; i < 64; i += 2) {
-            top = fmaxf(top, s[i]);
-            top1 = fmaxf(top1, s[i + 1]);
-          }
-          top = fmaxf(top, top1) * c;
-          const bool raise = top > m + kTcRaise || (m == -INFINITY && top > m);
-          if (__any_sync(0xffffffffu, raise)) {
-            const float nm = raise ? top : m;
-            const float f = m == -INFINITY ? 0.f : ex2(m - nm);
-            const float g = raise ? f : 1.f;                      // the other rows keep their maximum
-            if (u > u_lo) {
-              float o[16];
-#pragma unroll 1
-              for (int i = 0; i < HD / 16; ++i) {
-                tmem_ld16(to + i * 16, o);
-#pragma unroll
-                for (int e = 0; e < 16; ++e) o[e] *= g;
-                tmem_st16(to + i * 16, reinterpret_cast<const uint32_t*>(o));
-              }
-            }
-            l *= g;
-            m = nm;
-          }
-          const float rs = (m == -INFINITY ? 0.f : m) - kTcOffset;
-          float l0 = 0.f, l1 = 0.f;
-#pragma unroll
-          for (int h = 0; h < 2; ++h) {
-            if (h) load(1);
-#pragma unroll
-            for (int i = 0; i < 64; i += 2) {
-              s[i] = ex2(fmaf(s[i], c, -rs));
-              s[i + 1] = ex2(fmaf(s[i + 1], c, -rs));
-              l0 += s[i];
-              l1 += s[i + 1];
-            }
-            // FULL: 64 columns of weights over S's first 64.  SPLIT: the two
-            // parts of 32 positions over their own 32 columns.
-#pragma unroll
-            for (int i = 0; i < 2; ++i) {
-              uint32_t ph[16], pl[16];
-#pragma unroll
-              for (int e = 0; e < 16; ++e) {
-                if constexpr (SPLIT)
-                  h2_split(s[i * 32 + 2 * e], s[i * 32 + 2 * e + 1], ph[e], pl[e]);
-                else
-                  ph[e] = h2(s[i * 32 + 2 * e], s[i * 32 + 2 * e + 1]);
-              }
-              if constexpr (SPLIT) {
-                tmem_st16(ts + h * 64 + i * 32, ph);
-                tmem_st16(ts + h * 64 + i * 32 + 16, pl);
-              } else {
-                tmem_st16(ts + h * 32 + i * 16, ph);
-              }
-            }
-          }
-          l += l0 + l1;
-          tmem_wait_st();
-          if (half == 0 && edge) {
-            // V of a unit that some rows do not see wholly
-            const int nv = 2 * (n_kv + u - u_lo) + 1, st = nv % NS;
-            ok = wait(&kv_full[st], (nv / NS) & 1, 71);
-            uint8_t* V = Ts + st * L::tile;
-            int found = 0;
-            const int key = key0 + r_in;
-            const bool none = key >= at.hi || key < at.lo;
+        if (lane == 0) {
+          tiles[nt % kTcTiles] = t;
+          mbar_arrive(&t_full[nt % kTcTiles]);
+        }
+        if (!more) break;
+        if constexpr (!SPLIT) {
+          const int halves = t.rows > 128 ? 2 : 1;
+          const __half* src = static_cast<const __half*>(a.q) + ((int64_t)t.q0 * a.n_head + t.h * w.G) * HD + ch * 8;
+          int tok = (t.row0 + rl) / w.G, g = (t.row0 + rl) - tok * w.G;
+          for (int i = 0; i < halves && ok; ++i) {
+            if (fills[i] > 0) ok = __all_sync(0xffffffffu, wait(&q_empty[i], (fills[i] - 1) & 1, 80));
+            ++fills[i];
+            if (!ok) break;
+            const uint32_t qd = smem_u32(Qs) + i * L::half_q + (ch / 8) * (128 * 128);
 #pragma unroll 4
-            for (int ch = 0; ch < HD / 8; ++ch) {
-              uint4* q = reinterpret_cast<uint4*>(V + (ch / 8) * (kTcBk * 128) + r_in * 128 + ((ch & 7) << 4));
-              uint4 x = *q;
-              const uint4 was = x;
-              uint32_t* v = reinterpret_cast<uint32_t*>(&x);
-#pragma unroll
-              for (int e = 0; e < 4; ++e) {
-                if (none) v[e] = 0u;
-                if ((v[e] & 0x7C00u) == 0x7C00u) v[e] &= 0xFFFF0000u, found = 1;
-                if ((v[e] & 0x7C000000u) == 0x7C000000u) v[e] &= 0xFFFFu, found = 1;
+            for (int r = rl; r < 128; r += RI) {
+              const bool live = i * 128 + r < t.rows;
+              cp_async16(qd + r * 128 + (((ch & 7) ^ (r & 7)) << 4), live ? src + ((int64_t)tok * a.n_head + g) * HD : src,
+                         live);
+              tok += step_tok;
+              g += step_g;
+              if (g >= w.G) {
+                g -= w.G;
+                ++tok;
               }
-              if (x.x != was.x || x.y != was.y || x.z != was.z || x.w != was.w) *q = x;
             }
-            if (found) *reinterpret_cast<volatile int*>(bad_seen) = seg_id + 1;
+            cp_async_commit();
+          }
+          if (halves == 2) {
+            cp_async_wait<1>();
+            fence_async_proxy();
+            if (ok) mbar_arrive(&q_full[0]);
+          }
+          cp_async_wait<0>();
+          fence_async_proxy();
+          if (ok) mbar_arrive(&q_full[halves - 1]);
+        }
+        if (sh.u < sh.u_end) next_tile(w, sh.at);
+      }
+      if (lane == 0) a.split[blockIdx.x] = rec;
+    } else if (warp == 11) {
+      // ---------------- V of units that some rows do not see whole ----------------
+      int n = 0;
+      bool ok = true;
+      TcTile t;
+      for (int nt = 0; ok && take_tile(nt, t); ++nt) {
+        for (int u = 0; ok && u < t.units; ++u, ++n) {
+          const int key0 = t.key0 + u * kTcBk;
+          ok = wait(&v_full[n % NS], (n / NS) & 1, 71);
+          if (tc_edge(t, key0, w.window)) {
+            // zeros where the tile sees nothing; of the others only positions
+            // that some row does not see are looked over
+            uint8_t* V = Ts + ((2 * n + 1) % NS) * L::tile;
+            const int r_hi = max(min(t.hi - key0, kTcBk), 0), r_lo = min(max(t.lo - key0, 0), r_hi);
+            const int below = w.window > 0 ? min(max(t.p_max - w.window + 1 - key0, r_lo), r_hi) : r_lo;
+            const int above = max(min(t.p_min + 1 - key0, r_hi), below);
+#pragma unroll 1
+            for (int blk = 0; blk < HD / 64; ++blk) {
+              uint4* q = reinterpret_cast<uint4*>(V + blk * (kTcBk * 128));
+#pragma unroll 1
+              for (int i = lane; i < kTcBk * 8; i += 32)
+                if (i < r_lo * 8 || i >= r_hi * 8) q[i] = make_uint4(0, 0, 0, 0);
+              uint32_t any = 0;   // bit 15 or 31: an exponent of all ones
+#pragma unroll 1
+              for (int part = 0; part < 2; ++part) {
+                const int i1 = (part ? r_hi : below) * 8;
+#pragma unroll 8
+                for (int i = (part ? above : r_lo) * 8 + lane; i < i1; i += 32) {
+                  const uint4 x = q[i];
+                  any |= ((x.x & 0x7FFF7FFFu) + 0x04000400u) | ((x.y & 0x7FFF7FFFu) + 0x04000400u) |
+                         ((x.z & 0x7FFF7FFFu) + 0x04000400u) | ((x.w & 0x7FFF7FFFu) + 0x04000400u);
+                }
+              }
+              if (__any_sync(0xffffffffu, (any & 0x80008000u) != 0)) {
+                uint32_t* v = reinterpret_cast<uint32_t*>(q);
+#pragma unroll 1
+                for (int i = r_lo * 32 + lane; i < r_hi * 32; i += 32) {
+                  uint32_t x = v[i];
+                  if ((x & 0x7C00u) == 0x7C00u) x &= 0xFFFF0000u;
+                  if ((x & 0x7C000000u) == 0x7C000000u) x &= 0xFFFFu;
+                  v[i] = x;
+                }
+                *reinterpret_cast<volatile int*>(bad_seen) = nt + 1;
+              }
+            }
             fence_async_proxy();
           }
-          tc_before();
-          mbar_arrive(&p_full[half]);
+          mbar_arrive(&v_ok[n % NS]);
         }
-        // ---- the result ----
-        if (ok) ok = wait(&o_full[half], n_seg & 1, 72);
-        ++n_seg;
+      }
+    } else {
+      // ---------------- products (a converged warp; one lane issues) ----------------
+      // a negative scale negates Q (SPLIT has it in Q already)
+      const uint32_t id_s = tc_idesc(128, false) | (!SPLIT && a.scale_log2 < 0.f ? 1u << 13 : 0u);
+      constexpr uint32_t id_o = tc_idesc(HD, true);
+      const uint32_t q_desc = uniform(desc_k(smem_u32(Qs))), k_desc = uniform(desc_k(smem_u32(Ts))),
+                     v_desc = uniform(desc_n(smem_u32(Ts))), tm = uniform(tmem);
+      int n = 0, nq[2] = {0, 0}, np[2] = {0, 0};   // ring position; Q and P tiles of each half so far
+      bool ok = true;
+      auto qk = [&](int i, int st) {
+        const uint32_t kd = uniform(k_desc + st * (L::tile >> 4)), qd = q_desc + i * PARTS * (L::half_q >> 4);
+        if (elect_one()) {
+#pragma unroll
+          for (int part = 0; part < PARTS; ++part)
+#pragma unroll
+            for (int ks = 0; ks < HD / 16; ++ks) {
+              const uint32_t off = ((ks / 4) * (128 * 128) + (ks % 4) * 32) >> 4;
+              tc_mma_ss(tm + i * 128, qd + part * (L::half_q >> 4) + off, kd + off, id_s, (part | ks) != 0);
+            }
+          tc_commit(&s_full[i]);
+        }
+        __syncwarp();
+      };
+      auto pv = [&](int i, int st, int h, bool acc) {   // 64 positions
+        const uint32_t vd = uniform(v_desc + st * (L::tile >> 4)), add = uniform(acc);
+        if (elect_one()) {
+#pragma unroll
+          for (int part = 0; part < PARTS; ++part)
+#pragma unroll
+            for (int k4 = 0; k4 < 4; ++k4) {
+              const int ks = h * 4 + k4;
+              const uint32_t p = SPLIT ? (ks / 2) * 32 + part * 16 + (ks & 1) * 8 : ks * 8;
+              tc_mma_ts(tm + 256 + i * 128, tm + i * 128 + p, vd + ks * (2048 >> 4), id_o, (part | k4) ? 1u : add);
+            }
+        }
+        __syncwarp();
+      };
+      auto commit = [&](uint64_t* bar) {
+        if (elect_one()) tc_commit(bar);
+        __syncwarp();
+      };
+      // S of a tile's first unit
+      auto open_tile = [&](const TcTile& t) {
+        ok = ok && wait(&k_full[(n / 2) % NS], (n / 2 / NS) & 1, 60);
+#pragma unroll
+        for (int i = 0; i < 2; ++i)
+          if (i == 0 || t.rows > 128) {
+            ok = ok && wait(&q_full[i], nq[i]++ & 1, 61);
+            ok = __all_sync(0xffffffffu, ok);
+            if (!ok) return;
+            tc_after();
+            qk(i, n % NS);
+            if (!SPLIT && t.units == 1) commit(&q_empty[i]);
+          }
+        commit(&kv_empty[n % NS]);
+        ++n;
+      };
+      TcTile t;
+      int nt = 0;
+      bool have = take_tile(nt++, t);
+      if (have) open_tile(t);
+      while (ok && have) {
+        for (int u = 0; u < t.units; ++u) {
+          const int sv = n % NS, sk = (n + 1) % NS;
+          const bool more = u + 1 < t.units, two = t.rows > 128;
+          ok = wait(&v_full[(n / 2) % NS], (n / 2 / NS) & 1, 62) && wait(&v_ok[(n / 2) % NS], (n / 2 / NS) & 1, 66);
+#pragma unroll
+          for (int i = 0; i < 2; ++i)
+            if (i == 0 || two) {
+              ok = ok && wait(&p_full[i], np[i] & 1, 63);
+              tc_after();
+              pv(i, sv, 0, u > 0);
+              ok = ok && wait(&p_full[2 + i], np[i]++ & 1, 64);
+              tc_after();
+              pv(i, sv, 1, true);
+              if (!more) commit(&o_full[i]);
+              if (i == 1 || !two) commit(&kv_empty[sv]);
+              if (more) {
+                if (i == 0) ok = ok && wait(&k_full[((n + 1) / 2) % NS], ((n + 1) / 2 / NS) & 1, 65);
+                qk(i, sk);
+                if (!SPLIT && u + 2 == t.units) commit(&q_empty[i]);
+                if (i == 1 || !two) commit(&kv_empty[sk]);
+              }
+            }
+          n += more ? 2 : 1;
+          ok = __all_sync(0xffffffffu, ok);
+          if (!ok) break;
+        }
+        if (!ok) break;
+        have = take_tile(nt++, t);
+        have = __all_sync(0xffffffffu, have);
+        if (have) open_tile(t);
+      }
+      commit(done);   // every product has completed before TMEM is given back
+      mbar_wait_bounded(done, 0, a.status, 67);
+    }
+  } else {
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 200;");
+    // ---------------- softmax: a thread owns row 128·half + its lane of TMEM ----------------
+    const int half = warp >> 2, r = tid;   // row of the tile
+    const uint32_t tm = tmem + ((uint32_t)((warp & 3) * 32) << 16);
+    const uint32_t ts = tm + half * 128, to = tm + 256 + half * 128;
+    const float c = SPLIT ? 1.f : fmaxf(fabsf(a.scale_log2), 1e-30f);   // the product takes the sign
+    int n_o = 0, n_s = 0;   // tiles and units of this half so far
+    bool ok = true;
+    TcTile t;
+    for (int nt = 0; ok && take_tile(nt, t); ++nt) {
+      if (half * 128 >= t.rows) continue;
+      const bool on = r < t.rows;
+      int p = -1;
+      int64_t e0 = 0;          // the row in q and out
+      {
+        const int rr = t.row0 + (on ? r : 0), tok = rr / w.G;
+        if (on) p = t.first + tok;
+        e0 = ((int64_t)(t.q0 + tok) * a.n_head + t.h * w.G + (rr - tok * w.G)) * HD;
+      }
+      if constexpr (SPLIT) {
+        // ---- the warp's 32 rows of Q, a row (hd 64: two) per step, as two parts ----
+        constexpr int LR = HD / 4, RI = 32 / LR, B = 8;
+        uint8_t* qd = Qs + half * 2 * L::half_q;
+        const int ch = lane % LR;   // 4 values
+        const float f = a.scale_log2;
+#pragma unroll 1
+        for (int it = 0; it < 32 / RI; it += B) {
+          float4 x[B];
+#pragma unroll
+          for (int e = 0; e < B; ++e) {
+            const int rl = (it + e) * RI + lane / LR;
+            const int64_t at_r = __shfl_sync(0xffffffffu, e0, rl);
+            const bool live = __shfl_sync(0xffffffffu, (int)on, rl);
+            x[e] = make_float4(0.f, 0.f, 0.f, 0.f);
+            if (live) x[e] = __ldg(reinterpret_cast<const float4*>(static_cast<const float*>(a.q) + at_r) + ch);
+          }
+#pragma unroll
+          for (int e = 0; e < B; ++e) {
+            const int rl = (warp & 3) * 32 + (it + e) * RI + lane / LR;
+            uint2 hi, lo;
+            h2_split(x[e].x * f, x[e].y * f, hi.x, lo.x);
+            h2_split(x[e].z * f, x[e].w * f, hi.y, lo.y);
+            uint8_t* d = qd + (ch / 16) * (128 * 128) + rl * 128 + ((((ch >> 1) & 7) ^ (rl & 7)) << 4) + (ch & 1) * 8;
+            *reinterpret_cast<uint2*>(d) = hi;
+            *reinterpret_cast<uint2*>(d + L::half_q) = lo;
+          }
+        }
+        fence_async_proxy();
+        mbar_arrive(&q_full[half]);
+      }
+      float m = -INFINITY, l = 0.f;
+      for (int u = 0; u < t.units; ++u) {
+        const int key0 = t.key0 + u * kTcBk;
+        const bool edge = tc_edge(t, key0, w.window);
+        ok = wait(&s_full[half], n_s++ & 1, 70);
         ok = __all_sync(0xffffffffu, ok);
         if (!ok) break;
         tc_after();
-        const float inv = !whole ? 1.f : l != 0.f ? 1.f / l : 0.f;
-        float* part = a.slots + (int64_t)slot * slot_floats(kTcRows, HD);
-        const bool bad = *reinterpret_cast<volatile int*>(bad_seen) > seg_id;
-#pragma unroll 1
-        for (int i = 0; i < HD / 32; ++i) {
-          float o[32];
-          tmem_ld32(to + i * 32, o);
-          if (bad && on) {
-            for (int u = u_lo; u < u_hi; ++u) {
-              const int key0 = (at.lo_unit + u) * kTcBk;
-              if (!unit_edge(at, key0)) continue;
-              const int t1 = min(min(p + 1, at.hi), key0 + kTcBk);
-              for (int t = max(max(at.lo, key0), w.window > 0 ? p - w.window + 1 : 0); t < t1; ++t) {
-                const int64_t row = page_row(w.b, a.c, at.s, at.h, t);
-                if (row < 0) continue;
-                const __half* v = reinterpret_cast<const __half*>(a.c.v + row * a.c.rb_v) + i * 32;
+        float s[128];
+        tmem_ld128(ts, s);
+        // this row sees columns [lo, hi)
+        const int hi = min(p + 1, t.hi) - key0, lo = w.window > 0 ? p - w.window + 1 - key0 : 0;
+        if (edge) {
 #pragma unroll
-                for (int e = 0; e < 32; ++e) {
-                  const float f = __half2float(v[e]);
-                  if (!(fabsf(f) <= 65504.f)) o[e] += f;
-                }
-              }
-            }
-          }
+          for (int i = 0; i < 128; ++i)
+            if (i >= hi) s[i] = -INFINITY;
+          if (w.window > 0) {
 #pragma unroll
-          for (int e = 0; e < 32; ++e) o[e] *= inv;
-          if (!on) continue;
-          if (!whole) {
-#pragma unroll
-            for (int e = 0; e < 32; e += 4)
-              *reinterpret_cast<float4*>(part + r * HD + i * 32 + e) = make_float4(o[e], o[e + 1], o[e + 2], o[e + 3]);
-          } else if constexpr (SPLIT) {
-#pragma unroll
-            for (int e = 0; e < 32; e += 4)
-              *reinterpret_cast<float4*>(static_cast<float*>(a.out) + e0 + i * 32 + e) =
-                  make_float4(o[e], o[e + 1], o[e + 2], o[e + 3]);
-          } else {
-#pragma unroll
-            for (int e = 0; e < 32; e += 8)
-              *reinterpret_cast<uint4*>(static_cast<__half*>(a.out) + e0 + i * 32 + e) =
-                  make_uint4(h2(o[e], o[e + 1]), h2(o[e + 2], o[e + 3]), h2(o[e + 4], o[e + 5]), h2(o[e + 6], o[e + 7]));
+            for (int i = 0; i < 128; ++i)
+              if (i < lo) s[i] = -INFINITY;
           }
         }
-        if (!whole && on) *reinterpret_cast<float2*>(part + kTcRows * HD + 2 * r) = make_float2(m, l);
-        tc_before();
+        float top[4] = {s[0], s[1], s[2], s[3]};
+#pragma unroll
+        for (int i = 4; i < 124; i += 8)
+#pragma unroll
+          for (int e = 0; e < 4; ++e) top[e] = max3_nan(top[e], s[i + e], s[i + 4 + e]);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) top[e] = max_nan(top[e], s[124 + e]);
+        const float high = max_nan(max_nan(top[0], top[1]), max_nan(top[2], top[3])) * c;
+        const bool raise = !(high <= m + kTcRaise);   // from -inf, and to NaN, always
+        if (__any_sync(0xffffffffu, raise)) {
+          const float nm = raise ? high : m;
+          const float f = m == -INFINITY ? 0.f : ex2(m - nm);
+          const float g = raise ? f : 1.f;            // the other rows keep their maximum
+          if (u > 0) {
+            float o[16];
+#pragma unroll 1
+            for (int i = 0; i < HD / 16; ++i) {
+              tmem_ld16(to + i * 16, o);
+#pragma unroll
+              for (int e = 0; e < 16; ++e) o[e] *= g;
+              tmem_st16(to + i * 16, reinterpret_cast<const uint32_t*>(o));
+            }
+          }
+          l *= g;
+          m = nm;
+        }
+        const float rs = kTcOffset - (m == -INFINITY ? 0.f : m);
+        float2 sum[2] = {make_float2(0.f, 0.f), make_float2(0.f, 0.f)};
+#pragma unroll
+        for (int h = 0; h < 4; ++h) {
+#pragma unroll
+          for (int i = h * 32; i < h * 32 + 32; i += 2) {
+            const float2 x = fma2(make_float2(s[i], s[i + 1]), make_float2(c, c), make_float2(rs, rs));
+            float2 e;
+            if (!SPLIT && i % kTcFmaEvery == kTcFmaEvery - 2) {
+              e = ex2_fma(x);
+              if (edge) {
+                if (i >= hi || i < lo) e.x = 0.f;
+                if (i + 1 >= hi || i + 1 < lo) e.y = 0.f;
+              }
+            } else {
+              e = make_float2(ex2(x.x), ex2(x.y));
+            }
+            s[i] = e.x;
+            s[i + 1] = e.y;
+            sum[(i >> 1) & 1] = add2(sum[(i >> 1) & 1], e);
+          }
+          // FULL: 64 columns of weights over S's first 64.  SPLIT: the two
+          // parts of 32 positions over their own 32 columns.
+          uint32_t ph[16], pl[16];
+#pragma unroll
+          for (int e = 0; e < 16; ++e) {
+            if constexpr (SPLIT)
+              h2_split(s[h * 32 + 2 * e], s[h * 32 + 2 * e + 1], ph[e], pl[e]);
+            else
+              ph[e] = h2(s[h * 32 + 2 * e], s[h * 32 + 2 * e + 1]);
+          }
+          if constexpr (SPLIT) {
+            tmem_st16(ts + h * 32, ph);
+            tmem_st16(ts + h * 32 + 16, pl);
+          } else {
+            tmem_st16(ts + h * 16, ph);
+          }
+          if (h & 1) {   // 64 positions: their product can begin
+            tmem_wait_st();
+            tc_before();
+            mbar_arrive(&p_full[h - 1 + half]);
+          }
+        }
+        l += (sum[0].x + sum[0].y) + (sum[1].x + sum[1].y);
       }
-      if (u_lo == 0 && u_hi < at.units) {
-        rec.h = at.h;
-        rec.s = at.s;
-        rec.t = at.t;
-        rec.rows = rows;
-        rec.q0 = at.q0;
-        rec.slot = slot;
-        rec.last = cta_of_unit(sh.u + at.units - 1, sh.total, sh.n);
+      // ---- the result ----
+      if (ok) ok = wait(&o_full[half], n_o++ & 1, 72);
+      ok = __all_sync(0xffffffffu, ok);
+      if (!ok) break;
+      tc_after();
+      const float inv = !t.whole ? 1.f : l != 0.f ? 1.f / l : 0.f;
+      float* part = a.slots + (int64_t)t.slot * slot_floats(kTcRows, HD);
+      // Through shared memory, 32 columns at a time: 16-byte chunks of a row,
+      // moved so that neither side meets a bank conflict, then segments of rows.
+      uint8_t* stage = SPLIT ? Qs + half * 2 * L::half_q + (warp & 3) * 4096 : Ts + NS * L::tile + warp * 4096;
+      const bool wide = SPLIT || !t.whole;   // fp32 out
+#pragma unroll 1
+      for (int i = 0; i < HD / 32; ++i) {
+        float o[32];
+        tmem_ld32(to + i * 32, o);
+#pragma unroll
+        for (int e = 0; e < 32; ++e) o[e] *= inv;
+        __syncwarp();
+        if (wide) {
+#pragma unroll
+          for (int ch = 0; ch < 8; ++ch)
+            *reinterpret_cast<float4*>(stage + lane * 128 + ((ch ^ (lane & 7)) << 4)) =
+                make_float4(o[4 * ch], o[4 * ch + 1], o[4 * ch + 2], o[4 * ch + 3]);
+        } else {
+#pragma unroll
+          for (int ch = 0; ch < 4; ++ch)
+            *reinterpret_cast<uint4*>(stage + lane * 64 + ((ch ^ ((lane >> 1) & 3)) << 4)) =
+                make_uint4(h2(o[8 * ch], o[8 * ch + 1]), h2(o[8 * ch + 2], o[8 * ch + 3]),
+                           h2(o[8 * ch + 4], o[8 * ch + 5]), h2(o[8 * ch + 6], o[8 * ch + 7]));
+        }
+        __syncwarp();
+        if (wide) {
+          const int ch = lane & 7;
+#pragma unroll 2
+          for (int it = 0; it < 8; ++it) {
+            const int rl = it * 4 + (lane >> 3), rt = half * 128 + (warp & 3) * 32 + rl;
+            const float4 x = *reinterpret_cast<const float4*>(stage + rl * 128 + ((ch ^ (rl & 7)) << 4));
+            const int64_t at_r = __shfl_sync(0xffffffffu, e0, rl);
+            float* dst = t.whole ? static_cast<float*>(a.out) + at_r : part + rt * HD;
+            if (rt < t.rows) *reinterpret_cast<float4*>(dst + i * 32 + ch * 4) = x;
+          }
+        } else {
+          const int ch = lane & 3;
+#pragma unroll 2
+          for (int it = 0; it < 4; ++it) {
+            const int rl = it * 8 + (lane >> 2), rt = half * 128 + (warp & 3) * 32 + rl;
+            const uint4 x = *reinterpret_cast<const uint4*>(stage + rl * 64 + ((ch ^ ((rl >> 1) & 3)) << 4));
+            const int64_t at_r = __shfl_sync(0xffffffffu, e0, rl);
+            if (rt < t.rows) *reinterpret_cast<uint4*>(static_cast<__half*>(a.out) + at_r + i * 32 + ch * 8) = x;
+          }
+        }
       }
-      n_kv += u_hi - u_lo;
-      ++seg_id;
-      first_tile = false;
-      advance(u_hi);
+      if (!t.whole && on) *reinterpret_cast<float2*>(part + kTcRows * HD + 2 * r) = make_float2(m, l);
+      if (*reinterpret_cast<volatile int*>(bad_seen) > nt) {
+        // infinite and NaN values that were taken out of V, to the rows that
+        // see them: their weight is positive, so the value decides the sum
+        __syncwarp();
+        for (int u = 0; u < t.units && on; ++u) {
+          const int key0 = t.key0 + u * kTcBk;
+          if (!tc_edge(t, key0, w.window)) continue;
+          const int t1 = min(min(p + 1, t.hi), key0 + kTcBk);
+#pragma unroll 1
+          for (int pos = max(max(t.lo, key0), w.window > 0 ? p - w.window + 1 : 0); pos < t1; ++pos) {
+            const int64_t row = page_row(w.b, a.c, t.s, t.h, pos);
+            if (row < 0) continue;
+            const __half* v = reinterpret_cast<const __half*>(a.c.v + row * a.c.rb_v);
+#pragma unroll 1
+            for (int d = 0; d < HD; ++d) {
+              const float f = __half2float(v[d]);
+              if (fabsf(f) <= 65504.f) continue;
+              if (!t.whole)
+                part[r * HD + d] += f;
+              else if (SPLIT)
+                static_cast<float*>(a.out)[e0 + d] += f;
+              else
+                static_cast<__half*>(a.out)[e0 + d] =
+                    __float2half_rn(__half2float(static_cast<__half*>(a.out)[e0 + d]) + f);
+            }
+          }
+        }
+      }
+      tc_before();
     }
-    if (have && tid == 0) a.split[blockIdx.x] = rec;
   }
   tc_before();
   __syncthreads();

@@ -66,9 +66,9 @@ struct Share {
   TileAt at;
 };
 
-// Block-wide.  sums: shared memory of n_seq ints.  Returns false for a CTA
-// without work.
-__device__ __forceinline__ bool find_share(const PageWork& w, int cta, int ctas, int* sums, Share& sh) {
+// Block-wide: the units of every sequence (for one kv head) into sums, shared
+// memory of n_seq ints.  A barrier must follow.
+__device__ __forceinline__ void sum_units(const PageWork& w, int* sums) {
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, warps = blockDim.x >> 5;
   if (w.b.max_q * w.G <= w.rows) {   // one tile at most: a thread per sequence
     for (int s = tid; s < w.b.n_seq; s += blockDim.x) {
@@ -97,8 +97,12 @@ __device__ __forceinline__ bool find_share(const PageWork& w, int cta, int ctas,
       if (lane == 0) sums[s] = sum;
     }
   }
-  __syncthreads();
-  // every warp finds the same place (no second barrier)
+}
+
+// Warp-wide, from the sums: the share of CTA `cta` of `ctas`.  Returns false
+// for a CTA without work.
+__device__ __forceinline__ bool find_share(const PageWork& w, int cta, int ctas, const int* sums, Share& sh) {
+  const int lane = threadIdx.x & 31;
   int64_t per_head = 0;
   for (int s0 = 0; s0 < w.b.n_seq; s0 += 32) {
     int v = s0 + lane < w.b.n_seq ? sums[s0 + lane] : 0;

@@ -220,6 +220,16 @@ def test_attn_long_context_split(qt):
     s = Setup([1, 3], [9001, 4097], 8, 2, 128, 64, qt=qt, seed=9)
     s.check()
     s.check(scale=0.9)
+    s.check(scale=-0.2)
+    s.check(scale=0.0)
+
+
+@pytest.mark.parametrize("qt", [F32, F16])
+@pytest.mark.parametrize("hd", [64, 128])
+def test_attn_scale_signs(hd, qt):
+    s = Setup([1, 90], [200, 300], 8, 2, hd, 16, qt=qt, seed=6)
+    for scale in (-0.3, 0.0, 1.0):
+        s.check(scale=scale)
 
 
 @pytest.mark.parametrize("qt", [F32, F16])
