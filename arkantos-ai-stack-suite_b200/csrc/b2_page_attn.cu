@@ -23,11 +23,11 @@ __global__ void __launch_bounds__(kJoinThreads)
   constexpr int V = HD / 32;   // values of a lane
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const int n = t.last - (int)blockIdx.x + 1;
-  const int64_t slot = (int64_t)slot_floats(w.rows, HD);
+  const int64_t slot = (int64_t)slot_floats(w.rows(), HD);
   auto part = [&](int i) { return slots + (i == 0 ? t.slot : 2 * ((int)blockIdx.x + i)) * slot; };
   for (int r = blockIdx.y * (kJoinThreads / 32) + warp; r < t.rows; r += gridDim.y * (kJoinThreads / 32)) {
     float top = -INFINITY;
-    for (int i = lane; i < n; i += 32) top = fmaxf(top, part(i)[w.rows * HD + 2 * r]);
+    for (int i = lane; i < n; i += 32) top = fmaxf(top, part(i)[w.rows() * HD + 2 * r]);
     top = warp_max(top);
     float o[V], sum = 0.f;
 #pragma unroll
@@ -35,7 +35,7 @@ __global__ void __launch_bounds__(kJoinThreads)
     for (int i0 = 0; i0 < n; i0 += 32) {
       float wt = 0.f, l = 0.f;
       if (i0 + lane < n) {
-        const float2 ml = *reinterpret_cast<const float2*>(part(i0 + lane) + w.rows * HD + 2 * r);
+        const float2 ml = *reinterpret_cast<const float2*>(part(i0 + lane) + w.rows() * HD + 2 * r);
         l = ml.y;
         wt = ml.x == -INFINITY ? (l != 0.f ? 1.f : 0.f) : ex2(ml.x - top);   // l != 0 there: only NaN scores
       }
@@ -52,8 +52,8 @@ __global__ void __launch_bounds__(kJoinThreads)
       }
     }
     const float inv = sum != 0.f ? 1.f / sum : 0.f;
-    const int rr = t.t * w.rows + r;
-    const int64_t at = ((int64_t)(t.q0 + rr / w.G) * n_head + t.h * w.G + rr % w.G) * HD + lane;
+    const int rr = (t.t << w.rows_log2) + r, tok = w.G.div(rr), G = (int)w.G.d;
+    const int64_t at = ((int64_t)(t.q0 + tok) * n_head + t.h * G + rr - tok * G) * HD + lane;
 #pragma unroll
     for (int e = 0; e < V; ++e) {
       if (out_f32)
@@ -89,14 +89,14 @@ Plan plan_of(const PageAttnArgs& a) {
   return p;
 }
 PageWork work_of(const PageAttnArgs& a, const Plan& p) {
-  PageWork w;
+  PageWork w = {};
   w.b = a.b;
   w.ps_log2 = a.c.ps_log2;
   w.n_kv = a.c.n_kv;
-  w.G = a.n_head / a.c.n_kv;
+  w.G = FastDiv::of(a.n_head / a.c.n_kv);
   w.window = a.window;
-  w.rows = p.rows;
-  w.bk = p.bk;
+  while (w.rows() < p.rows) ++w.rows_log2;
+  while (w.bk() < p.bk) ++w.bk_log2;
   return w;
 }
 
@@ -105,7 +105,7 @@ PageWork work_of(const PageAttnArgs& a, const Plan& p) {
 int launch_page_join(const PageWork& w, const SplitTile* split, const float* slots, int ctas, int hd, int n_head,
                      void* out, bool out_f32, cudaStream_t s) {
   // a CTA of 4 rows per slice: large tiles are finished by many CTAs
-  const dim3 grid(ctas, std::min(16, (w.rows + 3) / 4)), block(kJoinThreads);
+  const dim3 grid(ctas, std::min(16, (w.rows() + 3) / 4)), block(kJoinThreads);
 #define B2_JOIN(HD) \
   if (hd == HD) return launch_pdl(page_join_kernel<HD>, grid, block, 0, s, w, split, slots, n_head, out, (int)out_f32);
   B2_JOIN(64)
@@ -123,6 +123,10 @@ size_t page_attn_workspace(const PageAttnArgs& a) {
 
 int launch_page_attn(const PageAttnArgs& a, cudaStream_t s) {
   const Plan p = plan_of(a);
+  // the units of a call are counted in 31 bits
+  const int64_t tiles = ((int64_t)a.b.n_tok * (a.n_head / a.c.n_kv)) / p.rows + a.b.n_seq;
+  B2_CHECK_ARG(a.c.n_kv * tiles * ((((int64_t)a.b.max_pages << a.c.ps_log2) / p.bk) + 2) < ((int64_t)1 << 31),
+               "page_attn: too many tokens for such a long table");
   const float scale_log2 = (float)((double)a.scale * 1.4426950408889634);
   SplitTile* split = reinterpret_cast<SplitTile*>(a.ws);
   float* slots = reinterpret_cast<float*>(a.ws + split_bytes(p.max_ctas));

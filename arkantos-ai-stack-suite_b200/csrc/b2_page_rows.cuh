@@ -54,6 +54,7 @@ __device__ __forceinline__ void cp_async16(uint32_t dst, const void* src, bool o
   asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(on ? 16 : 0) : "memory");
 }
 __device__ __forceinline__ void cp_async_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+__device__ __forceinline__ void cp_async_wait_all() { asm volatile("cp.async.wait_all;" ::: "memory"); }
 template <int N>
 __device__ __forceinline__ void cp_async_wait() {
   asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory");
@@ -171,9 +172,9 @@ __global__ void __launch_bounds__(kRowsThreads) page_rows_kernel(const PageRowsA
   bool first_tile = true;
   while (sh.u < sh.u_end) {
     const TileAt at = sh.at;
-    const int u_lo = sh.off, u_hi = (int)(sh.u_end - sh.u < at.units - u_lo ? u_lo + (sh.u_end - sh.u) : at.units);
-    const int row0 = at.t * w.rows;
-    const int rows = min(w.rows, at.rows_total - row0);
+    const int u_lo = sh.off, u_hi = min(at.units, u_lo + (sh.u_end - sh.u));
+    const int row0 = at.t << w.rows_log2, G = (int)w.G.d;
+    const int rows = min(w.rows(), at.rows_total - row0);
 
     // ---- queries: registers, scaled in fp32 and split, or as they are ----
     uint32_t qf[KS][4];
@@ -182,10 +183,11 @@ __global__ void __launch_bounds__(kRowsThreads) page_rows_kernel(const PageRowsA
       const int r = wm * WROWS + g, r1 = r + 8;
       const bool on0 = r < rows, on1 = !SPLIT && r1 < rows;
       const int rr0 = row0 + (on0 ? r : 0), rr1 = row0 + (on1 ? r1 : 0);
-      if (on0) p0 = at.first + rr0 / w.G;
-      if (on1) p1 = at.first + rr1 / w.G;
-      const int64_t e0 = ((int64_t)(at.q0 + rr0 / w.G) * a.n_head + at.h * w.G + rr0 % w.G) * HD;
-      const int64_t e1 = ((int64_t)(at.q0 + rr1 / w.G) * a.n_head + at.h * w.G + rr1 % w.G) * HD;
+      const int tok0 = w.G.div(rr0), tok1 = w.G.div(rr1);
+      if (on0) p0 = at.first + tok0;
+      if (on1) p1 = at.first + tok1;
+      const int64_t e0 = ((int64_t)(at.q0 + tok0) * a.n_head + at.h * G + rr0 - tok0 * G) * HD;
+      const int64_t e1 = ((int64_t)(at.q0 + tok1) * a.n_head + at.h * G + rr1 - tok1 * G) * HD;
 #pragma unroll
       for (int ks = 0; ks < KS; ++ks) {
         const int d0 = ks * 16 + 2 * j, d1 = d0 + 8;
@@ -283,7 +285,7 @@ __global__ void __launch_bounds__(kRowsThreads) page_rows_kernel(const PageRowsA
       cp_async_commit();
     }
     // positions every live row sees need no mask
-    const int p_min = at.first + row0 / w.G, p_max = at.first + (row0 + rows - 1) / w.G;
+    const int p_min = at.first + w.G.div(row0), p_max = at.first + w.G.div(row0 + rows - 1);
     for (int u = u_lo; u < u_hi; ++u) {
       // all but the newest stages - 2 groups have landed
       if (stages == 4) cp_async_wait<2>(); else if (stages == 3) cp_async_wait<1>(); else cp_async_wait<0>();
@@ -496,12 +498,12 @@ __global__ void __launch_bounds__(kRowsThreads) page_rows_kernel(const PageRowsA
     }
     const bool whole = u_lo == 0 && u_hi == at.units;
     const int slot = u_lo == 0 && !first_tile ? 2 * blockIdx.x + 1 : 2 * blockIdx.x;
-    float* part = a.slots + (int64_t)slot * slot_floats(w.rows, HD);
-    float* part_ml = part + w.rows * HD;
+    float* part = a.slots + (int64_t)slot * slot_floats(w.rows(), HD);
+    float* part_ml = part + w.rows() * HD;
 
     auto out_ptr = [&](int r) -> int64_t {
-      const int rr = row0 + r;
-      return ((int64_t)(at.q0 + rr / w.G) * a.n_head + at.h * w.G + rr % w.G) * HD;
+      const int rr = row0 + r, tok = w.G.div(rr);
+      return ((int64_t)(at.q0 + tok) * a.n_head + at.h * G + rr - tok * G) * HD;
     };
     auto put2 = [&](int r, int d, float x, float y) {   // values d, d + 1 of row r, normalized, or a partial result
       if (!whole) {
@@ -587,7 +589,7 @@ __global__ void __launch_bounds__(kRowsThreads) page_rows_kernel(const PageRowsA
       rec.rows = rows;
       rec.q0 = at.q0;
       rec.slot = slot;
-      rec.last = cta_of_unit(sh.u + at.units - 1, sh.total, sh.n);
+      rec.last = sh.deal.cta_of(sh.u + at.units - 1);
     }
     sh.u += u_hi - u_lo;
     sh.off = 0;

@@ -4,11 +4,10 @@
 namespace b2 {
 namespace {
 
-// One layer's pool as [rows][hd] fp16, copied in boxes of one page (at most
-// 128 rows) x 64 dims, 128-byte swizzled.
-int pool_map(const void* base, int hd, int64_t rows, int box_rows, CUtensorMap* map) {
-  static std::atomic<PFN_cuTensorMapEncodeTiled> encode{nullptr};
-  PFN_cuTensorMapEncodeTiled fn = encode.load(std::memory_order_relaxed);
+int encode(CUtensorMap* map, const void* base, int rank, const cuuint64_t* dims, const cuuint64_t* strides,
+           const cuuint32_t* box) {
+  static std::atomic<PFN_cuTensorMapEncodeTiled> found{nullptr};
+  PFN_cuTensorMapEncodeTiled fn = found.load(std::memory_order_relaxed);
   if (!fn) {
     void* p = nullptr;
     cudaDriverEntryPointQueryResult qr;
@@ -17,23 +16,37 @@ int pool_map(const void* base, int hd, int64_t rows, int box_rows, CUtensorMap* 
       return B2_ERR_CUDA;
     }
     fn = reinterpret_cast<PFN_cuTensorMapEncodeTiled>(p);
-    encode.store(fn, std::memory_order_relaxed);
+    found.store(fn, std::memory_order_relaxed);
   }
-  const cuuint64_t dims[2] = {(cuuint64_t)hd, (cuuint64_t)rows};
-  const cuuint64_t strides[1] = {(cuuint64_t)hd * 2};
-  const cuuint32_t box[2] = {64, (cuuint32_t)box_rows}, step[2] = {1, 1};
-  const CUresult r = fn(map, CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 2, const_cast<void*>(base), dims, strides, box, step,
-                        CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
-                        CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  const cuuint32_t step[3] = {1, 1, 1};
+  const CUresult r = fn(map, CU_TENSOR_MAP_DATA_TYPE_FLOAT16, (cuuint32_t)rank, const_cast<void*>(base), dims, strides,
+                        box, step, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
+                        CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
   if (r != CUDA_SUCCESS) {
-    set_error("page_attn: tensor map of the pool rejected (CUresult %d)", (int)r);
+    set_error("page_attn: tensor map rejected (CUresult %d)", (int)r);
     return B2_ERR_CUDA;
   }
   return B2_OK;
 }
 
+// One layer's pool as [rows][hd] fp16, copied in boxes of one page (at most
+// 128 rows) x 64 dims, 128-byte swizzled.
+int pool_map(const void* base, int hd, int64_t rows, int box_rows, CUtensorMap* map) {
+  const cuuint64_t dims[2] = {(cuuint64_t)hd, (cuuint64_t)rows}, strides[1] = {(cuuint64_t)hd * 2};
+  const cuuint32_t box[2] = {64, (cuuint32_t)box_rows};
+  return encode(map, base, 2, dims, strides, box);
+}
+// Queries [n_tok][n_head][hd], copied as the 128 rows (token, head of the
+// group) of half a tile x 64 dims.
+int query_map(const void* q, int hd, int n_head, int n_tok, int G, CUtensorMap* map) {
+  const cuuint64_t dims[3] = {(cuuint64_t)hd, (cuuint64_t)n_head, (cuuint64_t)n_tok};
+  const cuuint64_t strides[2] = {(cuuint64_t)hd * 2, (cuuint64_t)n_head * hd * 2};
+  const cuuint32_t box[3] = {64, (cuuint32_t)G, (cuuint32_t)(128 / G)};
+  return encode(map, q, 3, dims, strides, box);
+}
+
 template <int HD, bool SPLIT>
-int launch(const PageTcArgs& a, const CUtensorMap& km, const CUtensorMap& vm, cudaStream_t s) {
+int launch(const PageTcArgs& a, const CUtensorMap& km, const CUtensorMap& vm, const CUtensorMap& qm, cudaStream_t s) {
   auto kern = page_tc_kernel<HD, SPLIT>;
   static std::atomic<int> ready[kMaxDevices];
   int dev = 0;
@@ -44,7 +57,7 @@ int launch(const PageTcArgs& a, const CUtensorMap& km, const CUtensorMap& vm, cu
     ready[dev].store(1, std::memory_order_relaxed);
   }
   const int ctas = sm_count();   // one per SM: the kernel takes all of TMEM
-  const int rc = launch_pdl(kern, dim3(ctas), dim3(kTcThreads), (size_t)TcSmem<HD, SPLIT>::bytes, s, a, km, vm);
+  const int rc = launch_pdl(kern, dim3(ctas), dim3(kTcThreads), (size_t)TcSmem<HD, SPLIT>::bytes, s, a, km, vm, qm);
   if (rc != B2_OK) return rc;
   return launch_page_join(a.w, a.split, a.slots, ctas, HD, a.n_head, a.out, SPLIT, s);
 }
@@ -56,12 +69,15 @@ int launch_page_tc(PageTcArgs a, int hd, bool split, int page_size, cudaStream_t
   a.box_rows_log2 = 0;
   while ((1 << a.box_rows_log2) < box) ++a.box_rows_log2;
   a.pool_rows = (int64_t)a.c.n_pages * a.c.n_kv * page_size;
-  CUtensorMap km, vm;
+  CUtensorMap km, vm, qm = {};
   int rc = pool_map(a.c.k, hd, a.pool_rows, box, &km);
   if (rc == B2_OK) rc = pool_map(a.c.v, hd, a.pool_rows, box, &vm);
+  const int G = (int)a.w.G.d;
+  a.q_map = !split && 128 % G == 0;
+  if (rc == B2_OK && a.q_map) rc = query_map(a.q, hd, a.n_head, a.w.b.n_tok, G, &qm);
   if (rc != B2_OK) return rc;
-  if (hd == 128) return split ? launch<128, true>(a, km, vm, s) : launch<128, false>(a, km, vm, s);
-  return split ? launch<64, true>(a, km, vm, s) : launch<64, false>(a, km, vm, s);
+  if (hd == 128) return split ? launch<128, true>(a, km, vm, qm, s) : launch<128, false>(a, km, vm, qm, s);
+  return split ? launch<64, true>(a, km, vm, qm, s) : launch<64, false>(a, km, vm, qm, s);
 }
 
 }  // namespace b2

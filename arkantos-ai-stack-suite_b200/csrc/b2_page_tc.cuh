@@ -45,12 +45,12 @@
 // whole are taken out and added to the rows that see them at the end, so
 // nothing masked reaches a row as 0·NaN.
 //
-// The product warp stays converged and elects a lane at each issue, so that
-// descriptors live in uniform registers: issued from a branch of one lane, a
-// tcgen05.mma took about 100 cycles to issue and the issue bounded the kernel
-// (5700 cycles a unit).  For the same reason the tile walk exists once and the
-// waits are short: with everything inlined in every role the code was 160 KB
-// and its fetches showed at every change of tiles.
+// The product warp stays converged and elects a lane at each issue, which
+// keeps descriptors in uniform registers: with a branch of one lane around all
+// of it a unit took 4800 cycles instead of 4250.  It looks for K and V ahead
+// of need and waits for little else than the weights.  The walk over the
+// tiles exists once and the code is kept short: with everything inlined in
+// every role it was 160 KB, and its fetches showed at every change of tiles.
 //
 // Every wait is bounded: an expired one records a code in *status and ends
 // the other waits.
@@ -71,6 +71,7 @@ struct PageTcArgs {
   int n_head;
   float scale_log2;
   int box_rows_log2;      // rows of a tensor copy: min(page_size, 128)
+  int q_map;              // FULL: Q comes by tensor copies (G divides 128)
   int64_t pool_rows;      // rows of the layer's pool
   SplitTile* split;
   float* slots;
@@ -244,6 +245,13 @@ __device__ __forceinline__ float2 ex2_fma(float2 x) {
                      __int_as_float(__float_as_int(p.y) + (__float_as_int(t.y) << 23)));
 }
 
+__device__ __forceinline__ void tma_3d(uint32_t dst, const CUtensorMap* map, int x, int y, int z, uint64_t* bar) {
+  asm volatile(
+      "cp.async.bulk.tensor.3d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4, %5}], [%2];" ::"r"(
+          dst),
+      "l"(reinterpret_cast<uint64_t>(map)), "r"(smem_u32(bar)), "r"(x), "r"(y), "r"(z)
+      : "memory");
+}
 __device__ __forceinline__ void tma_2d(uint32_t dst, const CUtensorMap* map, int x, int y, uint64_t* bar) {
   asm volatile(
       "cp.async.bulk.tensor.2d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4}], [%2];" ::"r"(
@@ -272,7 +280,7 @@ __device__ __forceinline__ bool tc_edge(const TcTile& t, int key0, int window) {
 template <int HD, bool SPLIT>
 __global__ void __launch_bounds__(kTcThreads, 1)
     page_tc_kernel(const PageTcArgs a, const __grid_constant__ CUtensorMap k_map,
-                   const __grid_constant__ CUtensorMap v_map) {
+                   const __grid_constant__ CUtensorMap v_map, const __grid_constant__ CUtensorMap q_map) {
   using L = TcSmem<HD, SPLIT>;
   constexpr int NS = L::stages, PARTS = SPLIT ? 2 : 1;
   extern __shared__ __align__(1024) uint8_t smem_raw[];
@@ -309,7 +317,7 @@ __global__ void __launch_bounds__(kTcThreads, 1)
       mbar_init(&kv_empty[i], 1);
     }
     for (int i = 0; i < 2; ++i) {
-      mbar_init(&q_full[i], SPLIT ? 128 : 32);
+      mbar_init(&q_full[i], SPLIT ? 128 : a.q_map ? 1 : 32);
       mbar_init(&q_empty[i], 1);
       mbar_init(&s_full[i], 1);
       mbar_init(&p_full[i], 128);
@@ -318,7 +326,7 @@ __global__ void __launch_bounds__(kTcThreads, 1)
     }
     for (int i = 0; i < kTcTiles; ++i) {
       mbar_init(&t_full[i], 1);
-      mbar_init(&t_empty[i], 11 * 32);   // warps 0-9 and 11
+      mbar_init(&t_empty[i], 11);   // warps 0-9 and 11
     }
     mbar_init(done, 1);
     *abort_flag = 0;
@@ -350,14 +358,15 @@ __global__ void __launch_bounds__(kTcThreads, 1)
       }
     return true;
   };
-  // The n-th tile of the share, copied out of the ring.
+  // The n-th tile of the share, copied out of the ring (whole warps).
   auto take_tile = [&](int n, TcTile& t) -> bool {
     if (!wait(&t_full[n % kTcTiles], (n / kTcTiles) & 1, 90)) return false;
     const int4* src = reinterpret_cast<const int4*>(&tiles[n % kTcTiles]);
     int4* dst = reinterpret_cast<int4*>(&t);
 #pragma unroll
     for (int i = 0; i < 4; ++i) dst[i] = src[i];
-    mbar_arrive(&t_empty[n % kTcTiles]);
+    __syncwarp();
+    if (lane == 0) mbar_arrive(&t_empty[n % kTcTiles]);
     return t.units > 0;
   };
 
@@ -377,11 +386,17 @@ __global__ void __launch_bounds__(kTcThreads, 1)
       TcTile t;
       for (int nt = 0; ok && take_tile(nt, t); ++nt) {
         if (nt == 0) fence_async_proxy();
-        for (int u = 0; ok && u < t.units; ++u) {
+        // the unit's row in the pool; looked up a unit ahead
+        auto look_up = [&](int u) {
           const int p = t.key0 + u * kTcBk + bx * rows_box;
           int64_t row = -1;
           if (bh < HD / 64 && p < t.hi && p + rows_box > t.lo) row = page_row(w.b, a.c, t.s, t.h, p);
-          const int y = (int)(row < 0 ? a.pool_rows : row);
+          return (int)(row < 0 ? a.pool_rows : row);
+        };
+        int next_y = look_up(0);
+        for (int u = 0; ok && u < t.units; ++u) {
+          const int y = next_y;
+          if (u + 1 < t.units) next_y = look_up(u + 1);
 #pragma unroll
           for (int kv = 0; kv < 2; ++kv, ++n) {
             const int st = n % NS;
@@ -411,7 +426,7 @@ __global__ void __launch_bounds__(kTcThreads, 1)
       __syncwarp();   // the sums are read: the ring may take their place
       constexpr int LR = HD / 8, RI = 32 / LR;   // lanes per row of Q, rows per step
       const int ch = lane % LR, rl = lane / LR;
-      const int step_tok = RI / w.G, step_g = RI % w.G;
+      const int G = (int)w.G.d, step_tok = w.G.div(RI), step_g = RI - step_tok * G;
       int fills[2] = {0, 0};
       bool ok = true;
       for (int nt = 0; ok; ++nt) {
@@ -421,7 +436,7 @@ __global__ void __launch_bounds__(kTcThreads, 1)
         const bool more = sh.u < sh.u_end;
         if (more) {
           const TileAt& at = sh.at;
-          const int u_hi = sh.u_end - sh.u < at.units - sh.off ? sh.off + (int)(sh.u_end - sh.u) : at.units;
+          const int u_hi = min(at.units, sh.off + (sh.u_end - sh.u));
           t.h = at.h;
           t.s = at.s;
           t.q0 = at.q0;
@@ -432,8 +447,8 @@ __global__ void __launch_bounds__(kTcThreads, 1)
           t.units = u_hi - sh.off;
           t.lo = at.lo;
           t.hi = at.hi;
-          t.p_min = at.first + t.row0 / w.G;
-          t.p_max = at.first + (t.row0 + t.rows - 1) / w.G;
+          t.p_min = at.first + w.G.div(t.row0);
+          t.p_max = at.first + w.G.div(t.row0 + t.rows - 1);
           t.whole = sh.off == 0 && u_hi == at.units;
           t.slot = sh.off == 0 && nt > 0 ? 2 * blockIdx.x + 1 : 2 * blockIdx.x;
           if (sh.off == 0 && u_hi < at.units) {
@@ -443,7 +458,7 @@ __global__ void __launch_bounds__(kTcThreads, 1)
             rec.rows = t.rows;
             rec.q0 = at.q0;
             rec.slot = t.slot;
-            rec.last = cta_of_unit(sh.u + at.units - 1, sh.total, sh.n);
+            rec.last = sh.deal.cta_of(sh.u + at.units - 1);
           }
           sh.u += t.units;
           sh.off = 0;
@@ -455,39 +470,52 @@ __global__ void __launch_bounds__(kTcThreads, 1)
         if (!more) break;
         if constexpr (!SPLIT) {
           const int halves = t.rows > 128 ? 2 : 1;
-          const __half* src = static_cast<const __half*>(a.q) + ((int64_t)t.q0 * a.n_head + t.h * w.G) * HD + ch * 8;
-          int tok = (t.row0 + rl) / w.G, g = (t.row0 + rl) - tok * w.G;
-          for (int i = 0; i < halves && ok; ++i) {
-            if (fills[i] > 0) ok = __all_sync(0xffffffffu, wait(&q_empty[i], (fills[i] - 1) & 1, 80));
-            ++fills[i];
-            if (!ok) break;
-            const uint32_t qd = smem_u32(Qs) + i * L::half_q + (ch / 8) * (128 * 128);
-#pragma unroll 4
-            for (int r = rl; r < 128; r += RI) {
-              const bool live = i * 128 + r < t.rows;
-              cp_async16(qd + r * 128 + (((ch & 7) ^ (r & 7)) << 4), live ? src + ((int64_t)tok * a.n_head + g) * HD : src,
-                         live);
-              tok += step_tok;
-              g += step_g;
-              if (g >= w.G) {
-                g -= w.G;
-                ++tok;
-              }
+          if (a.q_map) {
+            // 128/G tokens x G heads x 64 dims a copy: the rows' own order.
+            // Rows past the sequence are other tokens' and are not written.
+            const int z = t.q0 + w.G.div(t.row0), dz = w.G.div(128);
+            for (int i = 0; i < halves && ok; ++i) {
+              if (fills[i] > 0) ok = __all_sync(0xffffffffu, wait(&q_empty[i], (fills[i] - 1) & 1, 80));
+              ++fills[i];
+              if (!ok) break;
+              if (lane == 0) mbar_arrive_expect_tx(&q_full[i], L::half_q);
+              __syncwarp();
+              if (lane < HD / 64)
+                tma_3d(smem_u32(Qs) + i * L::half_q + lane * (128 * 128), &q_map, lane * 64, t.h * G, z + i * dz, &q_full[i]);
             }
-            cp_async_commit();
+          } else {
+            const __half* src = static_cast<const __half*>(a.q) + ((int64_t)t.q0 * a.n_head + t.h * G) * HD + ch * 8;
+            int tok = w.G.div(t.row0 + rl), g = (t.row0 + rl) - tok * G;
+            for (int i = 0; i < halves && ok; ++i) {
+              if (fills[i] > 0) ok = __all_sync(0xffffffffu, wait(&q_empty[i], (fills[i] - 1) & 1, 80));
+              ++fills[i];
+              if (!ok) break;
+              const uint32_t qd = smem_u32(Qs) + i * L::half_q + (ch / 8) * (128 * 128);
+#pragma unroll 2
+              for (int r = rl; r < 128; r += RI) {
+                const bool live = i * 128 + r < t.rows;
+                cp_async16(qd + r * 128 + (((ch & 7) ^ (r & 7)) << 4),
+                           live ? src + ((int64_t)tok * a.n_head + g) * HD : src, live);
+                tok += step_tok;
+                g += step_g;
+                if (g >= G) {
+                  g -= G;
+                  ++tok;
+                }
+              }
+              cp_async_wait_all();
+              fence_async_proxy();
+              mbar_arrive(&q_full[i]);
+            }
           }
-          if (halves == 2) {
-            cp_async_wait<1>();
-            fence_async_proxy();
-            if (ok) mbar_arrive(&q_full[0]);
-          }
-          cp_async_wait<0>();
-          fence_async_proxy();
-          if (ok) mbar_arrive(&q_full[halves - 1]);
         }
         if (sh.u < sh.u_end) next_tile(w, sh.at);
       }
       if (lane == 0) a.split[blockIdx.x] = rec;
+      // the queries' copies have landed before the CTA may end
+      if (!SPLIT && a.q_map)
+        for (int i = 0; i < 2; ++i)
+          if (fills[i] > 0) mbar_wait_bounded(&q_full[i], (fills[i] - 1) & 1, a.status, 81);
     } else if (warp == 11) {
       // ---------------- V of units that some rows do not see whole ----------------
       int n = 0;
@@ -547,52 +575,44 @@ __global__ void __launch_bounds__(kTcThreads, 1)
                      v_desc = uniform(desc_n(smem_u32(Ts))), tm = uniform(tmem);
       int n = 0, nq[2] = {0, 0}, np[2] = {0, 0};   // ring position; Q and P tiles of each half so far
       bool ok = true;
-      auto qk = [&](int i, int st) {
-        const uint32_t kd = uniform(k_desc + st * (L::tile >> 4)), qd = q_desc + i * PARTS * (L::half_q >> 4);
-        if (elect_one()) {
+      auto qk = [&](int i, uint32_t kd) {          // in the elected lane
+        const uint32_t qd = q_desc + i * PARTS * (L::half_q >> 4);
 #pragma unroll
-          for (int part = 0; part < PARTS; ++part)
+        for (int part = 0; part < PARTS; ++part)
 #pragma unroll
-            for (int ks = 0; ks < HD / 16; ++ks) {
-              const uint32_t off = ((ks / 4) * (128 * 128) + (ks % 4) * 32) >> 4;
-              tc_mma_ss(tm + i * 128, qd + part * (L::half_q >> 4) + off, kd + off, id_s, (part | ks) != 0);
-            }
-          tc_commit(&s_full[i]);
-        }
-        __syncwarp();
+          for (int ks = 0; ks < HD / 16; ++ks) {
+            const uint32_t off = ((ks / 4) * (128 * 128) + (ks % 4) * 32) >> 4;
+            tc_mma_ss(tm + i * 128, qd + part * (L::half_q >> 4) + off, kd + off, id_s, (part | ks) != 0);
+          }
+        tc_commit(&s_full[i]);
       };
-      auto pv = [&](int i, int st, int h, bool acc) {   // 64 positions
-        const uint32_t vd = uniform(v_desc + st * (L::tile >> 4)), add = uniform(acc);
-        if (elect_one()) {
+      auto pv = [&](int i, uint32_t vd, int h, uint32_t acc) {   // 64 positions; in the elected lane
 #pragma unroll
-          for (int part = 0; part < PARTS; ++part)
+        for (int part = 0; part < PARTS; ++part)
 #pragma unroll
-            for (int k4 = 0; k4 < 4; ++k4) {
-              const int ks = h * 4 + k4;
-              const uint32_t p = SPLIT ? (ks / 2) * 32 + part * 16 + (ks & 1) * 8 : ks * 8;
-              tc_mma_ts(tm + 256 + i * 128, tm + i * 128 + p, vd + ks * (2048 >> 4), id_o, (part | k4) ? 1u : add);
-            }
-        }
-        __syncwarp();
-      };
-      auto commit = [&](uint64_t* bar) {
-        if (elect_one()) tc_commit(bar);
-        __syncwarp();
+          for (int k4 = 0; k4 < 4; ++k4) {
+            const int ks = h * 4 + k4;
+            const uint32_t p = SPLIT ? (ks / 2) * 32 + part * 16 + (ks & 1) * 8 : ks * 8;
+            tc_mma_ts(tm + 256 + i * 128, tm + i * 128 + p, vd + ks * (2048 >> 4), id_o, (part | k4) ? 1u : acc);
+          }
       };
       // S of a tile's first unit
       auto open_tile = [&](const TcTile& t) {
-        ok = ok && wait(&k_full[(n / 2) % NS], (n / 2 / NS) & 1, 60);
+        ok = wait(&k_full[(n / 2) % NS], (n / 2 / NS) & 1, 60);
+        const uint32_t kd = uniform(k_desc + (n % NS) * (L::tile >> 4));
 #pragma unroll
         for (int i = 0; i < 2; ++i)
           if (i == 0 || t.rows > 128) {
             ok = ok && wait(&q_full[i], nq[i]++ & 1, 61);
-            ok = __all_sync(0xffffffffu, ok);
-            if (!ok) return;
             tc_after();
-            qk(i, n % NS);
-            if (!SPLIT && t.units == 1) commit(&q_empty[i]);
+            if (elect_one()) {
+              qk(i, kd);
+              if (!SPLIT && t.units == 1) tc_commit(&q_empty[i]);
+            }
+            __syncwarp();
           }
-        commit(&kv_empty[n % NS]);
+        if (elect_one()) tc_commit(&kv_empty[n % NS]);
+        __syncwarp();
         ++n;
       };
       TcTile t;
@@ -600,38 +620,48 @@ __global__ void __launch_bounds__(kTcThreads, 1)
       bool have = take_tile(nt++, t);
       if (have) open_tile(t);
       while (ok && have) {
+        const bool two = t.rows > 128;
         for (int u = 0; u < t.units; ++u) {
           const int sv = n % NS, sk = (n + 1) % NS;
-          const bool more = u + 1 < t.units, two = t.rows > 128;
-          ok = wait(&v_full[(n / 2) % NS], (n / 2 / NS) & 1, 62) && wait(&v_ok[(n / 2) % NS], (n / 2 / NS) & 1, 66);
+          const bool more = u + 1 < t.units;
+          const uint32_t vd = uniform(v_desc + sv * (L::tile >> 4)), kd = uniform(k_desc + sk * (L::tile >> 4)),
+                         add = uniform(u > 0);
+          // K of the next unit and V of this one came while the softmax ran:
+          // these waits are not on its path
+          ok = wait(&v_ok[(n / 2) % NS], (n / 2 / NS) & 1, 62) &&
+               (!more || wait(&k_full[((n + 1) / 2) % NS], ((n + 1) / 2 / NS) & 1, 65));
 #pragma unroll
           for (int i = 0; i < 2; ++i)
             if (i == 0 || two) {
               ok = ok && wait(&p_full[i], np[i] & 1, 63);
               tc_after();
-              pv(i, sv, 0, u > 0);
+              if (elect_one()) pv(i, vd, 0, add);
+              __syncwarp();
               ok = ok && wait(&p_full[2 + i], np[i]++ & 1, 64);
               tc_after();
-              pv(i, sv, 1, true);
-              if (!more) commit(&o_full[i]);
-              if (i == 1 || !two) commit(&kv_empty[sv]);
-              if (more) {
-                if (i == 0) ok = ok && wait(&k_full[((n + 1) / 2) % NS], ((n + 1) / 2 / NS) & 1, 65);
-                qk(i, sk);
-                if (!SPLIT && u + 2 == t.units) commit(&q_empty[i]);
-                if (i == 1 || !two) commit(&kv_empty[sk]);
+              if (elect_one()) {
+                pv(i, vd, 1, 1u);
+                if (i == 1 || !two) tc_commit(&kv_empty[sv]);
+                if (more) {
+                  qk(i, kd);
+                  if (!SPLIT && u + 2 == t.units) tc_commit(&q_empty[i]);
+                  if (i == 1 || !two) tc_commit(&kv_empty[sk]);
+                } else {
+                  tc_commit(&o_full[i]);
+                }
               }
+              __syncwarp();
             }
           n += more ? 2 : 1;
           ok = __all_sync(0xffffffffu, ok);
           if (!ok) break;
         }
         if (!ok) break;
-        have = take_tile(nt++, t);
-        have = __all_sync(0xffffffffu, have);
+        have = __all_sync(0xffffffffu, take_tile(nt++, t));
         if (have) open_tile(t);
       }
-      commit(done);   // every product has completed before TMEM is given back
+      if (elect_one()) tc_commit(done);   // every product has completed before TMEM is given back
+      __syncwarp();
       mbar_wait_bounded(done, 0, a.status, 67);
     }
   } else {
@@ -650,9 +680,9 @@ __global__ void __launch_bounds__(kTcThreads, 1)
       int p = -1;
       int64_t e0 = 0;          // the row in q and out
       {
-        const int rr = t.row0 + (on ? r : 0), tok = rr / w.G;
+        const int rr = t.row0 + (on ? r : 0), tok = w.G.div(rr), G = (int)w.G.d;
         if (on) p = t.first + tok;
-        e0 = ((int64_t)(t.q0 + tok) * a.n_head + t.h * w.G + (rr - tok * w.G)) * HD;
+        e0 = ((int64_t)(t.q0 + tok) * a.n_head + t.h * G + (rr - tok * G)) * HD;
       }
       if constexpr (SPLIT) {
         // ---- the warp's 32 rows of Q, a row (hd 64: two) per step, as two parts ----

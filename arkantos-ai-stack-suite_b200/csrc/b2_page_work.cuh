@@ -18,9 +18,32 @@
 
 namespace b2 {
 
+// Division by a number fixed for a call, for 0 <= n < 2^31: the product with
+// floor(2^(31 + l) / d) + 1, l = ceil(log2 d), shifted (exact for 31-bit n).
+// The kernels divide row numbers by G at every change of tiles, and the code
+// of a general division is fetched cold there.
+struct FastDiv {
+  uint32_t d = 1, magic = 0, shift = 0;
+  __host__ static FastDiv of(uint32_t d) {
+    FastDiv f;
+    f.d = d;
+    if (d > 1) {
+      uint32_t l = 0;
+      while ((1u << l) < d) ++l;
+      f.magic = (uint32_t)(((uint64_t)1 << (31 + l)) / d + 1);
+      f.shift = l - 1;
+    }
+    return f;
+  }
+  __device__ __forceinline__ int div(int n) const { return magic ? (int)(__umulhi((uint32_t)n, magic) >> shift) : n; }
+};
+
 struct PageWork {
   PageSeqs b;
-  int ps_log2, n_kv, G, window, rows, bk;   // rows of a tile, positions of a unit
+  FastDiv G;                                     // query heads of a kv head
+  int ps_log2, n_kv, window, rows_log2, bk_log2;   // rows of a tile, positions of a unit
+  __host__ __device__ int rows() const { return 1 << rows_log2; }
+  __host__ __device__ int bk() const { return 1 << bk_log2; }
 };
 
 struct TileAt {
@@ -33,35 +56,46 @@ struct TileAt {
 };
 
 __device__ __forceinline__ int tiles_of(const PageWork& w, const SeqSpan& sp) {
-  return (sp.len * w.G + w.rows - 1) / w.rows;
+  return (sp.len * (int)w.G.d + w.rows() - 1) >> w.rows_log2;
 }
 
 __device__ __forceinline__ void tile_range(const PageWork& w, const SeqSpan& sp, int t, TileAt& a) {
-  const int total = sp.len * w.G;
-  const int last = min((t + 1) * w.rows, total) - 1;
-  const int p_lo = sp.first + (t * w.rows) / w.G, p_hi = sp.first + last / w.G;
+  const int total = sp.len * (int)w.G.d;
+  const int last = min((t + 1) << w.rows_log2, total) - 1;
+  const int p_lo = sp.first + w.G.div(t << w.rows_log2), p_hi = sp.first + w.G.div(last);
   const int lo = w.window > 0 ? max(0, p_lo - w.window + 1) : 0;
   const int hi = max(0, min(p_hi + 1, sp.kv));
-  a.lo_unit = lo / w.bk;
-  a.units = max(1, (hi + w.bk - 1) / w.bk - a.lo_unit);
+  a.lo_unit = lo >> w.bk_log2;
+  a.units = max(1, ((hi + w.bk() - 1) >> w.bk_log2) - a.lo_unit);
   a.lo = lo;
   a.hi = hi;
 }
 
 __device__ __forceinline__ void tile_load(const PageWork& w, TileAt& a) {
   const SeqSpan sp = seq_span(w.b, w.ps_log2, a.s);
-  a.rows_total = sp.len * w.G;
+  a.rows_total = sp.len * (int)w.G.d;
   a.first = sp.first;
   a.q0 = sp.q0;
   tile_range(w, sp, a.t, a);
 }
 
+// How the units of a call fall to its CTAs: n CTAs get work, the first `rem`
+// of them base + 1 units, the others base.  Fewer than 2^31 units.
+struct Deal {
+  int n, base, rem;
+  __device__ __forceinline__ int start(int cta) const { return cta * base + min(cta, rem); }
+  // the CTA that holds unit u
+  __device__ __forceinline__ int cta_of(int u) const {
+    const int cut = rem * (base + 1);
+    return u < cut ? (int)((unsigned)u / (unsigned)(base + 1)) : rem + (int)((unsigned)(u - cut) / (unsigned)base);
+  }
+};
+
 // The share of the calling CTA: units [u, u_end), the first of them `off`
-// units into tile `at`.  n is the number of CTAs that got work; total the
-// units of the call.
+// units into tile `at`.
 struct Share {
-  int64_t u, u_end, total;
-  int n;
+  Deal deal;
+  int u, u_end;
   int off;
   TileAt at;
 };
@@ -70,7 +104,7 @@ struct Share {
 // memory of n_seq ints.  A barrier must follow.
 __device__ __forceinline__ void sum_units(const PageWork& w, int* sums) {
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, warps = blockDim.x >> 5;
-  if (w.b.max_q * w.G <= w.rows) {   // one tile at most: a thread per sequence
+  if (w.b.max_q * (int64_t)w.G.d <= w.rows()) {   // one tile at most: a thread per sequence
     for (int s = tid; s < w.b.n_seq; s += blockDim.x) {
       const SeqSpan sp = seq_span(w.b, w.ps_log2, s);
       const int tiles = tiles_of(w, sp);
@@ -103,20 +137,22 @@ __device__ __forceinline__ void sum_units(const PageWork& w, int* sums) {
 // for a CTA without work.
 __device__ __forceinline__ bool find_share(const PageWork& w, int cta, int ctas, const int* sums, Share& sh) {
   const int lane = threadIdx.x & 31;
-  int64_t per_head = 0;
+  int per_head = 0;
   for (int s0 = 0; s0 < w.b.n_seq; s0 += 32) {
     int v = s0 + lane < w.b.n_seq ? sums[s0 + lane] : 0;
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
     per_head += v;
   }
-  sh.total = per_head * w.n_kv;
-  sh.n = (int)(sh.total < ctas ? sh.total : ctas);
-  if (cta >= sh.n) return false;
-  sh.u = sh.total * cta / sh.n;
-  sh.u_end = sh.total * (cta + 1) / sh.n;
-  sh.at.h = (int)(sh.u / per_head);
-  int64_t rem = sh.u - sh.at.h * per_head;
+  const int total = per_head * w.n_kv;
+  sh.deal.n = min(total, ctas);
+  if (cta >= sh.deal.n) return false;
+  sh.deal.base = (int)((unsigned)total / (unsigned)sh.deal.n);
+  sh.deal.rem = total - sh.deal.base * sh.deal.n;
+  sh.u = sh.deal.start(cta);
+  sh.u_end = sh.deal.start(cta + 1);
+  sh.at.h = (int)((unsigned)sh.u / (unsigned)per_head);
+  int rem = sh.u - sh.at.h * per_head;
   sh.at.s = -1;
   for (int s0 = 0; s0 < w.b.n_seq; s0 += 32) {
     const int v = s0 + lane < w.b.n_seq ? sums[s0 + lane] : 0;
@@ -156,14 +192,14 @@ __device__ __forceinline__ bool find_share(const PageWork& w, int cta, int ctas,
     }
     rem -= __shfl_sync(0xffffffffu, run, 31);
   }
-  sh.off = (int)rem;
+  sh.off = rem;
   tile_load(w, sh.at);
   return true;
 }
 
 // The tile after `a` (which has a successor: the caller has units left).
 __device__ __forceinline__ void next_tile(const PageWork& w, TileAt& a) {
-  if ((a.t + 1) * w.rows < a.rows_total) {
+  if ((a.t + 1) << w.rows_log2 < a.rows_total) {
     ++a.t;
   } else {
     a.t = 0;
@@ -177,11 +213,6 @@ __device__ __forceinline__ void next_tile(const PageWork& w, TileAt& a) {
     } while (true);
   }
   tile_load(w, a);
-}
-
-// The CTA that holds unit u: the largest c with floor(total·c / n) <= u.
-__device__ __forceinline__ int cta_of_unit(int64_t u, int64_t total, int n) {
-  return (int)(((u + 1) * n - 1) / total);
 }
 
 // What the finishing kernel needs about the tile that starts in a CTA's share
