@@ -81,7 +81,6 @@ struct PageTcArgs {
 constexpr int kTcRows = 256, kTcBk = 128, kTcThreads = 384;
 constexpr float kTcOffset = 7.f, kTcRaise = 8.f;
 constexpr int kTcPolls = 1 << 22;   // polls of a wait, each suspended by the hardware for a while
-constexpr int kTcFmaEvery = 8;   // one pair of weights in four is formed on the FMA pipe
 
 template <int HD, bool SPLIT>
 struct TcSmem {
@@ -228,23 +227,6 @@ __device__ __forceinline__ float max3_nan(float a, float b, float c) {
   asm("max.NaN.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
   return d;
 }
-// 2^x of two values on the FMA pipe: x = n + f with |f| <= 1/2, 2^f by the
-// cubic of least relative error (7.5e-5, fitted by exchange, a quarter of
-// what the rounding of a weight to fp16 costs), n added to the exponent.
-// Arguments below -125 count as -125.
-__device__ __forceinline__ float2 ex2_fma(float2 x) {
-  x = make_float2(max_nan(x.x, -125.f), max_nan(x.y, -125.f));
-  const float2 big = make_float2(12582912.f, 12582912.f);   // 1.5·2^23: the sum's low bits are n
-  const float2 t = add2(x, big);
-  const float2 n = add2(t, make_float2(-12582912.f, -12582912.f));
-  const float2 f = fma2(n, make_float2(-1.f, -1.f), x);
-  float2 p = fma2(f, make_float2(0.0551716685f, 0.0551716685f), make_float2(0.242611125f, 0.242611125f));
-  p = fma2(p, f, make_float2(0.693260968f, 0.693260968f));
-  p = fma2(p, f, make_float2(0.999928057f, 0.999928057f));
-  return make_float2(__int_as_float(__float_as_int(p.x) + (__float_as_int(t.x) << 23)),
-                     __int_as_float(__float_as_int(p.y) + (__float_as_int(t.y) << 23)));
-}
-
 __device__ __forceinline__ void tma_3d(uint32_t dst, const CUtensorMap* map, int x, int y, int z, uint64_t* bar) {
   asm volatile(
       "cp.async.bulk.tensor.3d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4, %5}], [%2];" ::"r"(
@@ -339,6 +321,9 @@ __global__ void __launch_bounds__(kTcThreads, 1)
                  : "memory");
     asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
   }
+  if (warp == 9 && lane < 3)
+    asm volatile("prefetch.tensormap [%0];" ::"l"(reinterpret_cast<uint64_t>(lane == 0 ? &k_map : lane == 1 ? &v_map : &q_map))
+                 : "memory");
   pdl_wait();
   const PageWork& w = a.w;
   sum_units(w, reinterpret_cast<int*>(Ts));
@@ -741,7 +726,9 @@ __global__ void __launch_bounds__(kTcThreads, 1)
 #pragma unroll
         for (int i = 4; i < 124; i += 8)
 #pragma unroll
-          for (int e = 0; e < 4; ++e) top[e] = max3_nan(top[e], s[i + e], s[i + 4 + e]);
+          for (int e = 0; e < 4; ++e)
+            top[e] = max3_nan(top[e], s[i + e], s[i + 4 + e]);
+
 #pragma unroll
         for (int e = 0; e < 4; ++e) top[e] = max_nan(top[e], s[124 + e]);
         const float high = max_nan(max_nan(top[0], top[1]), max_nan(top[2], top[3])) * c;
@@ -770,19 +757,9 @@ __global__ void __launch_bounds__(kTcThreads, 1)
 #pragma unroll
           for (int i = h * 32; i < h * 32 + 32; i += 2) {
             const float2 x = fma2(make_float2(s[i], s[i + 1]), make_float2(c, c), make_float2(rs, rs));
-            float2 e;
-            if (!SPLIT && i % kTcFmaEvery == kTcFmaEvery - 2) {
-              e = ex2_fma(x);
-              if (edge) {
-                if (i >= hi || i < lo) e.x = 0.f;
-                if (i + 1 >= hi || i + 1 < lo) e.y = 0.f;
-              }
-            } else {
-              e = make_float2(ex2(x.x), ex2(x.y));
-            }
-            s[i] = e.x;
-            s[i + 1] = e.y;
-            sum[(i >> 1) & 1] = add2(sum[(i >> 1) & 1], e);
+            s[i] = ex2(x.x);
+            s[i + 1] = ex2(x.y);
+            sum[(i >> 1) & 1] = add2(sum[(i >> 1) & 1], make_float2(s[i], s[i + 1]));
           }
           // FULL: 64 columns of weights over S's first 64.  SPLIT: the two
           // parts of 32 positions over their own 32 columns.
