@@ -740,6 +740,11 @@ int b2_page_attn(const b2_page_cache* cache, int32_t layer, const b2_page_batch*
     void* scratch = nullptr;
     B2_CUDA_TRY(cudaMallocAsync(&scratch, need, s));
     a.ws = static_cast<uint8_t*>(scratch);
+    if (cudaMemsetAsync(scratch, 0, page_attn_counters(a), s) != cudaSuccess) {
+      cudaFreeAsync(scratch, s);
+      set_error("page_attn: scratch");
+      return B2_ERR_CUDA;
+    }
   }
   rc = launch_page_attn(a, s);
   if (!workspace) cudaFreeAsync(a.ws, s);

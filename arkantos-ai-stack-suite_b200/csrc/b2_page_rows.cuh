@@ -44,7 +44,7 @@ struct PageRowsArgs {
   void* out;
   int n_head, q_f32;
   float scale_log2;          // scale · log2(e)
-  SplitTile* split;
+  unsigned* counters;
   float* slots;
 };
 
@@ -76,11 +76,6 @@ __device__ __forceinline__ void mma16816(float (&d)[4], const uint32_t (&a)[4], 
       "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
       : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
       : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
-}
-__device__ __forceinline__ float ex2(float x) {
-  float y;
-  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
-  return y;
 }
 __device__ __forceinline__ uint32_t h2(float lo, float hi) {
   const __half2 v = __floats2half2_rn(lo, hi);
@@ -151,12 +146,7 @@ __global__ void __launch_bounds__(kRowsThreads) page_rows_kernel(const PageRowsA
   sum_units(w, sums);
   __syncthreads();
   const bool have = find_share(w, blockIdx.x, gridDim.x, sums, sh);   // every warp finds the same place
-  SplitTile rec = {};
-  rec.last = -1;
-  if (!have) {
-    if (tid == 0) a.split[blockIdx.x] = rec;
-    return;
-  }
+  if (!have) return;
   __syncthreads();   // sums are read; the stages take their place
 
   const int stage_bytes = rows_stage_bytes<HD, KQ, VQ>(c.rb_k, c.rb_v);
@@ -169,7 +159,6 @@ __global__ void __launch_bounds__(kRowsThreads) page_rows_kernel(const PageRowsA
   float* scale_v = reinterpret_cast<float*>(conv_v + RowsSmem<HD>::tile);
   const float off = p_offset(c.type_v);
 
-  bool first_tile = true;
   while (sh.u < sh.u_end) {
     const TileAt at = sh.at;
     const int u_lo = sh.off, u_hi = min(at.units, u_lo + (sh.u_end - sh.u));
@@ -496,9 +485,9 @@ __global__ void __launch_bounds__(kRowsThreads) page_rows_kernel(const PageRowsA
         o[d][1] += o[d][3];
       }
     }
-    const bool whole = u_lo == 0 && u_hi == at.units;
-    const int slot = u_lo == 0 && !first_tile ? 2 * blockIdx.x + 1 : 2 * blockIdx.x;
-    float* part = a.slots + (int64_t)slot * slot_floats(w.rows(), HD);
+    const Split split = split_of(sh, blockIdx.x, u_hi);
+    const bool whole = split.n == 0;
+    float* part = a.slots + (int64_t)split.slot * slot_floats(w.rows(), HD);
     float* part_ml = part + w.rows() * HD;
 
     auto out_ptr = [&](int r) -> int64_t {
@@ -563,6 +552,23 @@ __global__ void __launch_bounds__(kRowsThreads) page_rows_kernel(const PageRowsA
         }
         put2(r, d, x, y);
       }
+      if (!whole) {
+        // all warps' shares of the rows are written before one counts the part
+        __threadfence();
+        __syncthreads();
+        if (warp == 0) {
+          const bool last = part_arrives(a.counters + split.cta0 * 8, split.n);
+          if (lane == 0) *reinterpret_cast<int*>(smem) = last;
+        }
+        __syncthreads();
+        if (*reinterpret_cast<volatile int*>(smem)) {
+          constexpr int R = WROWS / 4;
+          const int r = warp * R;
+          if (r < rows)
+            join_parts<HD, R, 16 / R>(a.slots, w.rows(), split, r, rows - r, out_ptr(min(r + lane, rows - 1)), a.out,
+                             a.q_f32 != 0);
+        }
+      }
       __syncthreads();   // the stages are free for the next tile
     } else {
       const float i0 = !whole ? 1.f : l0 != 0.f ? 1.f / l0 : 0.f, i1 = !whole ? 1.f : l1 != 0.f ? 1.f / l1 : 0.f;
@@ -574,29 +580,26 @@ __global__ void __launch_bounds__(kRowsThreads) page_rows_kernel(const PageRowsA
         if constexpr (!SPLIT)
           if (r + 8 < rows) put2(r + 8, i, o[d][2] * i1, o[d][3] * i1);
       }
-      if (!whole && j == 0) {
-        if (r < rows) *reinterpret_cast<float2*>(part_ml + 2 * r) = make_float2(m0, l0);
-        if constexpr (!SPLIT)
-          if (r + 8 < rows) *reinterpret_cast<float2*>(part_ml + 2 * (r + 8)) = make_float2(m1, l1);
+      if (!whole && wm * WROWS < rows) {
+        if (j == 0) {
+          if (r < rows) *reinterpret_cast<float2*>(part_ml + 2 * r) = make_float2(m0, l0);
+          if constexpr (!SPLIT)
+            if (r + 8 < rows) *reinterpret_cast<float2*>(part_ml + 2 * (r + 8)) = make_float2(m1, l1);
+        }
+        if (part_arrives(a.counters + split.cta0 * 8 + warp, split.n)) {
+          constexpr int R = HD == 256 ? 4 : 8;
+          for (int r0 = wm * WROWS; r0 < min((wm + 1) * WROWS, rows); r0 += R)
+            join_rows<HD, R>(a.slots, w.rows(), split, r0, rows - r0, out_ptr(min(r0 + lane, rows - 1)), a.out,
+                             a.q_f32 != 0);
+        }
       }
       __syncthreads();
     }
 
-    if (u_lo == 0 && u_hi < at.units) {   // starts here, ends elsewhere
-      rec.h = at.h;
-      rec.s = at.s;
-      rec.t = at.t;
-      rec.rows = rows;
-      rec.q0 = at.q0;
-      rec.slot = slot;
-      rec.last = sh.deal.cta_of(sh.u + at.units - 1);
-    }
     sh.u += u_hi - u_lo;
     sh.off = 0;
-    first_tile = false;
     if (sh.u < sh.u_end) next_tile(w, sh.at);
   }
-  if (tid == 0) a.split[blockIdx.x] = rec;
 }
 
 int launch_page_rows_64(const PageRowsArgs& a, bool split, int wm, cudaStream_t s);
@@ -632,9 +635,7 @@ int launch_page_rows_one(const PageRowsArgs& a, cudaStream_t s) {
     known.store(per_sm, std::memory_order_relaxed);
   }
   const int ctas = per_sm * sm_count();
-  const int rc = launch_pdl(kern, dim3(ctas), dim3(kRowsThreads), (size_t)smem, s, a, stages);
-  if (rc != B2_OK) return rc;
-  return launch_page_join(a.w, a.split, a.slots, ctas, HD, a.n_head, a.out, a.q_f32 != 0, s);
+  return launch_pdl(kern, dim3(ctas), dim3(kRowsThreads), (size_t)smem, s, a, stages);
 }
 
 template <int HD>

@@ -57,9 +57,7 @@ int launch(const PageTcArgs& a, const CUtensorMap& km, const CUtensorMap& vm, co
     ready[dev].store(1, std::memory_order_relaxed);
   }
   const int ctas = sm_count();   // one per SM: the kernel takes all of TMEM
-  const int rc = launch_pdl(kern, dim3(ctas), dim3(kTcThreads), (size_t)TcSmem<HD, SPLIT>::bytes, s, a, km, vm, qm);
-  if (rc != B2_OK) return rc;
-  return launch_page_join(a.w, a.split, a.slots, ctas, HD, a.n_head, a.out, SPLIT, s);
+  return launch_pdl(kern, dim3(ctas), dim3(kTcThreads), (size_t)TcSmem<HD, SPLIT>::bytes, s, a, km, vm, qm);
 }
 
 }  // namespace

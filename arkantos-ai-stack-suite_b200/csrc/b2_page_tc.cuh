@@ -73,7 +73,7 @@ struct PageTcArgs {
   int box_rows_log2;      // rows of a tensor copy: min(page_size, 128)
   int q_map;              // FULL: Q comes by tensor copies (G divides 128)
   int64_t pool_rows;      // rows of the layer's pool
-  SplitTile* split;
+  unsigned* counters;
   float* slots;
   int* status;
 };
@@ -248,8 +248,7 @@ struct TcTile {
   int row0, rows;                 // first row (of the sequence's) and rows of the tile
   int key0, units;                // first position and units of this CTA's part; units = 0: no more tiles
   int lo, hi, p_min, p_max;       // positions attended to; those of the first and last row
-  int whole, slot;                // whether the part is the whole tile; the slot of a partial result
-  int pad[2];
+  Split split;                    // of a tile that other CTAs share
 };
 static_assert(sizeof(TcTile) == 64, "four 16-byte words");
 constexpr int kTcTiles = 4;       // ring of tiles
@@ -404,8 +403,6 @@ __global__ void __launch_bounds__(kTcThreads, 1)
     } else if (warp == 10) {
       // ---------------- tiles, Q (FULL) ----------------
       Share sh;
-      SplitTile rec = {};
-      rec.last = -1;
       const bool have = find_share(w, blockIdx.x, gridDim.x, reinterpret_cast<const int*>(Ts), sh);
       if (!have) sh.u = sh.u_end = 0;
       __syncwarp();   // the sums are read: the ring may take their place
@@ -434,17 +431,7 @@ __global__ void __launch_bounds__(kTcThreads, 1)
           t.hi = at.hi;
           t.p_min = at.first + w.G.div(t.row0);
           t.p_max = at.first + w.G.div(t.row0 + t.rows - 1);
-          t.whole = sh.off == 0 && u_hi == at.units;
-          t.slot = sh.off == 0 && nt > 0 ? 2 * blockIdx.x + 1 : 2 * blockIdx.x;
-          if (sh.off == 0 && u_hi < at.units) {
-            rec.h = at.h;
-            rec.s = at.s;
-            rec.t = at.t;
-            rec.rows = t.rows;
-            rec.q0 = at.q0;
-            rec.slot = t.slot;
-            rec.last = sh.deal.cta_of(sh.u + at.units - 1);
-          }
+          t.split = split_of(sh, blockIdx.x, u_hi);
           sh.u += t.units;
           sh.off = 0;
         }
@@ -496,7 +483,6 @@ __global__ void __launch_bounds__(kTcThreads, 1)
         }
         if (sh.u < sh.u_end) next_tile(w, sh.at);
       }
-      if (lane == 0) a.split[blockIdx.x] = rec;
       // the queries' copies have landed before the CTA may end
       if (!SPLIT && a.q_map)
         for (int i = 0; i < 2; ++i)
@@ -658,23 +644,37 @@ __global__ void __launch_bounds__(kTcThreads, 1)
     const float c = SPLIT ? 1.f : fmaxf(fabsf(a.scale_log2), 1e-30f);   // the product takes the sign
     int n_o = 0, n_s = 0;   // tiles and units of this half so far
     bool ok = true;
-    TcTile t;
-    for (int nt = 0; ok && take_tile(nt, t); ++nt) {
-      if (half * 128 >= t.rows) continue;
-      const bool on = r < t.rows;
-      int p = -1;
-      int64_t e0 = 0;          // the row in q and out
-      {
-        const int rr = t.row0 + (on ? r : 0), tok = w.G.div(rr), G = (int)w.G.d;
-        if (on) p = t.first + tok;
-        e0 = ((int64_t)(t.q0 + tok) * a.n_head + t.h * G + (rr - tok * G)) * HD;
+    for (int nt = 0; ok; ++nt) {
+      // The tile stays in the ring until its results are out: what the units
+      // need is in registers, the rest is read where it is used.
+      ok = __all_sync(0xffffffffu, wait(&t_full[nt % kTcTiles], (nt / kTcTiles) & 1, 90));
+      if (!ok) break;
+      const TcTile& t = tiles[nt % kTcTiles];
+      auto leave_tile = [&]() {
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&t_empty[nt % kTcTiles]);
+      };
+      const int units = t.units, tile_key0 = t.key0, tile_hi = t.hi;
+      if (units == 0) break;
+      if (half * 128 >= t.rows) {
+        leave_tile();
+        continue;
       }
+      const bool on = r < t.rows;
+      // position, and place in q and out, of a row of the tile
+      auto token_of = [&](int row) { return w.G.div(t.row0 + row); };
+      auto place_of = [&](int row) {
+        const int tok = token_of(row), G = (int)w.G.d;
+        return ((int64_t)(t.q0 + tok) * a.n_head + t.h * G + (t.row0 + row - tok * G)) * HD;
+      };
+      const int p = on ? t.first + token_of(r) : -1;
       if constexpr (SPLIT) {
         // ---- the warp's 32 rows of Q, a row (hd 64: two) per step, as two parts ----
         constexpr int LR = HD / 4, RI = 32 / LR, B = 8;
         uint8_t* qd = Qs + half * 2 * L::half_q;
         const int ch = lane % LR;   // 4 values
         const float f = a.scale_log2;
+        const int64_t e0 = place_of(on ? r : 0);
 #pragma unroll 1
         for (int it = 0; it < 32 / RI; it += B) {
           float4 x[B];
@@ -701,8 +701,8 @@ __global__ void __launch_bounds__(kTcThreads, 1)
         mbar_arrive(&q_full[half]);
       }
       float m = -INFINITY, l = 0.f;
-      for (int u = 0; u < t.units; ++u) {
-        const int key0 = t.key0 + u * kTcBk;
+      for (int u = 0; u < units; ++u) {
+        const int key0 = tile_key0 + u * kTcBk;
         const bool edge = tc_edge(t, key0, w.window);
         ok = wait(&s_full[half], n_s++ & 1, 70);
         ok = __all_sync(0xffffffffu, ok);
@@ -711,7 +711,7 @@ __global__ void __launch_bounds__(kTcThreads, 1)
         float s[128];
         tmem_ld128(ts, s);
         // this row sees columns [lo, hi)
-        const int hi = min(p + 1, t.hi) - key0, lo = w.window > 0 ? p - w.window + 1 - key0 : 0;
+        const int hi = min(p + 1, tile_hi) - key0, lo = w.window > 0 ? p - w.window + 1 - key0 : 0;
         if (edge) {
 #pragma unroll
           for (int i = 0; i < 128; ++i)
@@ -790,12 +790,14 @@ __global__ void __launch_bounds__(kTcThreads, 1)
       ok = __all_sync(0xffffffffu, ok);
       if (!ok) break;
       tc_after();
-      const float inv = !t.whole ? 1.f : l != 0.f ? 1.f / l : 0.f;
-      float* part = a.slots + (int64_t)t.slot * slot_floats(kTcRows, HD);
+      const bool whole = t.split.n == 0;
+      const int64_t e0 = place_of(on ? r : 0);
+      const float inv = !whole ? 1.f : l != 0.f ? 1.f / l : 0.f;
+      float* part = a.slots + (int64_t)t.split.slot * slot_floats(kTcRows, HD);
       // Through shared memory, 32 columns at a time: 16-byte chunks of a row,
       // moved so that neither side meets a bank conflict, then segments of rows.
       uint8_t* stage = SPLIT ? Qs + half * 2 * L::half_q + (warp & 3) * 4096 : Ts + NS * L::tile + warp * 4096;
-      const bool wide = SPLIT || !t.whole;   // fp32 out
+      const bool wide = SPLIT || !whole;   // fp32 out
 #pragma unroll 1
       for (int i = 0; i < HD / 32; ++i) {
         float o[32];
@@ -823,7 +825,7 @@ __global__ void __launch_bounds__(kTcThreads, 1)
             const int rl = it * 4 + (lane >> 3), rt = half * 128 + (warp & 3) * 32 + rl;
             const float4 x = *reinterpret_cast<const float4*>(stage + rl * 128 + ((ch ^ (rl & 7)) << 4));
             const int64_t at_r = __shfl_sync(0xffffffffu, e0, rl);
-            float* dst = t.whole ? static_cast<float*>(a.out) + at_r : part + rt * HD;
+            float* dst = whole ? static_cast<float*>(a.out) + at_r : part + rt * HD;
             if (rt < t.rows) *reinterpret_cast<float4*>(dst + i * 32 + ch * 4) = x;
           }
         } else {
@@ -837,7 +839,7 @@ __global__ void __launch_bounds__(kTcThreads, 1)
           }
         }
       }
-      if (!t.whole && on) *reinterpret_cast<float2*>(part + kTcRows * HD + 2 * r) = make_float2(m, l);
+      if (!whole && on) *reinterpret_cast<float2*>(part + kTcRows * HD + 2 * r) = make_float2(m, l);
       if (*reinterpret_cast<volatile int*>(bad_seen) > nt) {
         // infinite and NaN values that were taken out of V, to the rows that
         // see them: their weight is positive, so the value decides the sum
@@ -855,7 +857,7 @@ __global__ void __launch_bounds__(kTcThreads, 1)
             for (int d = 0; d < HD; ++d) {
               const float f = __half2float(v[d]);
               if (fabsf(f) <= 65504.f) continue;
-              if (!t.whole)
+              if (!whole)
                 part[r * HD + d] += f;
               else if (SPLIT)
                 static_cast<float*>(a.out)[e0 + d] += f;
@@ -866,7 +868,18 @@ __global__ void __launch_bounds__(kTcThreads, 1)
           }
         }
       }
+      const int warp_row = (half * 4 + (warp & 3)) * 32;
+      if (!whole && warp_row < t.rows) {
+        if (part_arrives(a.counters + t.split.cta0 * 8 + half * 4 + (warp & 3), t.split.n)) {
+          constexpr int R = 16;
+#pragma unroll 1
+          for (int r0 = 0; r0 < 32 && warp_row + r0 < t.rows; r0 += R)
+            join_rows<HD, R>(a.slots, kTcRows, t.split, warp_row + r0, t.rows - warp_row - r0,
+                             __shfl_sync(0xffffffffu, e0, (lane + r0) & 31), a.out, SPLIT);
+        }
+      }
       tc_before();
+      leave_tile();
     }
   }
   tc_before();

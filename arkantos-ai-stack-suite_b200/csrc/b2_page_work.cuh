@@ -8,9 +8,10 @@
 // of one wave: a ragged batch, a single long sequence and a triangular prompt
 // all fill the machine, with no plan made on the host, so lengths may live on
 // the device and a call can be captured.  A tile whose units fall to several
-// CTAs is finished by a second kernel from their partial results (fp32
+// CTAs is finished by the last of them from all their partial results (fp32
 // weighted sums, maximum and sum of each row), always in unit order, so the
-// result does not depend on timing.
+// result does not depend on timing.  (A second kernel for that took 3 us of a
+// single token's 13, and 9 us behind a 512-token chunk.)
 #pragma once
 
 #include "b2_common.cuh"
@@ -215,24 +216,207 @@ __device__ __forceinline__ void next_tile(const PageWork& w, TileAt& a) {
   tile_load(w, a);
 }
 
-// What the finishing kernel needs about the tile that starts in a CTA's share
-// and runs past its end (at most one per CTA): its rows, the CTA that ends it
-// and the slot of its first partial result.  A CTA's other partial result,
-// the rest of a tile that began before it, is in slot 2·cta.
-struct SplitTile {
-  int32_t h, s, t, last, slot, rows, q0, pad;
+// How a tile that is split over CTAs is put together: its parts come from n
+// CTAs beginning with cta0, the first one's partial result in slot0, the
+// others' in slot 2·cta.  A CTA has two slots, one for the rest of a tile that
+// began before its share or with it, one for a tile that runs past its end.
+struct Split {
+  int cta0, n, slot0, slot;   // n = 0: the tile is not split
 };
+__device__ __forceinline__ Split split_of(const Share& sh, int cta, int u_hi) {
+  Split p = {0, 0, 0, 0};
+  if (sh.off == 0 && u_hi == sh.at.units) return p;
+  const int start = sh.u - sh.off;   // the tile's first unit among all
+  p.cta0 = sh.deal.cta_of(start);
+  p.n = sh.deal.cta_of(start + sh.at.units - 1) - p.cta0 + 1;
+  p.slot0 = 2 * p.cta0 + (sh.deal.start(p.cta0) == start ? 0 : 1);
+  p.slot = cta == p.cta0 ? p.slot0 : 2 * cta;
+  return p;
+}
 
-// Workspace: [ctas] SplitTile, then 2·ctas slots of rows · (hd + 2) floats
-// (the weighted sums of all rows, then (maximum, sum) of each).
-__host__ __device__ inline size_t split_bytes(int ctas) { return (size_t)ctas * sizeof(SplitTile); }
+// Workspace: counters of the parts that have arrived, 8 a CTA (by the CTA that
+// begins a tile; a warp of the tile each), zero between calls; then two slots
+// a CTA of rows · (hd + 2) floats (the weighted sums of all rows, then
+// (maximum, sum) of each).
+constexpr int kPageMaxCtasPerSm = 4;   // most CTAs an attention kernel is launched with
+__host__ __device__ inline size_t counter_bytes(int ctas) { return (size_t)ctas * 32; }
 __host__ __device__ inline size_t slot_floats(int rows, int hd) { return (size_t)rows * (hd + 2); }
 
-// Most CTAs an attention kernel is launched with (the workspace has room for them).
-constexpr int kPageMaxCtasPerSm = 4;
+__device__ __forceinline__ float ex2(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
 
-// Finishes the tiles that were split over CTAs (b2_page_attn.cu).
-int launch_page_join(const PageWork& w, const SplitTile* split, const float* slots, int ctas, int hd, int n_head,
-                     void* out, bool out_f32, cudaStream_t s);
+// Whether the calling warp's part is the last of its n: the parts' rows are
+// then visible to it.  All lanes have written theirs; the counter is left at
+// zero.
+__device__ __forceinline__ bool part_arrives(unsigned* counter, int n) {
+  __threadfence();
+  __syncwarp();
+  unsigned last = 0;
+  if ((threadIdx.x & 31) == 0) {
+    last = atomicAdd(counter, 1u) == (unsigned)(n - 1);
+    if (last) *counter = 0;
+    __threadfence();
+  }
+  return __shfl_sync(0xffffffffu, last, 0) != 0;
+}
+
+// HD/32 values of a row and lane, from a partial result and to the output.
+template <int V>
+__device__ __forceinline__ void load_part(const float* src, float (&x)[V]) {
+  if constexpr (V == 4) {
+    const float4 f = __ldcg(reinterpret_cast<const float4*>(src));
+    x[0] = f.x, x[1] = f.y, x[2] = f.z, x[3] = f.w;
+  } else if constexpr (V == 2) {
+    const float2 f = __ldcg(reinterpret_cast<const float2*>(src));
+    x[0] = f.x, x[1] = f.y;
+  } else {
+#pragma unroll
+    for (int v = 0; v < V; ++v) x[v] = __ldcg(src + v);
+  }
+}
+template <int V>
+__device__ __forceinline__ void store_joined(void* out, bool f32, int64_t at, const float (&x)[V], float inv) {
+  if (f32) {
+    float* d = static_cast<float*>(out) + at;
+    if constexpr (V == 4) {
+      *reinterpret_cast<float4*>(d) = make_float4(x[0] * inv, x[1] * inv, x[2] * inv, x[3] * inv);
+    } else {
+#pragma unroll
+      for (int v = 0; v < V; ++v) d[v] = x[v] * inv;
+    }
+  } else {
+    __half* d = static_cast<__half*>(out) + at;
+    if constexpr (V % 2 == 0) {
+#pragma unroll
+      for (int v = 0; v < V; v += 2) *reinterpret_cast<__half2*>(d + v) = __floats2half2_rn(x[v] * inv, x[v + 1] * inv);
+    } else {
+#pragma unroll
+      for (int v = 0; v < V; ++v) d[v] = __float2half_rn(x[v] * inv);
+    }
+  }
+}
+// A part's weight for a row with maximum m and sum l in it: a part that saw
+// nothing of the row adds nothing; a sum without a maximum comes from scores
+// that are all NaN.
+__device__ __forceinline__ float part_weight(float m, float l, float top) {
+  return l == 0.f ? 0.f : m == -INFINITY ? 1.f : ex2(m - top);
+}
+
+// Rows row .. row + min(R, n_rows) - 1 of a split tile from its parts, by one
+// warp: w_i = 2^(m_i − M), the weighted sums added in the CTAs' order and
+// divided by the joined sum.  e: where row `row` + lane starts in the output.
+//
+// Few rows of many parts (a single token's): the weights are formed a lane per
+// part, 32 parts at a time, and U parts' rows are loaded at once.
+template <int HD, int R, int U>
+__device__ __forceinline__ void join_parts(const float* slots, int tile_rows, const Split& p, int row, int n_rows,
+                                           int64_t e, void* out, bool f32) {
+  constexpr int V = HD / 32;
+  const int lane = threadIdx.x & 31;
+  const int64_t size = (int64_t)slot_floats(tile_rows, HD);
+  auto part = [&](int i) { return slots + (i == 0 ? p.slot0 : 2 * (p.cta0 + i)) * size; };
+  auto stat = [&](int i, int r) {   // (maximum, sum) of a row in a part
+    const int at = row + min(r, n_rows - 1);
+    return i < p.n ? __ldcg(reinterpret_cast<const float2*>(part(i) + tile_rows * HD + 2 * at)) : make_float2(-INFINITY, 0.f);
+  };
+  float top[R], sum[R], acc[R][V];
+#pragma unroll
+  for (int r = 0; r < R; ++r) {
+    top[r] = -INFINITY;
+    sum[r] = 0.f;
+#pragma unroll
+    for (int v = 0; v < V; ++v) acc[r][v] = 0.f;
+  }
+#pragma unroll 1
+  for (int i0 = 0; i0 < p.n; i0 += 32) {
+#pragma unroll
+    for (int r = 0; r < R; ++r) top[r] = fmaxf(top[r], stat(i0 + lane, r).x);
+  }
+#pragma unroll
+  for (int r = 0; r < R; ++r) top[r] = warp_max(top[r]);
+#pragma unroll 1
+  for (int i0 = 0; i0 < p.n; i0 += 32) {
+    float wt[R];
+#pragma unroll
+    for (int r = 0; r < R; ++r) {
+      const float2 ml = stat(i0 + lane, r);
+      wt[r] = part_weight(ml.x, ml.y, top[r]);
+      sum[r] += wt[r] * ml.y;
+    }
+    const int m = min(32, p.n - i0);
+#pragma unroll 1
+    for (int i1 = 0; i1 < m; i1 += U) {
+      float x[U][R][V];
+#pragma unroll
+      for (int u = 0; u < U; ++u)
+#pragma unroll
+        for (int r = 0; r < R; ++r)
+          load_part<V>(part(i0 + min(i1 + u, m - 1)) + (row + min(r, n_rows - 1)) * HD + lane * V, x[u][r]);
+#pragma unroll
+      for (int u = 0; u < U; ++u)
+#pragma unroll
+        for (int r = 0; r < R; ++r) {
+          const float wr = i1 + u < m ? __shfl_sync(0xffffffffu, wt[r], i1 + u) : 0.f;
+          if (wr != 0.f) {
+#pragma unroll
+            for (int v = 0; v < V; ++v) acc[r][v] += wr * x[u][r][v];
+          }
+        }
+    }
+  }
+#pragma unroll
+  for (int r = 0; r < R; ++r) {
+    sum[r] = warp_sum(sum[r]);
+    const int64_t at = __shfl_sync(0xffffffffu, e, r) + lane * V;
+    if (r < n_rows) store_joined<V>(out, f32, at, acc[r], sum[r] != 0.f ? 1.f / sum[r] : 0.f);
+  }
+}
+
+// Many rows of few parts: a lane holds one row's maximum, weight and sum, and
+// a part's R rows are loaded at once.
+template <int HD, int R>
+__device__ __forceinline__ void join_rows(const float* slots, int tile_rows, const Split& p, int row, int n_rows,
+                                          int64_t e, void* out, bool f32) {
+  constexpr int V = HD / 32;
+  const int lane = threadIdx.x & 31, own = row + min(lane, min(R, n_rows) - 1);
+  const int64_t size = (int64_t)slot_floats(tile_rows, HD);
+  auto part = [&](int i) { return slots + (i == 0 ? p.slot0 : 2 * (p.cta0 + i)) * size; };
+  float top = -INFINITY;
+#pragma unroll 4
+  for (int i = 0; i < p.n; ++i) top = fmaxf(top, __ldcg(part(i) + tile_rows * HD + 2 * own));
+  float sum = 0.f, acc[R][V];
+#pragma unroll
+  for (int r = 0; r < R; ++r)
+#pragma unroll
+    for (int v = 0; v < V; ++v) acc[r][v] = 0.f;
+#pragma unroll 1
+  for (int i = 0; i < p.n; ++i) {
+    const float* q = part(i);
+    const float2 ml = __ldcg(reinterpret_cast<const float2*>(q + tile_rows * HD + 2 * own));
+    float x[R][V];
+#pragma unroll
+    for (int r = 0; r < R; ++r) load_part<V>(q + (row + min(r, n_rows - 1)) * HD + lane * V, x[r]);
+    const float wt = part_weight(ml.x, ml.y, top);
+    sum += wt * ml.y;
+#pragma unroll
+    for (int r = 0; r < R; ++r) {
+      const float wr = __shfl_sync(0xffffffffu, wt, r);
+      if (wr != 0.f) {
+#pragma unroll
+        for (int v = 0; v < V; ++v) acc[r][v] += wr * x[r][v];
+      }
+    }
+  }
+  const float inv = sum != 0.f ? 1.f / sum : 0.f;
+#pragma unroll
+  for (int r = 0; r < R; ++r) {
+    const float ir = __shfl_sync(0xffffffffu, inv, r);
+    const int64_t at = __shfl_sync(0xffffffffu, e, r) + lane * V;
+    if (r < n_rows) store_joined<V>(out, f32, at, acc[r], ir);
+  }
+}
 
 }  // namespace b2

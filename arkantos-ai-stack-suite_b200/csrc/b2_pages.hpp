@@ -71,7 +71,10 @@ struct PageAttnArgs {
   uint8_t* ws = nullptr;
   int* status = nullptr;
 };
+// Bytes of the workspace, and of its counters, which come first and are zero
+// between calls.
 size_t page_attn_workspace(const PageAttnArgs& a);
+size_t page_attn_counters(const PageAttnArgs& a);
 int launch_page_attn(const PageAttnArgs& a, cudaStream_t s);
 
 // Whole pages src[i] -> dst[i] in every layer; bytes per page and layer of K and V.

@@ -415,9 +415,11 @@ B2_API int b2_rope_sections(const int32_t* sections, int32_t n_axes, int32_t n_p
  * included.  Results do not depend on timing: the same call gives the same
  * bits.  Unlike b2_attn_decode the sums are not in the reference's sequential
  * order.  |scale·q| and |v| up to 65504 (fp16's range).
- * workspace: device, 16-byte aligned, b2_page_attn_workspace_bytes for this
- * batch's n_tok, max_q and n_seq or larger ones; one call at a time may use
- * it.  NULL: the call allocates stream-ordered scratch.  status (device int,
+ * workspace: device, 16-byte aligned, of at least
+ * b2_page_attn_workspace_bytes for the call's shapes, set to zero (b2_memset)
+ * before its first use; every call leaves it fit for the next, of any shape
+ * that it is large enough for, and one call at a time may use it.  NULL: the
+ * call allocates stream-ordered scratch.  status (device int,
  * may be NULL) receives a nonzero code if a pipeline wait expired. */
 B2_API int b2_page_attn_workspace_bytes(const b2_page_cache* cache, const b2_page_batch* batch, int32_t n_head,
                                         int type_q, size_t* bytes);
