@@ -71,6 +71,7 @@ int launch_page_attn(const PageAttnArgs& a, cudaStream_t s) {
     t.status = a.status;
     return launch_page_tc(t, a.hd, p.split, 1 << a.c.ps_log2, s);
   }
+  B2_CHECK_ARG((((int64_t)a.c.n_pages * a.c.n_kv) << a.c.ps_log2) < ((int64_t)1 << 31), "page_attn: pool rows");
   PageRowsArgs r;
   r.c = a.c;
   r.w = work_of(a, p);

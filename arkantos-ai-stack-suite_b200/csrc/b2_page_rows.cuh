@@ -22,13 +22,17 @@
 // fp32.
 //
 // Layout.  A unit is 64 positions.  cp.async brings its K and V rows into a
-// ring of stages, 16 bytes a thread, row by row through the page table, so a
-// page may end anywhere; positions the tile does not attend to and table
-// entries outside the pool are filled with zeros.  Quantized rows land as stored and
-// are unpacked to fp16 codes by the CTA.  WM = 1: the 4 warps take 16
-// positions each of the one 16-row operand and their results are joined at
-// the end of a tile; WM = 4: each warp has its own 16-row operand and runs
-// over all 64 positions.
+// ring of stages, 16 bytes a thread, from row numbers that were looked up in
+// the page table two units earlier, so a page may end anywhere; positions the
+// tile does not attend to and table entries outside the pool are filled with
+// zeros.  The ring runs on over the tiles of a CTA's share.  WM = 1: the 4
+// warps take 16 positions each of the one 16-row operand and their results are
+// joined at the end of a tile; quantized rows go from their stored bytes
+// straight into the operands' registers: the order of the dims within a block
+// is free in q·k (q is loaded in the same order), and in P·V a byte permute
+// pairs two positions' codes, a lane then holding 8 consecutive dims of the
+// result.  WM = 4: each warp has its own 16-row operand and runs over all 64
+// positions; quantized rows are unpacked to fp16 codes once for all of them.
 #pragma once
 
 #include <atomic>
@@ -44,6 +48,7 @@ struct PageRowsArgs {
   void* out;
   int n_head, q_f32;
   float scale_log2;          // scale · log2(e)
+  FastDiv cpr_k, cpr_v;      // 16-byte chunks of a row
   unsigned* counters;
   float* slots;
 };
@@ -118,9 +123,50 @@ template <int HD, bool KQ, bool VQ>
 __host__ __device__ inline int rows_stage_bytes(int rb_k, int rb_v) {
   return (KQ ? RowsSmem<HD>::raw(rb_k) : RowsSmem<HD>::tile) + (VQ ? RowsSmem<HD>::raw(rb_v) : RowsSmem<HD>::tile);
 }
-template <int HD, bool KQ, bool VQ>
+template <int HD, bool KQ, bool VQ, int WM>
 __host__ __device__ inline int rows_conv_bytes() {
-  return (KQ ? RowsSmem<HD>::tile + RowsSmem<HD>::scales : 0) + (VQ ? RowsSmem<HD>::tile + RowsSmem<HD>::scales : 0);
+  return WM == 1 ? 0
+                 : (KQ ? RowsSmem<HD>::tile + RowsSmem<HD>::scales : 0) + (VQ ? RowsSmem<HD>::tile + RowsSmem<HD>::scales : 0);
+}
+constexpr int kRowTabs = 8;   // units whose row numbers are kept (more than any ring has stages)
+
+// Bytes 0-3 of w, 4-bit codes 0..15 (offset 8), as exact fp16 values - 8..7.
+__device__ __forceinline__ void n4x4_to_h2(uint32_t w, uint32_t& a, uint32_t& b) {
+  const uint32_t x = __byte_perm(w, 0x64646464u, 0x4140), y = __byte_perm(w, 0x64646464u, 0x4342);
+  const __half2 off = __halves2half2(__ushort_as_half(0x6408), __ushort_as_half(0x6408));   // 1032
+  const __half2 p = __hsub2(*reinterpret_cast<const __half2*>(&x), off);
+  const __half2 q = __hsub2(*reinterpret_cast<const __half2*>(&y), off);
+  a = *reinterpret_cast<const uint32_t*>(&p);
+  b = *reinterpret_cast<const uint32_t*>(&q);
+}
+// Bytes of two positions' words as (position, next position) pairs of fp16:
+// out[t] from byte t of each.  `off`: 1152 for signed codes (their top bits
+// flipped before), 1032 for 4-bit ones.
+__device__ __forceinline__ void pair_to_h2(uint32_t w0, uint32_t w1, uint32_t off, uint32_t (&out)[4]) {
+  const uint32_t lo = __byte_perm(w0, w1, 0x5140), hi = __byte_perm(w0, w1, 0x7362);
+  const uint32_t x[4] = {__byte_perm(lo, 0x64646464u, 0x4140), __byte_perm(lo, 0x64646464u, 0x4342),
+                         __byte_perm(hi, 0x64646464u, 0x4140), __byte_perm(hi, 0x64646464u, 0x4342)};
+#pragma unroll
+  for (int t = 0; t < 4; ++t) {
+    const __half2 v = __hsub2(*reinterpret_cast<const __half2*>(&x[t]), *reinterpret_cast<const __half2*>(&off));
+    out[t] = *reinterpret_cast<const uint32_t*>(&v);
+  }
+}
+// The NB block scales behind a row's codes.
+template <int NB>
+__device__ __forceinline__ void row_scales(const uint8_t* p, float (&d)[NB]) {
+  uint32_t w[(NB + 1) / 2];
+  if constexpr (NB == 8) {
+    const uint4 v = *reinterpret_cast<const uint4*>(p);
+    w[0] = v.x, w[1] = v.y, w[2] = v.z, w[3] = v.w;
+  } else if constexpr (NB > 2) {
+    const uint2 v = *reinterpret_cast<const uint2*>(p);
+    w[0] = v.x, w[1] = v.y;
+  } else {
+    w[0] = *reinterpret_cast<const uint32_t*>(p);
+  }
+#pragma unroll
+  for (int b = 0; b < NB; ++b) d[b] = h2f((uint16_t)(w[b / 2] >> (16 * (b & 1))));
 }
 
 template <int HD, bool KQ, bool VQ, bool SPLIT, int WM>
@@ -131,7 +177,9 @@ __global__ void __launch_bounds__(kRowsThreads) page_rows_kernel(const PageRowsA
   constexpr int NT = NC / 8, KS = HD / 16, NB = HD / 32, DT = HD / 8;
   constexpr int WROWS = SPLIT ? 8 : 16;        // rows of a warp's operand
   constexpr int PITCH = RowsSmem<HD>::pitch;
+  constexpr bool KD = KQ && WM == 1, VD = VQ && WM == 1;   // stored bytes straight into registers
   extern __shared__ __align__(128) uint8_t smem[];
+  __shared__ int row_tab[kRowTabs][kRowsBk];
   pdl_wait();
   pdl_launch_dependents();
 
@@ -140,6 +188,7 @@ __global__ void __launch_bounds__(kRowsThreads) page_rows_kernel(const PageRowsA
   const int g = lane >> 2, j = lane & 3;
   const PageView& c = a.c;
   const PageWork& w = a.w;
+  const int G = (int)w.G.d;
 
   Share sh;
   int* sums = reinterpret_cast<int*>(smem);
@@ -147,39 +196,132 @@ __global__ void __launch_bounds__(kRowsThreads) page_rows_kernel(const PageRowsA
   __syncthreads();
   const bool have = find_share(w, blockIdx.x, gridDim.x, sums, sh);   // every warp finds the same place
   if (!have) return;
-  __syncthreads();   // sums are read; the stages take their place
 
   const int stage_bytes = rows_stage_bytes<HD, KQ, VQ>(c.rb_k, c.rb_v);
   const int k_bytes = KQ ? RowsSmem<HD>::raw(c.rb_k) : RowsSmem<HD>::tile;
   uint8_t* ring = smem;
-  uint8_t* conv = smem + stages * stage_bytes;
-  uint8_t* conv_k = conv;
-  float* scale_k = reinterpret_cast<float*>(conv + RowsSmem<HD>::tile);
-  uint8_t* conv_v = conv + (KQ ? RowsSmem<HD>::tile + RowsSmem<HD>::scales : 0);
+  uint8_t* conv_k = smem + stages * stage_bytes;
+  float* scale_k = reinterpret_cast<float*>(conv_k + RowsSmem<HD>::tile);
+  uint8_t* conv_v = conv_k + (KQ ? RowsSmem<HD>::tile + RowsSmem<HD>::scales : 0);
   float* scale_v = reinterpret_cast<float*>(conv_v + RowsSmem<HD>::tile);
   const float off = p_offset(c.type_v);
 
+  // ---- staging: units are numbered through the share; a cursor runs ahead ----
+  const int n_units = sh.u_end - sh.u;
+  TileAt ahead = sh.at;
+  int ahead_off = sh.off, looked = 0;   // next unit of tile `ahead` to look up; units looked up so far
+  // the row number of this thread's position of the next unit (-1: zeros)
+  auto look_up = [&]() {
+    int row = -1;
+    if (looked < n_units && tid < kRowsBk) {
+      const int p = (ahead.lo_unit + ahead_off) * kRowsBk + tid;
+      if (p >= ahead.lo && p < ahead.hi) row = (int)page_row(w.b, c, ahead.s, ahead.h, p);
+    }
+    if (++looked < n_units && ++ahead_off == ahead.units) {
+      next_tile(w, ahead);
+      ahead_off = 0;
+    }
+    return row;
+  };
+  auto copy_in = [&](int u) {
+    const int* tab = row_tab[u % kRowTabs];
+    uint8_t* st = ring + (u % stages) * stage_bytes;
+    auto rows_in = [&](uint32_t dst, const uint8_t* pool, int rb, int pitch, const FastDiv& cpr) {
+      const int total = kRowsBk * (int)cpr.d;
+#pragma unroll 4
+      for (int i = tid; i < total; i += kRowsThreads) {
+        const int key = cpr.div(i), ch = i - key * (int)cpr.d, row = tab[key];
+        cp_async16(dst + key * pitch + ch * 16, pool + (row < 0 ? 0 : (int64_t)row * rb + ch * 16), row >= 0);
+      }
+    };
+    rows_in(smem_u32(st), c.k, c.rb_k, KQ ? c.rb_k : PITCH, a.cpr_k);
+    rows_in(smem_u32(st + k_bytes), c.v, c.rb_v, VQ ? c.rb_v : PITCH, a.cpr_v);
+  };
+  {
+    int row[4];   // of the first units (at most 4 stages)
+#pragma unroll
+    for (int n = 0; n < 4; ++n)
+      if (n < stages) row[n] = look_up();
+#pragma unroll
+    for (int n = 0; n < 4; ++n)
+      if (n < stages && tid < kRowsBk) row_tab[n][tid] = row[n];
+  }
+  __syncthreads();   // also: the sums are read, the stages take their place
+  for (int n = 0; n < stages - 1; ++n) {
+    if (n < n_units) copy_in(n);
+    cp_async_commit();
+  }
+  int next_row = look_up();   // of unit `stages`
+
+  // Quantized rows of a stage -> fp16 codes and fp32 scales [block][position] (WM = 4).
+  auto unpack = [&](const uint8_t* raw, int type, int rb, uint8_t* dst, float* sc, const FastDiv& cpr) {
+    const int cb = type == B2_Q8_0 ? HD : HD / 2;
+    const int cpk = (int)cpr.d - 1, total = kRowsBk * (int)cpr.d;   // a row: code chunks, then the scales'
+#pragma unroll 2
+    for (int i = tid; i < total; i += kRowsThreads) {
+      const int key = cpr.div(i), ch = i - key * (int)cpr.d;
+      const uint8_t* row = raw + key * rb;
+      if (ch == cpk) {
+        float d[NB];
+        row_scales<NB>(row + cb, d);
+#pragma unroll
+        for (int b = 0; b < NB; ++b) sc[b * kRowsBk + key] = d[b];
+        continue;
+      }
+      const uint4 x = *reinterpret_cast<const uint4*>(row + ch * 16);
+      uint32_t h[8];
+      if (type == B2_Q8_0) {
+        s8x4_to_h2(x.x, h[0], h[1]);
+        s8x4_to_h2(x.y, h[2], h[3]);
+        s8x4_to_h2(x.z, h[4], h[5]);
+        s8x4_to_h2(x.w, h[6], h[7]);
+        uint4* t = reinterpret_cast<uint4*>(dst + key * PITCH + ch * 32);
+        t[0] = make_uint4(h[0], h[1], h[2], h[3]);
+        t[1] = make_uint4(h[4], h[5], h[6], h[7]);
+      } else {
+        uint4* t = reinterpret_cast<uint4*>(dst + key * PITCH + ch * 64);
+        n4x4_to_h2(x.x & 0x0F0F0F0Fu, h[0], h[1]);
+        n4x4_to_h2(x.y & 0x0F0F0F0Fu, h[2], h[3]);
+        n4x4_to_h2(x.z & 0x0F0F0F0Fu, h[4], h[5]);
+        n4x4_to_h2(x.w & 0x0F0F0F0Fu, h[6], h[7]);
+        t[0] = make_uint4(h[0], h[1], h[2], h[3]);
+        t[1] = make_uint4(h[4], h[5], h[6], h[7]);
+        n4x4_to_h2((x.x >> 4) & 0x0F0F0F0Fu, h[0], h[1]);
+        n4x4_to_h2((x.y >> 4) & 0x0F0F0F0Fu, h[2], h[3]);
+        n4x4_to_h2((x.z >> 4) & 0x0F0F0F0Fu, h[4], h[5]);
+        n4x4_to_h2((x.w >> 4) & 0x0F0F0F0Fu, h[6], h[7]);
+        t[2] = make_uint4(h[0], h[1], h[2], h[3]);
+        t[3] = make_uint4(h[4], h[5], h[6], h[7]);
+      }
+    }
+  };
+
+  int done = 0;   // units of the share so far
   while (sh.u < sh.u_end) {
     const TileAt at = sh.at;
     const int u_lo = sh.off, u_hi = min(at.units, u_lo + (sh.u_end - sh.u));
-    const int row0 = at.t << w.rows_log2, G = (int)w.G.d;
+    const int row0 = at.t << w.rows_log2;
     const int rows = min(w.rows(), at.rows_total - row0);
+    // where row r of the tile stands in q and out
+    auto place = [&](int r) -> int64_t {
+      const int rr = row0 + r, tok = w.G.div(rr);
+      return ((int64_t)(at.q0 + tok) * a.n_head + at.h * G + rr - tok * G) * HD;
+    };
 
-    // ---- queries: registers, scaled in fp32 and split, or as they are ----
+    // ---- queries: registers, scaled in fp32 and split, or as they are; in
+    // the dims' order within a block of 32 that the K operand is loaded in ----
     uint32_t qf[KS][4];
     int p0 = -1, p1 = -1;   // positions of rows g and g + 8 (-1: sees nothing)
     {
       const int r = wm * WROWS + g, r1 = r + 8;
       const bool on0 = r < rows, on1 = !SPLIT && r1 < rows;
-      const int rr0 = row0 + (on0 ? r : 0), rr1 = row0 + (on1 ? r1 : 0);
-      const int tok0 = w.G.div(rr0), tok1 = w.G.div(rr1);
-      if (on0) p0 = at.first + tok0;
-      if (on1) p1 = at.first + tok1;
-      const int64_t e0 = ((int64_t)(at.q0 + tok0) * a.n_head + at.h * G + rr0 - tok0 * G) * HD;
-      const int64_t e1 = ((int64_t)(at.q0 + tok1) * a.n_head + at.h * G + rr1 - tok1 * G) * HD;
+      if (on0) p0 = at.first + w.G.div(row0 + r);
+      if (on1) p1 = at.first + w.G.div(row0 + r1);
+      const int64_t e0 = place(on0 ? r : 0), e1 = place(on1 ? r1 : 0);
 #pragma unroll
       for (int ks = 0; ks < KS; ++ks) {
-        const int d0 = ks * 16 + 2 * j, d1 = d0 + 8;
+        // dims of operand columns 2j, 2j + 1 and 2j + 8, 2j + 9
+        const int d0 = KD ? (ks / 2) * 32 + (ks & 1) * 16 + 4 * j : ks * 16 + 2 * j, d1 = KD ? d0 + 2 : d0 + 8;
         if constexpr (SPLIT) {
           float2 x = make_float2(0.f, 0.f), y = x;
           if (on0) {
@@ -210,102 +352,49 @@ __global__ void __launch_bounds__(kRowsThreads) page_rows_kernel(const PageRowsA
     for (int d = 0; d < DT; ++d)
 #pragma unroll
       for (int e = 0; e < 4; ++e) o[d][e] = 0.f;
+    // dim of o[d][e] and o[d][e + 2]
+    auto dim_of = [&](int d, int e) { return VD ? (d >> 2) * 32 + 8 * j + 4 * e + (d & 3) : d * 8 + 2 * j + e; };
     float m0 = -INFINITY, m1 = -INFINITY, l0 = 0.f, l1 = 0.f;   // rows g and g + 8 (SPLIT: row g)
-
-    // ---- staging ----
-    auto stage_in = [&](int u) {
-      const int key0 = (at.lo_unit + u) * kRowsBk;
-      uint8_t* st = ring + (u % stages) * stage_bytes;
-      const uint32_t sk = smem_u32(st), sv = smem_u32(st + k_bytes);
-      auto rows_in = [&](uint32_t dst, const uint8_t* pool, int rb, int pitch) {
-        const int cpr = rb >> 4;
-        for (int i = tid; i < kRowsBk * cpr; i += kRowsThreads) {
-          const int key = i / cpr, ch = i - key * cpr, p = key0 + key;
-          const int64_t row = p >= at.lo && p < at.hi ? page_row(w.b, c, at.s, at.h, p) : -1;
-          cp_async16(dst + key * pitch + ch * 16, pool + (row < 0 ? 0 : row * rb + ch * 16), row >= 0);
-        }
-      };
-      rows_in(sk, c.k, c.rb_k, KQ ? c.rb_k : PITCH);
-      rows_in(sv, c.v, c.rb_v, VQ ? c.rb_v : PITCH);
-    };
-    // Quantized rows of a stage -> fp16 codes and fp32 scales [block][position].
-    auto unpack = [&](const uint8_t* raw, int type, int rb, uint8_t* dst, float* sc) {
-      const int cb = type == B2_Q8_0 ? HD : HD / 2, cpr = cb / 16;
-      for (int i = tid; i < kRowsBk * cpr; i += kRowsThreads) {
-        const int key = i / cpr, ch = i - key * cpr;
-        const uint4 x = *reinterpret_cast<const uint4*>(raw + key * rb + ch * 16);
-        uint32_t h[8];
-        if (type == B2_Q8_0) {
-          s8x4_to_h2(x.x, h[0], h[1]);
-          s8x4_to_h2(x.y, h[2], h[3]);
-          s8x4_to_h2(x.z, h[4], h[5]);
-          s8x4_to_h2(x.w, h[6], h[7]);
-          uint4* t = reinterpret_cast<uint4*>(dst + key * PITCH + ch * 32);
-          t[0] = make_uint4(h[0], h[1], h[2], h[3]);
-          t[1] = make_uint4(h[4], h[5], h[6], h[7]);
-        } else {
-          uint4* t = reinterpret_cast<uint4*>(dst + key * PITCH + ch * 64);
-          const uint32_t lo[4] = {(uint32_t)nib_lo_s8(x.x), (uint32_t)nib_lo_s8(x.y), (uint32_t)nib_lo_s8(x.z),
-                                  (uint32_t)nib_lo_s8(x.w)};
-          const uint32_t hi[4] = {(uint32_t)nib_hi_s8(x.x), (uint32_t)nib_hi_s8(x.y), (uint32_t)nib_hi_s8(x.z),
-                                  (uint32_t)nib_hi_s8(x.w)};
-          s8x4_to_h2(lo[0], h[0], h[1]);
-          s8x4_to_h2(lo[1], h[2], h[3]);
-          s8x4_to_h2(lo[2], h[4], h[5]);
-          s8x4_to_h2(lo[3], h[6], h[7]);
-          t[0] = make_uint4(h[0], h[1], h[2], h[3]);
-          t[1] = make_uint4(h[4], h[5], h[6], h[7]);
-          s8x4_to_h2(hi[0], h[0], h[1]);
-          s8x4_to_h2(hi[1], h[2], h[3]);
-          s8x4_to_h2(hi[2], h[4], h[5]);
-          s8x4_to_h2(hi[3], h[6], h[7]);
-          t[2] = make_uint4(h[0], h[1], h[2], h[3]);
-          t[3] = make_uint4(h[4], h[5], h[6], h[7]);
-        }
-      }
-      for (int i = tid; i < kRowsBk * NB; i += kRowsThreads) {
-        const int b = i / kRowsBk, key = i - b * kRowsBk;
-        sc[i] = h2f(*reinterpret_cast<const uint16_t*>(raw + key * rb + cb + 2 * b));
-      }
-    };
-
-    for (int n = 0; n < stages - 1; ++n) {
-      if (u_lo + n < u_hi) stage_in(u_lo + n);
-      cp_async_commit();
-    }
     // positions every live row sees need no mask
     const int p_min = at.first + w.G.div(row0), p_max = at.first + w.G.div(row0 + rows - 1);
-    for (int u = u_lo; u < u_hi; ++u) {
+
+    for (int u = u_lo; u < u_hi; ++u, ++done) {
       // all but the newest stages - 2 groups have landed
       if (stages == 4) cp_async_wait<2>(); else if (stages == 3) cp_async_wait<1>(); else cp_async_wait<0>();
-      __syncthreads();   // unit u is here; everyone is done with unit u - 1, whose stage the next copy takes
-      if (u + stages - 1 < u_hi) stage_in(u + stages - 1);
+      __syncthreads();   // the unit is here; everyone is done with the one before, whose stage the next copy takes
+      if (done + stages - 1 < n_units) copy_in(done + stages - 1);
       cp_async_commit();
-      uint8_t* st = ring + (u % stages) * stage_bytes;
+      if (tid < kRowsBk) row_tab[(done + stages) % kRowTabs][tid] = next_row;
+      next_row = look_up();
+      uint8_t* st = ring + (done % stages) * stage_bytes;
       const int key0 = (at.lo_unit + u) * kRowsBk;
       const bool edge = key0 + kRowsBk > at.hi || key0 + kRowsBk - 1 > p_min ||
                         (w.window > 0 && key0 <= p_max - w.window);
-      if constexpr (KQ) unpack(st, c.type_k, c.rb_k, conv_k, scale_k);
-      if constexpr (VQ) unpack(st + k_bytes, c.type_v, c.rb_v, conv_v, scale_v);
-      uint8_t* Vt = VQ ? conv_v : st + k_bytes;
-      const uint32_t ks_base = smem_u32(KQ ? conv_k : st), vs_base = smem_u32(Vt);
+      // A value that some row must not see can still reach it as 0·v when v is
+      // infinite or NaN.  Such values are taken out of the operand and added
+      // at the end to the rows that do see them.
+      const bool guard = edge && p_max > p_min;
+      int found = 0;
       bool bad = false;
-      if (edge && p_max > p_min) {
-        // A value that some row must not see can still reach it as 0·v when v
-        // is infinite or NaN.  Such values are taken out of the operand here
-        // and added below to the rows that do see them.
-        if constexpr (VQ) __syncthreads();   // the scales are written
-        int found = 0;
+      if constexpr (KQ && !KD) unpack(st, c.type_k, c.rb_k, conv_k, scale_k, a.cpr_k);
+      if constexpr (VQ && !VD) unpack(st + k_bytes, c.type_v, c.rb_v, conv_v, scale_v, a.cpr_v);
+      uint8_t* Kt = KQ && !KD ? conv_k : st;
+      uint8_t* Vt = VQ && !VD ? conv_v : st + k_bytes;
+      const uint32_t ks_base = smem_u32(Kt), vs_base = smem_u32(Vt);
+      if (guard && !VD) {
         if constexpr (VQ) {
+          __syncthreads();   // the scales are written
           for (int i = tid; i < kRowsBk * NB; i += kRowsThreads)
             if (!(fabsf(scale_v[i]) <= 65504.f)) {
               scale_v[i] = 0.f;
               found = 1;
             }
         } else {
-          for (int i = tid; i < kRowsBk * (HD / 2); i += kRowsThreads) {
+          // WM = 1: a warp looks over its own positions
+          const int first = WM == 1 ? wk * KEYS : 0, n = WM == 1 ? KEYS : kRowsBk;
+          for (int i = WM == 1 ? lane : tid; i < n * (HD / 2); i += WM == 1 ? 32 : kRowsThreads) {
             const int key = i / (HD / 2), x = i - key * (HD / 2);
-            uint32_t* p = reinterpret_cast<uint32_t*>(Vt + key * PITCH) + x;
+            uint32_t* p = reinterpret_cast<uint32_t*>(Vt + (first + key) * PITCH) + x;
             uint32_t v = *p;
             if ((v & 0x7C00u) == 0x7C00u) v &= 0xFFFF0000u;
             if ((v & 0x7C000000u) == 0x7C000000u) v &= 0xFFFFu;
@@ -315,8 +404,13 @@ __global__ void __launch_bounds__(kRowsThreads) page_rows_kernel(const PageRowsA
             }
           }
         }
-        bad = __syncthreads_or(found);
-      } else if constexpr (KQ || VQ) {
+        if constexpr (WM == 1) {
+          __syncwarp();
+          bad = __any_sync(0xffffffffu, found);
+        } else {
+          bad = __syncthreads_or(found);
+        }
+      } else if constexpr (WM != 1 && (KQ || VQ)) {
         __syncthreads();
       }
 
@@ -327,15 +421,37 @@ __global__ void __launch_bounds__(kRowsThreads) page_rows_kernel(const PageRowsA
 #pragma unroll
         for (int n = 0; n < NT; ++n) {
           float acc[4] = {0.f, 0.f, 0.f, 0.f};
+          const uint8_t* kr = Kt + (kw + n * 8 + g) * c.rb_k;   // KD: the row of operand column g
+          float da[NB], db[NB];                                 // KD: scales of positions 2j, 2j + 1
+          if constexpr (KD) {
+            const uint8_t* sr = Kt + (kw + n * 8 + 2 * j) * c.rb_k + (c.type_k == B2_Q8_0 ? HD : HD / 2);
+            row_scales<NB>(sr, da);
+            row_scales<NB>(sr + c.rb_k, db);
+          }
 #pragma unroll
           for (int b = 0; b < NB; ++b) {
             uint32_t kf[4];   // 8 positions x 32 dims
-            ldsm4(ks_base + (kw + n * 8 + (lane & 7)) * PITCH + b * 64 + (lane >> 3) * 16, kf);
+            if constexpr (KD) {
+              if (c.type_k == B2_Q8_0) {
+                s8x4_to_h2(*reinterpret_cast<const uint32_t*>(kr + b * 32 + 4 * j), kf[0], kf[1]);
+                s8x4_to_h2(*reinterpret_cast<const uint32_t*>(kr + b * 32 + 16 + 4 * j), kf[2], kf[3]);
+              } else {
+                const uint32_t x = *reinterpret_cast<const uint32_t*>(kr + b * 16 + 4 * j);
+                n4x4_to_h2(x & 0x0F0F0F0Fu, kf[0], kf[1]);
+                n4x4_to_h2((x >> 4) & 0x0F0F0F0Fu, kf[2], kf[3]);
+              }
+            } else {
+              ldsm4(ks_base + (kw + n * 8 + (lane & 7)) * PITCH + b * 64 + (lane >> 3) * 16, kf);
+            }
             if constexpr (KQ) {
               float t[4] = {0.f, 0.f, 0.f, 0.f};
               mma16816(t, qf[2 * b], kf[0], kf[1]);
               mma16816(t, qf[2 * b + 1], kf[2], kf[3]);
-              const float2 d = *reinterpret_cast<const float2*>(scale_k + b * kRowsBk + kw + n * 8 + 2 * j);
+              float2 d;
+              if constexpr (KD)
+                d = make_float2(da[b], db[b]);
+              else
+                d = *reinterpret_cast<const float2*>(scale_k + b * kRowsBk + kw + n * 8 + 2 * j);
               acc[0] = fmaf(t[0], d.x, acc[0]);
               acc[1] = fmaf(t[1], d.y, acc[1]);
               acc[2] = fmaf(t[2], d.x, acc[2]);
@@ -419,23 +535,64 @@ __global__ void __launch_bounds__(kRowsThreads) page_rows_kernel(const PageRowsA
             }
           };
           if constexpr (!VQ) operand(1.f, 1.f, 1.f, 1.f);
+          const uint8_t* vr = Vt + (kw + k * 16 + 2 * j) * c.rb_v;   // VD: the row of position 2j
+          float sc[4][NB];                                           // VD: scales of positions 2j, 2j+1, 2j+8, 2j+9
+          if constexpr (VD) {
+            const uint8_t* sr = vr + (c.type_v == B2_Q8_0 ? HD : HD / 2);
+            row_scales<NB>(sr, sc[0]);
+            row_scales<NB>(sr + c.rb_v, sc[1]);
+            row_scales<NB>(sr + 8 * c.rb_v, sc[2]);
+            row_scales<NB>(sr + 9 * c.rb_v, sc[3]);
+            if (guard) {
+#pragma unroll
+              for (int r = 0; r < 4; ++r)
+#pragma unroll
+                for (int b = 0; b < NB; ++b)
+                  if (!(fabsf(sc[r][b]) <= 65504.f)) {
+                    sc[r][b] = 0.f;
+                    found = 1;
+                  }
+            }
+          }
 #pragma unroll
           for (int b = 0; b < NB; ++b) {
-            if constexpr (VQ) {
-              const float* sc = scale_v + b * kRowsBk + kw + k * 16 + 2 * j;
-              const float2 da = *reinterpret_cast<const float2*>(sc), db = *reinterpret_cast<const float2*>(sc + 8);
-              operand(da.x, da.y, db.x, db.y);
-            }
+            if constexpr (VD) {
+              operand(sc[0][b], sc[1][b], sc[2][b], sc[3][b]);
+              uint32_t v0[4], v1[4];   // positions 2j, 2j+1 and 2j+8, 2j+9 of dims 4g + t of the block
+              if (c.type_v == B2_Q8_0) {
+                const uint8_t* q = vr + b * 32 + 4 * g;
+                pair_to_h2(*reinterpret_cast<const uint32_t*>(q) ^ 0x80808080u,
+                           *reinterpret_cast<const uint32_t*>(q + c.rb_v) ^ 0x80808080u, 0x64806480u, v0);
+                pair_to_h2(*reinterpret_cast<const uint32_t*>(q + 8 * c.rb_v) ^ 0x80808080u,
+                           *reinterpret_cast<const uint32_t*>(q + 9 * c.rb_v) ^ 0x80808080u, 0x64806480u, v1);
+              } else {
+                const uint8_t* q = vr + b * 16 + 4 * (g & 3);
+                const int sf = g & 4;   // values 16..31 are the high nibbles
+                pair_to_h2((*reinterpret_cast<const uint32_t*>(q) >> sf) & 0x0F0F0F0Fu,
+                           (*reinterpret_cast<const uint32_t*>(q + c.rb_v) >> sf) & 0x0F0F0F0Fu, 0x64086408u, v0);
+                pair_to_h2((*reinterpret_cast<const uint32_t*>(q + 8 * c.rb_v) >> sf) & 0x0F0F0F0Fu,
+                           (*reinterpret_cast<const uint32_t*>(q + 9 * c.rb_v) >> sf) & 0x0F0F0F0Fu, 0x64086408u, v1);
+              }
 #pragma unroll
-            for (int d = 0; d < 2; ++d) {
-              uint32_t vf[4];   // 16 positions x 16 dims
-              ldsm4_t(vs_base + (kw + k * 16 + (lane & 15)) * PITCH + (b * 32 + d * 16 + (lane >> 4) * 8) * 2, vf);
-              mma16816(o[b * 4 + 2 * d], pf, vf[0], vf[1]);
-              mma16816(o[b * 4 + 2 * d + 1], pf, vf[2], vf[3]);
+              for (int t = 0; t < 4; ++t) mma16816(o[b * 4 + t], pf, v0[t], v1[t]);
+            } else {
+              if constexpr (VQ) {
+                const float* q = scale_v + b * kRowsBk + kw + k * 16 + 2 * j;
+                const float2 da = *reinterpret_cast<const float2*>(q), db = *reinterpret_cast<const float2*>(q + 8);
+                operand(da.x, da.y, db.x, db.y);
+              }
+#pragma unroll
+              for (int d = 0; d < 2; ++d) {
+                uint32_t vf[4];   // 16 positions x 16 dims
+                ldsm4_t(vs_base + (kw + k * 16 + (lane & 15)) * PITCH + (b * 32 + d * 16 + (lane >> 4) * 8) * 2, vf);
+                mma16816(o[b * 4 + 2 * d], pf, vf[0], vf[1]);
+                mma16816(o[b * 4 + 2 * d + 1], pf, vf[2], vf[3]);
+              }
             }
           }
         }
       }
+      if (VD && guard) bad = __any_sync(0xffffffffu, found);
       if (bad) {
         // infinite and NaN values of V, to the rows that see them (their
         // weight is positive, so the value itself decides the sum)
@@ -451,7 +608,7 @@ __global__ void __launch_bounds__(kRowsThreads) page_rows_kernel(const PageRowsA
           for (int d = 0; d < DT; ++d)
 #pragma unroll
             for (int e = 0; e < 2; ++e) {
-              const int i = d * 8 + 2 * j + e;
+              const int i = dim_of(d, e);
               float v;
               if constexpr (VQ) {
                 const float sc = h2f(*reinterpret_cast<const uint16_t*>(
@@ -470,7 +627,6 @@ __global__ void __launch_bounds__(kRowsThreads) page_rows_kernel(const PageRowsA
         }
       }
     }
-    cp_async_wait<0>();
 
     // ---- join the lanes' sums, and for WM = 1 the warps ----
 #pragma unroll
@@ -489,26 +645,21 @@ __global__ void __launch_bounds__(kRowsThreads) page_rows_kernel(const PageRowsA
     const bool whole = split.n == 0;
     float* part = a.slots + (int64_t)split.slot * slot_floats(w.rows(), HD);
     float* part_ml = part + w.rows() * HD;
-
-    auto out_ptr = [&](int r) -> int64_t {
-      const int rr = row0 + r, tok = w.G.div(rr);
-      return ((int64_t)(at.q0 + tok) * a.n_head + at.h * G + rr - tok * G) * HD;
-    };
     auto put2 = [&](int r, int d, float x, float y) {   // values d, d + 1 of row r, normalized, or a partial result
       if (!whole) {
         *reinterpret_cast<float2*>(part + r * HD + d) = make_float2(x, y);
       } else if (a.q_f32) {
-        *reinterpret_cast<float2*>(static_cast<float*>(a.out) + out_ptr(r) + d) = make_float2(x, y);
+        *reinterpret_cast<float2*>(static_cast<float*>(a.out) + place(r) + d) = make_float2(x, y);
       } else {
-        *reinterpret_cast<uint32_t*>(static_cast<__half*>(a.out) + out_ptr(r) + d) = h2(x, y);
+        *reinterpret_cast<uint32_t*>(static_cast<__half*>(a.out) + place(r) + d) = h2(x, y);
       }
     };
 
     if constexpr (WM == 1) {
-      // [4 warps][16] (m, l), then [4 warps][WROWS][HD] sums, over the stages
-      __syncthreads();
-      float2* ml = reinterpret_cast<float2*>(smem);
-      float* so = reinterpret_cast<float*>(smem + 4 * 16 * 8);
+      // [4 warps][16] (m, l), then [4 warps][WROWS][HD] sums, after the ring
+      float2* ml = reinterpret_cast<float2*>(smem + stages * stage_bytes);
+      float* so = reinterpret_cast<float*>(ml + 64);
+      int* last_part = reinterpret_cast<int*>(so + 4 * WROWS * HD);
       if (j == 0) {
         ml[warp * 16 + g] = make_float2(m0, l0);
         if constexpr (!SPLIT) ml[warp * 16 + g + 8] = make_float2(m1, l1);
@@ -522,14 +673,13 @@ __global__ void __launch_bounds__(kRowsThreads) page_rows_kernel(const PageRowsA
       if constexpr (!SPLIT) f1 = m1 == -INFINITY ? 0.f : ex2(m1 - top(g + 8));
       // a warp that saw nothing of a row contributes nothing, not 0·NaN
 #pragma unroll
-      for (int d = 0; d < DT; ++d) {
-        const int i = d * 8 + 2 * j;
-        *reinterpret_cast<float2*>(so + (warp * WROWS + g) * HD + i) =
-            l0 != 0.f ? make_float2(o[d][0] * f0, o[d][1] * f0) : make_float2(0.f, 0.f);
-        if constexpr (!SPLIT)
-          *reinterpret_cast<float2*>(so + (warp * WROWS + g + 8) * HD + i) =
-              l1 != 0.f ? make_float2(o[d][2] * f1, o[d][3] * f1) : make_float2(0.f, 0.f);
-      }
+      for (int d = 0; d < DT; ++d)
+#pragma unroll
+        for (int e = 0; e < 2; ++e) {
+          const int i = dim_of(d, e);
+          so[(warp * WROWS + g) * HD + i] = l0 != 0.f ? o[d][e] * f0 : 0.f;
+          if constexpr (!SPLIT) so[(warp * WROWS + g + 8) * HD + i] = l1 != 0.f ? o[d][2 + e] * f1 : 0.f;
+        }
       __syncthreads();
       for (int i = tid; i < rows * (HD / 2); i += kRowsThreads) {
         const int r = i / (HD / 2), d = 2 * (i - r * (HD / 2));
@@ -558,18 +708,18 @@ __global__ void __launch_bounds__(kRowsThreads) page_rows_kernel(const PageRowsA
         __syncthreads();
         if (warp == 0) {
           const bool last = part_arrives(a.counters + split.cta0 * 8, split.n);
-          if (lane == 0) *reinterpret_cast<int*>(smem) = last;
+          if (lane == 0) *last_part = last;
         }
         __syncthreads();
-        if (*reinterpret_cast<volatile int*>(smem)) {
+        if (*reinterpret_cast<volatile int*>(last_part)) {
           constexpr int R = WROWS / 4;
           const int r = warp * R;
           if (r < rows)
-            join_parts<HD, R, 16 / R>(a.slots, w.rows(), split, r, rows - r, out_ptr(min(r + lane, rows - 1)), a.out,
-                             a.q_f32 != 0);
+            join_parts<HD, R, 16 / R>(a.slots, w.rows(), split, r, rows - r, place(min(r + lane, rows - 1)), a.out,
+                                      a.q_f32 != 0);
         }
       }
-      __syncthreads();   // the stages are free for the next tile
+      __syncthreads();   // the join's space is free for the next tile
     } else {
       const float i0 = !whole ? 1.f : l0 != 0.f ? 1.f / l0 : 0.f, i1 = !whole ? 1.f : l1 != 0.f ? 1.f / l1 : 0.f;
       const int r = wm * WROWS + g;
@@ -589,17 +739,17 @@ __global__ void __launch_bounds__(kRowsThreads) page_rows_kernel(const PageRowsA
         if (part_arrives(a.counters + split.cta0 * 8 + warp, split.n)) {
           constexpr int R = HD == 256 ? 4 : 8;
           for (int r0 = wm * WROWS; r0 < min((wm + 1) * WROWS, rows); r0 += R)
-            join_rows<HD, R>(a.slots, w.rows(), split, r0, rows - r0, out_ptr(min(r0 + lane, rows - 1)), a.out,
+            join_rows<HD, R>(a.slots, w.rows(), split, r0, rows - r0, place(min(r0 + lane, rows - 1)), a.out,
                              a.q_f32 != 0);
         }
       }
-      __syncthreads();
     }
 
     sh.u += u_hi - u_lo;
     sh.off = 0;
     if (sh.u < sh.u_end) next_tile(w, sh.at);
   }
+  cp_async_wait<0>();
 }
 
 int launch_page_rows_64(const PageRowsArgs& a, bool split, int wm, cudaStream_t s);
@@ -607,19 +757,21 @@ int launch_page_rows_96(const PageRowsArgs& a, bool split, int wm, cudaStream_t 
 int launch_page_rows_128(const PageRowsArgs& a, bool split, int wm, cudaStream_t s);
 int launch_page_rows_256(const PageRowsArgs& a, bool split, int wm, cudaStream_t s);
 
-// Stages of the ring and the CTAs that fit on an SM with them.
-template <int HD, bool KQ, bool VQ>
+// The ring, then what the tile's end needs beside it (WM = 1: the next tile's
+// units are already on their way).
+template <int HD, bool KQ, bool VQ, bool SPLIT, int WM>
 inline int rows_smem_bytes(const PageRowsArgs& a, int stages) {
-  const int ring = stages * rows_stage_bytes<HD, KQ, VQ>(a.c.rb_k, a.c.rb_v) + rows_conv_bytes<HD, KQ, VQ>();
-  const int join = 4 * 16 * 8 + 4 * 16 * HD * 4, sums = kPageMaxSeq * 4;
-  return std::max(ring, std::max(join, sums));
+  const int ring = stages * rows_stage_bytes<HD, KQ, VQ>(a.c.rb_k, a.c.rb_v) + rows_conv_bytes<HD, KQ, VQ, WM>();
+  const int join = WM == 1 ? 64 * 8 + 4 * (SPLIT ? 8 : 16) * HD * 4 + 16 : 0, sums = kPageMaxSeq * 4;
+  return std::max(ring + join, sums);
 }
 
 template <int HD, bool KQ, bool VQ, bool SPLIT, int WM>
-int launch_page_rows_one(const PageRowsArgs& a, cudaStream_t s) {
-  // As deep a ring as leaves two CTAs on an SM (one at head_dim 256 with fp16 rows).
-  const int stages = HD == 256 && !(KQ && VQ) ? 2 : 3;
-  const int smem = rows_smem_bytes<HD, KQ, VQ>(a, stages);
+int launch_page_rows_one(PageRowsArgs a, cudaStream_t s) {
+  // A ring that leaves two CTAs or more on an SM where it can (head_dim 256
+  // with fp16 rows: one).
+  const int stages = HD == 256 && !(KQ && VQ) ? 2 : WM == 1 && KQ && VQ ? 4 : 3;
+  const int smem = rows_smem_bytes<HD, KQ, VQ, SPLIT, WM>(a, stages);
   auto kern = page_rows_kernel<HD, KQ, VQ, SPLIT, WM>;
   // looked up once per device and cache type pair
   static std::atomic<int> resident[kMaxDevices][2][2];
@@ -629,11 +781,13 @@ int launch_page_rows_one(const PageRowsArgs& a, cudaStream_t s) {
   std::atomic<int>& known = resident[dev][a.c.type_k == B2_Q4_0][a.c.type_v == B2_Q4_0];
   int per_sm = known.load(std::memory_order_relaxed);
   if (per_sm == 0) {
-    B2_CUDA_TRY(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, 227 * 1024));
+    B2_CUDA_TRY(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, 225 * 1024));
     B2_CUDA_TRY(cudaOccupancyMaxActiveBlocksPerMultiprocessor(&per_sm, kern, kRowsThreads, smem));
     per_sm = std::max(1, std::min(per_sm, kPageMaxCtasPerSm));
     known.store(per_sm, std::memory_order_relaxed);
   }
+  a.cpr_k = FastDiv::of(a.c.rb_k / 16);
+  a.cpr_v = FastDiv::of(a.c.rb_v / 16);
   const int ctas = per_sm * sm_count();
   return launch_pdl(kern, dim3(ctas), dim3(kRowsThreads), (size_t)smem, s, a, stages);
 }
