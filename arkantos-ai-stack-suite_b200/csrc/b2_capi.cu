@@ -571,8 +571,8 @@ namespace {
 int page_check(const b2_page_cache* c, bool pools = true) {
   B2_CHECK_ARG(c && (!pools || (c->k && c->v)), "page cache pools");
   B2_CHECK_ARG(c->n_layer > 0 && c->n_pages > 0 && c->n_kv > 0, "page cache sizes");
-  B2_CHECK_ARG(c->page_size >= 1 && c->page_size <= 256 && (c->page_size & (c->page_size - 1)) == 0,
-               "page_size must be a power of two up to 256");
+  B2_CHECK_ARG(c->page_size >= 8 && c->page_size <= 256 && (c->page_size & (c->page_size - 1)) == 0,
+               "page_size must be a power of two from 8 to 256");
   B2_CHECK_ARG(c->head_dim > 0 && c->head_dim % 32 == 0 && c->head_dim <= 256,
                "head_dim must be a multiple of 32 up to 256");
   B2_CHECK_ARG(kv_type_ok(c->type_k) && kv_type_ok(c->type_v), "KV cache types must be B2_F16, B2_Q8_0 or B2_Q4_0");

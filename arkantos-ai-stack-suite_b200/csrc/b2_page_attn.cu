@@ -55,6 +55,8 @@ int launch_page_attn(const PageAttnArgs& a, cudaStream_t s) {
   const int64_t tiles = ((int64_t)a.b.n_tok * (a.n_head / a.c.n_kv)) / p.rows + a.b.n_seq;
   B2_CHECK_ARG(a.c.n_kv * tiles * ((((int64_t)a.b.max_pages << a.c.ps_log2) / p.bk) + 2) < ((int64_t)1 << 31),
                "page_attn: too many tokens for such a long table");
+  const int64_t pool_rows = ((int64_t)a.c.n_pages * a.c.n_kv) << a.c.ps_log2;
+  B2_CHECK_ARG(pool_rows < ((int64_t)1 << 31), "page_attn: rows of a layer's pool below 2^31");
   const float scale_log2 = (float)((double)a.scale * 1.4426950408889634);
   unsigned* counters = reinterpret_cast<unsigned*>(a.ws);
   float* slots = reinterpret_cast<float*>(a.ws + page_attn_counters(a));
@@ -69,9 +71,9 @@ int launch_page_attn(const PageAttnArgs& a, cudaStream_t s) {
     t.counters = counters;
     t.slots = slots;
     t.status = a.status;
+    t.pool_rows = pool_rows;
     return launch_page_tc(t, a.hd, p.split, 1 << a.c.ps_log2, s);
   }
-  B2_CHECK_ARG((((int64_t)a.c.n_pages * a.c.n_kv) << a.c.ps_log2) < ((int64_t)1 << 31), "page_attn: pool rows");
   PageRowsArgs r;
   r.c = a.c;
   r.w = work_of(a, p);
@@ -81,6 +83,8 @@ int launch_page_attn(const PageAttnArgs& a, cudaStream_t s) {
   r.q_f32 = a.type_q == B2_F32;
   r.scale_log2 = scale_log2;
   r.counters = counters;
+  r.pool_rows = pool_rows;
+  r.status = a.status;
   r.slots = slots;
   switch (a.hd) {
     case 64: return launch_page_rows_64(r, p.split, p.wm, s);

@@ -21,21 +21,28 @@
 // error the fp16 output has by itself.  Accumulators, maxima and sums are
 // fp32.
 //
-// Layout.  A unit is 64 positions.  cp.async brings its K and V rows into a
-// ring of stages, 16 bytes a thread, from row numbers that were looked up in
-// the page table two units earlier, so a page may end anywhere; positions the
-// tile does not attend to and table entries outside the pool are filled with
-// zeros.  The ring runs on over the tiles of a CTA's share.  WM = 1: the 4
-// warps take 16 positions each of the one 16-row operand and their results are
-// joined at the end of a tile; quantized rows go from their stored bytes
-// straight into the operands' registers: the order of the dims within a block
-// is free in q·k (q is loaded in the same order), and in P·V a byte permute
-// pairs two positions' codes, a lane then holding 8 consecutive dims of the
-// result.  WM = 4: each warp has its own 16-row operand and runs over all 64
-// positions; quantized rows are unpacked to fp16 codes once for all of them.
+// Layout.  A unit is 64 positions.  One warp brings K and V through a ring of
+// stages that runs on over the tiles of a CTA's share, looking pages up a unit
+// ahead: fp16 rows by tensor copies of a page and 64 dims, 128-byte swizzled
+// for ldmatrix; quantized rows, whose 16 bytes of scales already put them on
+// different banks, by plain bulk copies of a page's run.  (Copies of 16 bytes
+// a thread took 150 cycles each to issue, more than the products.)  Table
+// entries outside the pool read as zeros; rows past the tile's positions are
+// left as they come: K's scores there are masked, V is zeroed before use.
+// The other 4 warps compute.  WM = 1: they take 16 positions each of the one
+// 16-row operand and their results are joined at the end of a tile; quantized
+// rows go from their stored bytes straight into the operands' registers: the
+// order of the dims within a block is free in q·k (q is loaded in the same
+// order), and in P·V a byte permute pairs two positions' codes, a lane then
+// holding 8 consecutive dims of the result.  WM = 4: each warp has its own
+// 16-row operand and runs over all 64 positions; quantized rows are unpacked
+// to fp16 codes once for all of them.
 #pragma once
 
 #include <atomic>
+
+#include <cuda.h>
+#include <cudaTypedefs.h>
 
 #include "b2_page_work.cuh"
 
@@ -49,21 +56,18 @@ struct PageRowsArgs {
   int n_head, q_f32;
   float scale_log2;          // scale · log2(e)
   FastDiv cpr_k, cpr_v;      // 16-byte chunks of a row
+  int64_t pool_rows;
+  int* status;
   unsigned* counters;
   float* slots;
 };
 
-constexpr int kRowsThreads = 128, kRowsBk = 64, kMaxDevices = 64;
+constexpr int kRowsThreads = 128, kRowsBk = 64, kMaxDevices = 64;   // computing threads, positions of a unit
 
 __device__ __forceinline__ void cp_async16(uint32_t dst, const void* src, bool on) {
   asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(on ? 16 : 0) : "memory");
 }
-__device__ __forceinline__ void cp_async_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
 __device__ __forceinline__ void cp_async_wait_all() { asm volatile("cp.async.wait_all;" ::: "memory"); }
-template <int N>
-__device__ __forceinline__ void cp_async_wait() {
-  asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory");
-}
 __device__ __forceinline__ void ldsm4(uint32_t a, uint32_t (&r)[4]) {
   asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0,%1,%2,%3}, [%4];"
                : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3])
@@ -112,12 +116,18 @@ __device__ __forceinline__ void s8x4_to_h2(uint32_t w, uint32_t& a, uint32_t& b)
 // leaves room for 2^6 and 2^3.
 __host__ __device__ inline float p_offset(int type_v) { return type_v == B2_F16 ? 10.f : type_v == B2_Q8_0 ? 6.f : 3.f; }
 
+// An fp16 (or unpacked) operand: [dims / 64][64 rows][128 bytes], 16-byte
+// chunk c of row r at c ^ (r % 8).
 template <int HD>
 struct RowsSmem {
-  static constexpr int pitch = HD * 2 + 16;                  // ldmatrix rows 16 bytes apart modulo 128
-  static constexpr int tile = kRowsBk * pitch;               // an fp16 (or unpacked) operand
+  static constexpr int blocks = (HD + 63) / 64;
+  static constexpr int tile = blocks * kRowsBk * 128;
   static constexpr int scales = (HD / 32) * kRowsBk * 4;
   __host__ __device__ static int raw(int rb) { return kRowsBk * rb; }
+  // chunk of 8 values of a row
+  __device__ static __forceinline__ uint32_t at(int row, int chunk) {
+    return (uint32_t)((chunk >> 3) * (kRowsBk * 128) + row * 128 + (((chunk & 7) ^ (row & 7)) << 4));
+  }
 };
 template <int HD, bool KQ, bool VQ>
 __host__ __device__ inline int rows_stage_bytes(int rb_k, int rb_v) {
@@ -128,7 +138,30 @@ __host__ __device__ inline int rows_conv_bytes() {
   return WM == 1 ? 0
                  : (KQ ? RowsSmem<HD>::tile + RowsSmem<HD>::scales : 0) + (VQ ? RowsSmem<HD>::tile + RowsSmem<HD>::scales : 0);
 }
-constexpr int kRowTabs = 8;   // units whose row numbers are kept (more than any ring has stages)
+constexpr int kRowsStagesMax = 8, kRowsCtrl = 1024;
+constexpr int kWaitPolls = 1 << 22;   // polls of a wait, each suspended by the hardware for a while
+
+__device__ __forceinline__ void tma_2d(uint32_t dst, const CUtensorMap* map, int x, int y, uint64_t* bar) {
+  asm volatile(
+      "cp.async.bulk.tensor.2d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4}], [%2];" ::"r"(
+          dst),
+      "l"(reinterpret_cast<uint64_t>(map)), "r"(smem_u32(bar)), "r"(x), "r"(y)
+      : "memory");
+}
+__device__ __forceinline__ void fence_async_proxy() {
+  asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+}
+// The computing warps' barrier, and one that tells whether any thread said so.
+__device__ __forceinline__ void bar_compute() { asm volatile("barrier.cta.sync 1, 128;" ::: "memory"); }
+__device__ __forceinline__ bool bar_compute_or(int x) {
+  uint32_t r;
+  asm volatile(
+      "{\n\t.reg .pred p, q;\n\tsetp.ne.s32 p, %1, 0;\n\tbarrier.cta.red.or.pred q, 1, 128, p;\n\tselp.u32 %0, 1, 0, q;\n\t}\n"
+      : "=r"(r)
+      : "r"(x)
+      : "memory");
+  return r != 0;
+}
 
 // Bytes 0-3 of w, 4-bit codes 0..15 (offset 8), as exact fp16 values - 8..7.
 __device__ __forceinline__ void n4x4_to_h2(uint32_t w, uint32_t& a, uint32_t& b) {
@@ -170,91 +203,161 @@ __device__ __forceinline__ void row_scales(const uint8_t* p, float (&d)[NB]) {
 }
 
 template <int HD, bool KQ, bool VQ, bool SPLIT, int WM>
-__global__ void __launch_bounds__(kRowsThreads) page_rows_kernel(const PageRowsArgs a, int stages) {
+__global__ void __launch_bounds__(kRowsThreads + 32)
+    page_rows_kernel(const PageRowsArgs a, int stages, const __grid_constant__ CUtensorMap k_map,
+                     const __grid_constant__ CUtensorMap v_map) {
+  using L = RowsSmem<HD>;
   constexpr int WK = 4 / WM;                   // warps along the positions
   constexpr int KEYS = kRowsBk / WK;           // positions of a warp in a unit
   constexpr int NC = WM == 1 ? 16 : 32;        // positions per softmax step
   constexpr int NT = NC / 8, KS = HD / 16, NB = HD / 32, DT = HD / 8;
   constexpr int WROWS = SPLIT ? 8 : 16;        // rows of a warp's operand
-  constexpr int PITCH = RowsSmem<HD>::pitch;
   constexpr bool KD = KQ && WM == 1, VD = VQ && WM == 1;   // stored bytes straight into registers
-  extern __shared__ __align__(128) uint8_t smem[];
-  __shared__ int row_tab[kRowTabs][kRowsBk];
+  extern __shared__ __align__(1024) uint8_t smem_raw[];
+  uint8_t* smem = smem_raw + ((1024 - (smem_u32(smem_raw) & 1023)) & 1023);
+  uint64_t* full = reinterpret_cast<uint64_t*>(smem);      // [stages]
+  uint64_t* empty = full + kRowsStagesMax;                 // [stages]
+  int* abort_flag = reinterpret_cast<int*>(smem + 256);
+  int* last_part = abort_flag + 1;
+  uint8_t* ring = smem + kRowsCtrl;
+
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  if (tid == 0) {
+    for (int i = 0; i < stages; ++i) {
+      mbar_init(&full[i], 1);
+      mbar_init(&empty[i], 4);
+    }
+    *abort_flag = 0;
+    fence_mbar_init();
+  }
+  if (warp == 4 && lane < 2 && !(lane ? VQ : KQ))
+    asm volatile("prefetch.tensormap [%0];" ::"l"(reinterpret_cast<uint64_t>(lane ? &v_map : &k_map)) : "memory");
   pdl_wait();
   pdl_launch_dependents();
 
-  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   const int wm = WM == 1 ? 0 : warp, wk = WM == 1 ? warp : 0;
   const int g = lane >> 2, j = lane & 3;
   const PageView& c = a.c;
   const PageWork& w = a.w;
   const int G = (int)w.G.d;
 
+  const int stage_bytes = rows_stage_bytes<HD, KQ, VQ>(c.rb_k, c.rb_v);
+  const int k_bytes = KQ ? L::raw(c.rb_k) : L::tile;
   Share sh;
-  int* sums = reinterpret_cast<int*>(smem);
+  int* sums = reinterpret_cast<int*>(ring);
   sum_units(w, sums);
   __syncthreads();
   const bool have = find_share(w, blockIdx.x, gridDim.x, sums, sh);   // every warp finds the same place
   if (!have) return;
+  __syncthreads();   // the sums are read, the stages take their place
 
-  const int stage_bytes = rows_stage_bytes<HD, KQ, VQ>(c.rb_k, c.rb_v);
-  const int k_bytes = KQ ? RowsSmem<HD>::raw(c.rb_k) : RowsSmem<HD>::tile;
-  uint8_t* ring = smem;
-  uint8_t* conv_k = smem + stages * stage_bytes;
-  float* scale_k = reinterpret_cast<float*>(conv_k + RowsSmem<HD>::tile);
-  uint8_t* conv_v = conv_k + (KQ ? RowsSmem<HD>::tile + RowsSmem<HD>::scales : 0);
-  float* scale_v = reinterpret_cast<float*>(conv_v + RowsSmem<HD>::tile);
-  const float off = p_offset(c.type_v);
-
-  // ---- staging: units are numbered through the share; a cursor runs ahead ----
-  const int n_units = sh.u_end - sh.u;
-  TileAt ahead = sh.at;
-  int ahead_off = sh.off, looked = 0;   // next unit of tile `ahead` to look up; units looked up so far
-  // the row number of this thread's position of the next unit (-1: zeros)
-  auto look_up = [&]() {
-    int row = -1;
-    if (looked < n_units && tid < kRowsBk) {
-      const int p = (ahead.lo_unit + ahead_off) * kRowsBk + tid;
-      if (p >= ahead.lo && p < ahead.hi) row = (int)page_row(w.b, c, ahead.s, ahead.h, p);
-    }
-    if (++looked < n_units && ++ahead_off == ahead.units) {
-      next_tile(w, ahead);
-      ahead_off = 0;
-    }
-    return row;
+  // A wait; after one in the CTA has expired all others return.
+  auto wait = [&](uint64_t* bar, uint32_t parity, int code) -> bool {
+    for (int i = 0; !mbar_try_wait(bar, parity); ++i)
+      if (i == kWaitPolls || *reinterpret_cast<volatile int*>(abort_flag)) {
+        *reinterpret_cast<volatile int*>(abort_flag) = 1;
+        if (a.status) atomicExch(a.status, code);
+        return false;
+      }
+    return true;
   };
-  auto copy_in = [&](int u) {
-    const int* tab = row_tab[u % kRowTabs];
-    uint8_t* st = ring + (u % stages) * stage_bytes;
-    auto rows_in = [&](uint32_t dst, const uint8_t* pool, int rb, int pitch, const FastDiv& cpr) {
-      const int total = kRowsBk * (int)cpr.d;
-#pragma unroll 4
-      for (int i = tid; i < total; i += kRowsThreads) {
-        const int key = cpr.div(i), ch = i - key * (int)cpr.d, row = tab[key];
-        cp_async16(dst + key * pitch + ch * 16, pool + (row < 0 ? 0 : (int64_t)row * rb + ch * 16), row >= 0);
+
+  if (warp == 4) {
+    // ---------------- K and V ----------------
+    fence_async_proxy();
+    const int n_units = sh.u_end - sh.u;
+    const int run_log2 = min(c.ps_log2, 6), run = 1 << run_log2, runs = kRowsBk >> run_log2;   // rows of a copy
+    const int nk = KQ ? 1 : L::blocks, nv = VQ ? 1 : L::blocks;   // copies of a run
+    const int total = runs * (nk + nv);
+    constexpr int PER = (8 * 2 * L::blocks + 31) / 32;            // copies of a lane, pages of 8 positions
+    int y[PER], next_y[PER];                                      // row of each copy's run, -1: zeros
+    auto look_up = [&](int (&row)[PER]) {
+#pragma unroll
+      for (int e = 0; e < PER; ++e) {
+        const int i = lane + 32 * e, p = (sh.at.lo_unit + sh.off) * kRowsBk + (i & (runs - 1)) * run;
+        row[e] = -1;
+        if (i < total && p < sh.at.hi && p + run > sh.at.lo) row[e] = (int)page_row(w.b, c, sh.at.s, sh.at.h, p);
       }
     };
-    rows_in(smem_u32(st), c.k, c.rb_k, KQ ? c.rb_k : PITCH, a.cpr_k);
-    rows_in(smem_u32(st + k_bytes), c.v, c.rb_v, VQ ? c.rb_v : PITCH, a.cpr_v);
-  };
-  {
-    int row[4];   // of the first units (at most 4 stages)
+    look_up(next_y);
+    bool ok = true, wrote = false;
+    int n = 0;
+    for (; n < n_units; ++n) {
+      uint8_t* st = ring + (n % stages) * stage_bytes;
+      uint64_t* bar = &full[n % stages];
+      const TileAt& at = sh.at;
+      const int key0 = (at.lo_unit + sh.off) * kRowsBk, lo = at.lo, hi = at.hi;
+      uint32_t bytes = 0;
 #pragma unroll
-    for (int n = 0; n < 4; ++n)
-      if (n < stages) row[n] = look_up();
+      for (int e = 0; e < PER; ++e) {
+        y[e] = next_y[e];
+        const int i = lane + 32 * e, r = i >> (6 - run_log2);   // which copy of its run
+        // runs without a page that the tile needs are zeroed by hand when quantized
+        if (i < total) bytes += r < nk ? (KQ ? (y[e] >= 0 ? run * c.rb_k : 0) : run * 128)
+                                       : (VQ ? (y[e] >= 0 ? run * c.rb_v : 0) : run * 128);
+      }
+      bytes = __reduce_add_sync(0xffffffffu, bytes);
+      if (n + 1 < n_units) {
+        if (++sh.off == sh.at.units) {
+          next_tile(w, sh.at);
+          sh.off = 0;
+        }
+        look_up(next_y);
+      }
+      if (n >= stages) ok = __all_sync(0xffffffffu, wait(&empty[n % stages], (n / stages - 1) & 1, 50));
+      if (!ok) break;
+      if (wrote) fence_async_proxy();   // a stage may hold rows zeroed by hand
 #pragma unroll
-    for (int n = 0; n < 4; ++n)
-      if (n < stages && tid < kRowsBk) row_tab[n][tid] = row[n];
+      for (int e = 0; e < PER; ++e) {
+        const int i = lane + 32 * e, r = i >> (6 - run_log2), first = (i & (runs - 1)) * run;
+        const bool is_v = r >= nk, quant = is_v ? VQ : KQ;
+        bool zero = false;
+        if (i < total && quant && y[e] < 0) {
+          const int p = key0 + first;
+          if (p < hi && p + run > lo) {   // a missing page, not a run past the positions
+            uint4* d = reinterpret_cast<uint4*>(st + (is_v ? k_bytes : 0) + first * (is_v ? c.rb_v : c.rb_k));
+            for (int x = 0; x < run * (is_v ? c.rb_v : c.rb_k) / 16; ++x) d[x] = make_uint4(0, 0, 0, 0);
+            zero = true;
+          }
+        }
+        wrote |= __any_sync(0xffffffffu, zero);
+      }
+      __syncwarp();
+      if (lane == 0) mbar_arrive_expect_tx(bar, bytes);
+      __syncwarp();
+#pragma unroll
+      for (int e = 0; e < PER; ++e) {
+        const int i = lane + 32 * e, r = i >> (6 - run_log2), first = (i & (runs - 1)) * run;
+        if (i >= total) continue;
+        if (r < nk) {
+          if (!KQ)
+            tma_2d(smem_u32(st) + r * (kRowsBk * 128) + first * 128, &k_map, r * 64, (int)(y[e] < 0 ? a.pool_rows : y[e]), bar);
+          else if (y[e] >= 0)
+            bulk_g2s(st + first * c.rb_k, c.k + (int64_t)y[e] * c.rb_k, run * c.rb_k, bar);
+        } else {
+          if (!VQ)
+            tma_2d(smem_u32(st + k_bytes) + (r - nk) * (kRowsBk * 128) + first * 128, &v_map, (r - nk) * 64,
+                   (int)(y[e] < 0 ? a.pool_rows : y[e]), bar);
+          else if (y[e] >= 0)
+            bulk_g2s(st + k_bytes + first * c.rb_v, c.v + (int64_t)y[e] * c.rb_v, run * c.rb_v, bar);
+        }
+      }
+    }
+    // every copy issued has landed before the CTA may end
+    for (int i = max(0, n - stages); i < n; ++i) mbar_wait_bounded(&full[i % stages], (i / stages) & 1, a.status, 51);
+    return;
   }
-  __syncthreads();   // also: the sums are read, the stages take their place
-  for (int n = 0; n < stages - 1; ++n) {
-    if (n < n_units) copy_in(n);
-    cp_async_commit();
-  }
-  int next_row = look_up();   // of unit `stages`
+
+  uint8_t* conv_k = ring + stages * stage_bytes;
+  float* scale_k = reinterpret_cast<float*>(conv_k + L::tile);
+  uint8_t* conv_v = conv_k + (KQ ? L::tile + L::scales : 0);
+  float* scale_v = reinterpret_cast<float*>(conv_v + L::tile);
+  const float off = p_offset(c.type_v);
 
   // Quantized rows of a stage -> fp16 codes and fp32 scales [block][position] (WM = 4).
-  auto unpack = [&](const uint8_t* raw, int type, int rb, uint8_t* dst, float* sc, const FastDiv& cpr) {
+  auto unpack = [&](const uint8_t* raw, int type, int rb, uint8_t* dst, float* sc, const FastDiv& cpr, int lo, int hi,
+                    bool guard) {
+    int found = 0;   // infinite or NaN scales, taken out when guarded; rows outside [lo, hi) count as zeros
     const int cb = type == B2_Q8_0 ? HD : HD / 2;
     const int cpk = (int)cpr.d - 1, total = kRowsBk * (int)cpr.d;   // a row: code chunks, then the scales'
 #pragma unroll 2
@@ -265,7 +368,11 @@ __global__ void __launch_bounds__(kRowsThreads) page_rows_kernel(const PageRowsA
         float d[NB];
         row_scales<NB>(row + cb, d);
 #pragma unroll
-        for (int b = 0; b < NB; ++b) sc[b * kRowsBk + key] = d[b];
+        for (int b = 0; b < NB; ++b) {
+          if (key < lo || key >= hi) d[b] = 0.f;
+          if (guard && !(fabsf(d[b]) <= 65504.f)) d[b] = 0.f, found = 1;
+          sc[b * kRowsBk + key] = d[b];
+        }
         continue;
       }
       const uint4 x = *reinterpret_cast<const uint4*>(row + ch * 16);
@@ -275,25 +382,24 @@ __global__ void __launch_bounds__(kRowsThreads) page_rows_kernel(const PageRowsA
         s8x4_to_h2(x.y, h[2], h[3]);
         s8x4_to_h2(x.z, h[4], h[5]);
         s8x4_to_h2(x.w, h[6], h[7]);
-        uint4* t = reinterpret_cast<uint4*>(dst + key * PITCH + ch * 32);
-        t[0] = make_uint4(h[0], h[1], h[2], h[3]);
-        t[1] = make_uint4(h[4], h[5], h[6], h[7]);
+        *reinterpret_cast<uint4*>(dst + L::at(key, 2 * ch)) = make_uint4(h[0], h[1], h[2], h[3]);
+        *reinterpret_cast<uint4*>(dst + L::at(key, 2 * ch + 1)) = make_uint4(h[4], h[5], h[6], h[7]);
       } else {
-        uint4* t = reinterpret_cast<uint4*>(dst + key * PITCH + ch * 64);
         n4x4_to_h2(x.x & 0x0F0F0F0Fu, h[0], h[1]);
         n4x4_to_h2(x.y & 0x0F0F0F0Fu, h[2], h[3]);
         n4x4_to_h2(x.z & 0x0F0F0F0Fu, h[4], h[5]);
         n4x4_to_h2(x.w & 0x0F0F0F0Fu, h[6], h[7]);
-        t[0] = make_uint4(h[0], h[1], h[2], h[3]);
-        t[1] = make_uint4(h[4], h[5], h[6], h[7]);
+        *reinterpret_cast<uint4*>(dst + L::at(key, 4 * ch)) = make_uint4(h[0], h[1], h[2], h[3]);
+        *reinterpret_cast<uint4*>(dst + L::at(key, 4 * ch + 1)) = make_uint4(h[4], h[5], h[6], h[7]);
         n4x4_to_h2((x.x >> 4) & 0x0F0F0F0Fu, h[0], h[1]);
         n4x4_to_h2((x.y >> 4) & 0x0F0F0F0Fu, h[2], h[3]);
         n4x4_to_h2((x.z >> 4) & 0x0F0F0F0Fu, h[4], h[5]);
         n4x4_to_h2((x.w >> 4) & 0x0F0F0F0Fu, h[6], h[7]);
-        t[2] = make_uint4(h[0], h[1], h[2], h[3]);
-        t[3] = make_uint4(h[4], h[5], h[6], h[7]);
+        *reinterpret_cast<uint4*>(dst + L::at(key, 4 * ch + 2)) = make_uint4(h[0], h[1], h[2], h[3]);
+        *reinterpret_cast<uint4*>(dst + L::at(key, 4 * ch + 3)) = make_uint4(h[4], h[5], h[6], h[7]);
       }
     }
+    return found;
   };
 
   int done = 0;   // units of the share so far
@@ -359,13 +465,6 @@ __global__ void __launch_bounds__(kRowsThreads) page_rows_kernel(const PageRowsA
     const int p_min = at.first + w.G.div(row0), p_max = at.first + w.G.div(row0 + rows - 1);
 
     for (int u = u_lo; u < u_hi; ++u, ++done) {
-      // all but the newest stages - 2 groups have landed
-      if (stages == 4) cp_async_wait<2>(); else if (stages == 3) cp_async_wait<1>(); else cp_async_wait<0>();
-      __syncthreads();   // the unit is here; everyone is done with the one before, whose stage the next copy takes
-      if (done + stages - 1 < n_units) copy_in(done + stages - 1);
-      cp_async_commit();
-      if (tid < kRowsBk) row_tab[(done + stages) % kRowTabs][tid] = next_row;
-      next_row = look_up();
       uint8_t* st = ring + (done % stages) * stage_bytes;
       const int key0 = (at.lo_unit + u) * kRowsBk;
       const bool edge = key0 + kRowsBk > at.hi || key0 + kRowsBk - 1 > p_min ||
@@ -376,43 +475,47 @@ __global__ void __launch_bounds__(kRowsThreads) page_rows_kernel(const PageRowsA
       const bool guard = edge && p_max > p_min;
       int found = 0;
       bool bad = false;
-      if constexpr (KQ && !KD) unpack(st, c.type_k, c.rb_k, conv_k, scale_k, a.cpr_k);
-      if constexpr (VQ && !VD) unpack(st + k_bytes, c.type_v, c.rb_v, conv_v, scale_v, a.cpr_v);
+      wait(&full[done % stages], (done / stages) & 1, 52);
       uint8_t* Kt = KQ && !KD ? conv_k : st;
       uint8_t* Vt = VQ && !VD ? conv_v : st + k_bytes;
-      const uint32_t ks_base = smem_u32(Kt), vs_base = smem_u32(Vt);
-      if (guard && !VD) {
-        if constexpr (VQ) {
-          __syncthreads();   // the scales are written
-          for (int i = tid; i < kRowsBk * NB; i += kRowsThreads)
-            if (!(fabsf(scale_v[i]) <= 65504.f)) {
-              scale_v[i] = 0.f;
-              found = 1;
+      const int v_lo = edge ? at.lo - key0 : 0, v_hi = edge ? at.hi - key0 : kRowsBk;   // rows of V the tile sees
+      if constexpr (WM == 4) {
+        if constexpr (KQ || VQ) bar_compute();   // the last unit's operands are done with
+        if constexpr (KQ) unpack(st, c.type_k, c.rb_k, conv_k, scale_k, a.cpr_k, 0, kRowsBk, false);
+        if constexpr (VQ) found = unpack(st + k_bytes, c.type_v, c.rb_v, conv_v, scale_v, a.cpr_v, v_lo, v_hi, guard);
+      }
+      if (!VQ && edge) {
+        // WM = 1: a warp looks over its own positions
+        constexpr int CH = L::blocks * 8;
+        const int n = (WM == 1 ? KEYS : kRowsBk) * CH;
+        for (int i = WM == 1 ? lane : tid; i < n; i += WM == 1 ? 32 : kRowsThreads) {
+          const int key = (WM == 1 ? wk * KEYS : 0) + i / CH;
+          uint4* q = reinterpret_cast<uint4*>(Vt + L::at(key, i % CH));
+          if (key < v_lo || key >= v_hi) {
+            *q = make_uint4(0, 0, 0, 0);
+          } else if (guard) {
+            uint4 x = *q;
+            uint32_t* v = reinterpret_cast<uint32_t*>(&x);
+            bool changed = false;
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+              if ((v[e] & 0x7C00u) == 0x7C00u) v[e] &= 0xFFFF0000u, changed = true;
+              if ((v[e] & 0x7C000000u) == 0x7C000000u) v[e] &= 0xFFFFu, changed = true;
             }
-        } else {
-          // WM = 1: a warp looks over its own positions
-          const int first = WM == 1 ? wk * KEYS : 0, n = WM == 1 ? KEYS : kRowsBk;
-          for (int i = WM == 1 ? lane : tid; i < n * (HD / 2); i += WM == 1 ? 32 : kRowsThreads) {
-            const int key = i / (HD / 2), x = i - key * (HD / 2);
-            uint32_t* p = reinterpret_cast<uint32_t*>(Vt + (first + key) * PITCH) + x;
-            uint32_t v = *p;
-            if ((v & 0x7C00u) == 0x7C00u) v &= 0xFFFF0000u;
-            if ((v & 0x7C000000u) == 0x7C000000u) v &= 0xFFFFu;
-            if (v != *p) {
-              *p = v;
-              found = 1;
-            }
+            if (changed) *q = x, found = 1;
           }
         }
-        if constexpr (WM == 1) {
-          __syncwarp();
-          bad = __any_sync(0xffffffffu, found);
-        } else {
-          bad = __syncthreads_or(found);
-        }
-      } else if constexpr (WM != 1 && (KQ || VQ)) {
-        __syncthreads();
       }
+      if constexpr (WM == 4) {
+        if (edge)
+          bad = bar_compute_or(found);
+        else if (KQ || VQ)
+          bar_compute();
+      } else if (!VQ && edge) {
+        __syncwarp();
+        bad = __any_sync(0xffffffffu, found);
+      }
+      const uint32_t ks_base = smem_u32(Kt), vs_base = smem_u32(Vt);
 
       for (int c0 = 0; c0 < KEYS; c0 += NC) {
         const int kw = wk * KEYS + c0;   // first position of this step within the unit
@@ -441,7 +544,7 @@ __global__ void __launch_bounds__(kRowsThreads) page_rows_kernel(const PageRowsA
                 n4x4_to_h2((x >> 4) & 0x0F0F0F0Fu, kf[2], kf[3]);
               }
             } else {
-              ldsm4(ks_base + (kw + n * 8 + (lane & 7)) * PITCH + b * 64 + (lane >> 3) * 16, kf);
+              ldsm4(ks_base + L::at(kw + n * 8 + (lane & 7), b * 4 + (lane >> 3)), kf);
             }
             if constexpr (KQ) {
               float t[4] = {0.f, 0.f, 0.f, 0.f};
@@ -543,15 +646,16 @@ __global__ void __launch_bounds__(kRowsThreads) page_rows_kernel(const PageRowsA
             row_scales<NB>(sr + c.rb_v, sc[1]);
             row_scales<NB>(sr + 8 * c.rb_v, sc[2]);
             row_scales<NB>(sr + 9 * c.rb_v, sc[3]);
-            if (guard) {
+            if (edge) {
 #pragma unroll
-              for (int r = 0; r < 4; ++r)
+              for (int r = 0; r < 4; ++r) {
+                const int key = kw + k * 16 + 2 * j + (r & 1) + (r >> 1) * 8;
 #pragma unroll
-                for (int b = 0; b < NB; ++b)
-                  if (!(fabsf(sc[r][b]) <= 65504.f)) {
-                    sc[r][b] = 0.f;
-                    found = 1;
-                  }
+                for (int b = 0; b < NB; ++b) {
+                  if (key < v_lo || key >= v_hi) sc[r][b] = 0.f;
+                  if (guard && !(fabsf(sc[r][b]) <= 65504.f)) sc[r][b] = 0.f, found = 1;
+                }
+              }
             }
           }
 #pragma unroll
@@ -584,7 +688,7 @@ __global__ void __launch_bounds__(kRowsThreads) page_rows_kernel(const PageRowsA
 #pragma unroll
               for (int d = 0; d < 2; ++d) {
                 uint32_t vf[4];   // 16 positions x 16 dims
-                ldsm4_t(vs_base + (kw + k * 16 + (lane & 15)) * PITCH + (b * 32 + d * 16 + (lane >> 4) * 8) * 2, vf);
+                ldsm4_t(vs_base + L::at(kw + k * 16 + (lane & 15), b * 4 + 2 * d + (lane >> 4)), vf);
                 mma16816(o[b * 4 + 2 * d], pf, vf[0], vf[1]);
                 mma16816(o[b * 4 + 2 * d + 1], pf, vf[2], vf[3]);
               }
@@ -593,6 +697,8 @@ __global__ void __launch_bounds__(kRowsThreads) page_rows_kernel(const PageRowsA
         }
       }
       if (VD && guard) bad = __any_sync(0xffffffffu, found);
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&empty[done % stages]);
       if (bad) {
         // infinite and NaN values of V, to the rows that see them (their
         // weight is positive, so the value itself decides the sum)
@@ -657,14 +763,13 @@ __global__ void __launch_bounds__(kRowsThreads) page_rows_kernel(const PageRowsA
 
     if constexpr (WM == 1) {
       // [4 warps][16] (m, l), then [4 warps][WROWS][HD] sums, after the ring
-      float2* ml = reinterpret_cast<float2*>(smem + stages * stage_bytes);
+      float2* ml = reinterpret_cast<float2*>(ring + stages * stage_bytes);
       float* so = reinterpret_cast<float*>(ml + 64);
-      int* last_part = reinterpret_cast<int*>(so + 4 * WROWS * HD);
       if (j == 0) {
         ml[warp * 16 + g] = make_float2(m0, l0);
         if constexpr (!SPLIT) ml[warp * 16 + g + 8] = make_float2(m1, l1);
       }
-      __syncthreads();
+      bar_compute();
       auto top = [&](int r) {
         return fmaxf(fmaxf(ml[r].x, ml[16 + r].x), fmaxf(ml[32 + r].x, ml[48 + r].x));
       };
@@ -680,7 +785,7 @@ __global__ void __launch_bounds__(kRowsThreads) page_rows_kernel(const PageRowsA
           so[(warp * WROWS + g) * HD + i] = l0 != 0.f ? o[d][e] * f0 : 0.f;
           if constexpr (!SPLIT) so[(warp * WROWS + g + 8) * HD + i] = l1 != 0.f ? o[d][2 + e] * f1 : 0.f;
         }
-      __syncthreads();
+      bar_compute();
       for (int i = tid; i < rows * (HD / 2); i += kRowsThreads) {
         const int r = i / (HD / 2), d = 2 * (i - r * (HD / 2));
         const float t = top(r);
@@ -705,12 +810,12 @@ __global__ void __launch_bounds__(kRowsThreads) page_rows_kernel(const PageRowsA
       if (!whole) {
         // all warps' shares of the rows are written before one counts the part
         __threadfence();
-        __syncthreads();
+        bar_compute();
         if (warp == 0) {
           const bool last = part_arrives(a.counters + split.cta0 * 8, split.n);
           if (lane == 0) *last_part = last;
         }
-        __syncthreads();
+        bar_compute();
         if (*reinterpret_cast<volatile int*>(last_part)) {
           constexpr int R = WROWS / 4;
           const int r = warp * R;
@@ -719,7 +824,7 @@ __global__ void __launch_bounds__(kRowsThreads) page_rows_kernel(const PageRowsA
                                       a.q_f32 != 0);
         }
       }
-      __syncthreads();   // the join's space is free for the next tile
+      bar_compute();   // the join's space is free for the next tile
     } else {
       const float i0 = !whole ? 1.f : l0 != 0.f ? 1.f / l0 : 0.f, i1 = !whole ? 1.f : l1 != 0.f ? 1.f / l1 : 0.f;
       const int r = wm * WROWS + g;
@@ -749,7 +854,6 @@ __global__ void __launch_bounds__(kRowsThreads) page_rows_kernel(const PageRowsA
     sh.off = 0;
     if (sh.u < sh.u_end) next_tile(w, sh.at);
   }
-  cp_async_wait<0>();
 }
 
 int launch_page_rows_64(const PageRowsArgs& a, bool split, int wm, cudaStream_t s);
@@ -757,20 +861,26 @@ int launch_page_rows_96(const PageRowsArgs& a, bool split, int wm, cudaStream_t 
 int launch_page_rows_128(const PageRowsArgs& a, bool split, int wm, cudaStream_t s);
 int launch_page_rows_256(const PageRowsArgs& a, bool split, int wm, cudaStream_t s);
 
+// Tensor map of one layer's pool as [rows][hd] fp16, copied in boxes of
+// box_rows x 64 dims, 128-byte swizzled (b2_page_tc.cu).
+int page_pool_map(const void* base, int hd, int64_t rows, int box_rows, CUtensorMap* map);
+
 // The ring, then what the tile's end needs beside it (WM = 1: the next tile's
 // units are already on their way).
 template <int HD, bool KQ, bool VQ, bool SPLIT, int WM>
 inline int rows_smem_bytes(const PageRowsArgs& a, int stages) {
   const int ring = stages * rows_stage_bytes<HD, KQ, VQ>(a.c.rb_k, a.c.rb_v) + rows_conv_bytes<HD, KQ, VQ, WM>();
-  const int join = WM == 1 ? 64 * 8 + 4 * (SPLIT ? 8 : 16) * HD * 4 + 16 : 0, sums = kPageMaxSeq * 4;
-  return std::max(ring + join, sums);
+  const int join = WM == 1 ? 64 * 8 + 4 * (SPLIT ? 8 : 16) * HD * 4 : 0, sums = kPageMaxSeq * 4;
+  return 1024 + kRowsCtrl + std::max(ring + join, sums);   // the first for alignment
 }
 
 template <int HD, bool KQ, bool VQ, bool SPLIT, int WM>
 int launch_page_rows_one(PageRowsArgs a, cudaStream_t s) {
-  // A ring that leaves two CTAs or more on an SM where it can (head_dim 256
+  // The deepest ring that leaves two CTAs on an SM where it can (head_dim 256
   // with fp16 rows: one).
-  const int stages = HD == 256 && !(KQ && VQ) ? 2 : WM == 1 && KQ && VQ ? 4 : 3;
+  const int stage = rows_stage_bytes<HD, KQ, VQ>(a.c.rb_k, a.c.rb_v);
+  int stages = kRowsStagesMax;
+  while (stages > 2 && rows_smem_bytes<HD, KQ, VQ, SPLIT, WM>(a, stages) > (stage > 40 * 1024 ? 226 : 112) * 1024) --stages;
   const int smem = rows_smem_bytes<HD, KQ, VQ, SPLIT, WM>(a, stages);
   auto kern = page_rows_kernel<HD, KQ, VQ, SPLIT, WM>;
   // looked up once per device and cache type pair
@@ -781,15 +891,21 @@ int launch_page_rows_one(PageRowsArgs a, cudaStream_t s) {
   std::atomic<int>& known = resident[dev][a.c.type_k == B2_Q4_0][a.c.type_v == B2_Q4_0];
   int per_sm = known.load(std::memory_order_relaxed);
   if (per_sm == 0) {
-    B2_CUDA_TRY(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, 225 * 1024));
-    B2_CUDA_TRY(cudaOccupancyMaxActiveBlocksPerMultiprocessor(&per_sm, kern, kRowsThreads, smem));
+    B2_CUDA_TRY(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, 227 * 1024));
+    B2_CUDA_TRY(cudaOccupancyMaxActiveBlocksPerMultiprocessor(&per_sm, kern, kRowsThreads + 32, smem));
     per_sm = std::max(1, std::min(per_sm, kPageMaxCtasPerSm));
     known.store(per_sm, std::memory_order_relaxed);
   }
   a.cpr_k = FastDiv::of(a.c.rb_k / 16);
   a.cpr_v = FastDiv::of(a.c.rb_v / 16);
+  CUtensorMap km = {}, vm = {};
+  const int box = std::min(1 << a.c.ps_log2, kRowsBk);
+  int rc = B2_OK;
+  if (!KQ) rc = page_pool_map(a.c.k, HD, a.pool_rows, box, &km);
+  if (rc == B2_OK && !VQ) rc = page_pool_map(a.c.v, HD, a.pool_rows, box, &vm);
+  if (rc != B2_OK) return rc;
   const int ctas = per_sm * sm_count();
-  return launch_pdl(kern, dim3(ctas), dim3(kRowsThreads), (size_t)smem, s, a, stages);
+  return launch_pdl(kern, dim3(ctas), dim3(kRowsThreads + 32), (size_t)smem, s, a, stages, km, vm);
 }
 
 template <int HD>

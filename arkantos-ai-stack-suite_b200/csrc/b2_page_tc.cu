@@ -4,7 +4,7 @@
 namespace b2 {
 namespace {
 
-int encode(CUtensorMap* map, const void* base, int rank, const cuuint64_t* dims, const cuuint64_t* strides,
+int encode_map(CUtensorMap* map, const void* base, int rank, const cuuint64_t* dims, const cuuint64_t* strides,
            const cuuint32_t* box) {
   static std::atomic<PFN_cuTensorMapEncodeTiled> found{nullptr};
   PFN_cuTensorMapEncodeTiled fn = found.load(std::memory_order_relaxed);
@@ -29,20 +29,13 @@ int encode(CUtensorMap* map, const void* base, int rank, const cuuint64_t* dims,
   return B2_OK;
 }
 
-// One layer's pool as [rows][hd] fp16, copied in boxes of one page (at most
-// 128 rows) x 64 dims, 128-byte swizzled.
-int pool_map(const void* base, int hd, int64_t rows, int box_rows, CUtensorMap* map) {
-  const cuuint64_t dims[2] = {(cuuint64_t)hd, (cuuint64_t)rows}, strides[1] = {(cuuint64_t)hd * 2};
-  const cuuint32_t box[2] = {64, (cuuint32_t)box_rows};
-  return encode(map, base, 2, dims, strides, box);
-}
 // Queries [n_tok][n_head][hd], copied as the 128 rows (token, head of the
 // group) of half a tile x 64 dims.
 int query_map(const void* q, int hd, int n_head, int n_tok, int G, CUtensorMap* map) {
   const cuuint64_t dims[3] = {(cuuint64_t)hd, (cuuint64_t)n_head, (cuuint64_t)n_tok};
   const cuuint64_t strides[2] = {(cuuint64_t)hd * 2, (cuuint64_t)n_head * hd * 2};
   const cuuint32_t box[3] = {64, (cuuint32_t)G, (cuuint32_t)(128 / G)};
-  return encode(map, q, 3, dims, strides, box);
+  return encode_map(map, q, 3, dims, strides, box);
 }
 
 template <int HD, bool SPLIT>
@@ -62,14 +55,19 @@ int launch(const PageTcArgs& a, const CUtensorMap& km, const CUtensorMap& vm, co
 
 }  // namespace
 
+int page_pool_map(const void* base, int hd, int64_t rows, int box_rows, CUtensorMap* map) {
+  const cuuint64_t dims[2] = {(cuuint64_t)hd, (cuuint64_t)rows}, strides[1] = {(cuuint64_t)hd * 2};
+  const cuuint32_t box[2] = {64, (cuuint32_t)box_rows};
+  return encode_map(map, base, 2, dims, strides, box);
+}
+
 int launch_page_tc(PageTcArgs a, int hd, bool split, int page_size, cudaStream_t s) {
   const int box = std::min(page_size, kTcBk);
   a.box_rows_log2 = 0;
   while ((1 << a.box_rows_log2) < box) ++a.box_rows_log2;
-  a.pool_rows = (int64_t)a.c.n_pages * a.c.n_kv * page_size;
   CUtensorMap km, vm, qm = {};
-  int rc = pool_map(a.c.k, hd, a.pool_rows, box, &km);
-  if (rc == B2_OK) rc = pool_map(a.c.v, hd, a.pool_rows, box, &vm);
+  int rc = page_pool_map(a.c.k, hd, a.pool_rows, box, &km);
+  if (rc == B2_OK) rc = page_pool_map(a.c.v, hd, a.pool_rows, box, &vm);
   const int G = (int)a.w.G.d;
   a.q_map = !split && 128 % G == 0;
   if (rc == B2_OK && a.q_map) rc = query_map(a.q, hd, a.n_head, a.w.b.n_tok, G, &qm);

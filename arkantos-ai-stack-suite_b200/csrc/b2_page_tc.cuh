@@ -80,7 +80,6 @@ struct PageTcArgs {
 
 constexpr int kTcRows = 256, kTcBk = 128, kTcThreads = 384;
 constexpr float kTcOffset = 7.f, kTcRaise = 8.f;
-constexpr int kTcPolls = 1 << 22;   // polls of a wait, each suspended by the hardware for a while
 
 template <int HD, bool SPLIT>
 struct TcSmem {
@@ -134,10 +133,6 @@ __device__ __forceinline__ void tc_commit(uint64_t* bar) {
 }
 __device__ __forceinline__ void tc_before() { asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory"); }
 __device__ __forceinline__ void tc_after() { asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory"); }
-__device__ __forceinline__ void fence_async_proxy() {
-  asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
-}
-
 // Columns of the warp's 32 lanes; the wait is in the same asm block, so no
 // register can be used before it.
 __device__ __forceinline__ void tmem_ld32(uint32_t t, float* r) {
@@ -234,14 +229,6 @@ __device__ __forceinline__ void tma_3d(uint32_t dst, const CUtensorMap* map, int
       "l"(reinterpret_cast<uint64_t>(map)), "r"(smem_u32(bar)), "r"(x), "r"(y), "r"(z)
       : "memory");
 }
-__device__ __forceinline__ void tma_2d(uint32_t dst, const CUtensorMap* map, int x, int y, uint64_t* bar) {
-  asm volatile(
-      "cp.async.bulk.tensor.2d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4}], [%2];" ::"r"(
-          dst),
-      "l"(reinterpret_cast<uint64_t>(map)), "r"(smem_u32(bar)), "r"(x), "r"(y)
-      : "memory");
-}
-
 // A tile of the CTA's share as the warps see it.
 struct TcTile {
   int h, s, q0, first;            // kv head, sequence; its first new token's row and position
@@ -335,7 +322,7 @@ __global__ void __launch_bounds__(kTcThreads, 1)
   // A wait of one thread; after one in the CTA has expired all others return.
   auto wait = [&](uint64_t* bar, uint32_t parity, int code) -> bool {
     for (int i = 0; !mbar_try_wait(bar, parity); ++i)
-      if (i == kTcPolls || *reinterpret_cast<volatile int*>(abort_flag)) {
+      if (i == kWaitPolls || *reinterpret_cast<volatile int*>(abort_flag)) {
         *reinterpret_cast<volatile int*>(abort_flag) = 1;
         if (a.status) atomicExch(a.status, code);
         return false;
@@ -891,10 +878,9 @@ __global__ void __launch_bounds__(kTcThreads, 1)
 }
 
 int launch_page_tc(PageTcArgs a, int hd, bool split, int page_size, cudaStream_t s);
-// Pools a tensor map can describe, in pages that hold whole 8-row groups.
+// The caches this kernel reads.
 inline bool page_tc_ok(const PageView& c, int hd) {
-  return (hd == 64 || hd == 128) && c.type_k == B2_F16 && c.type_v == B2_F16 && c.ps_log2 >= 3 &&
-         (((int64_t)c.n_pages * c.n_kv) << c.ps_log2) < (int64_t)1 << 31;
+  return (hd == 64 || hd == 128) && c.type_k == B2_F16 && c.type_v == B2_F16;
 }
 
 }  // namespace b2

@@ -349,7 +349,7 @@ B2_API int b2_flag_wait(const uint64_t* flags, int n, uint64_t target, int* stat
  * k and v are device pools of b2_page_cache_bytes bytes each (16-byte
  * aligned): [n_layer][n_pages][n_kv][page_size] rows of
  * b2_kv_row_bytes(type, head_dim) bytes, in the storage of the typed caches
- * above.  page_size a power of two, 1..256; head_dim a multiple of 32 up to
+ * above.  page_size a power of two, 8..256; head_dim a multiple of 32 up to
  * 256 (attention: 64, 96, 128 and 256). */
 typedef struct b2_page_cache {
     void*   k;

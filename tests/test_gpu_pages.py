@@ -194,7 +194,7 @@ def test_attn_chunks(q_len, kv_len, qt):
     Setup(q_len, kv_len, 8, 2, 128, 16, qt=qt, seed=sum(kv_len)).check()
 
 
-@pytest.mark.parametrize("page", [1, 2, 8, 64, 256])
+@pytest.mark.parametrize("page", [8, 16, 32, 64, 128, 256])
 @pytest.mark.parametrize("q_len", [1, 40])
 def test_attn_page_sizes(page, q_len):
     Setup([q_len, q_len], [q_len + 70, q_len + 257], 4, 2, 64, page, qt=F16, seed=page).check()
@@ -440,7 +440,7 @@ def test_copy(kt, vt, n_copy):
 
 
 @pytest.mark.parametrize("kt,vt", [(F16, F16), (Q8, Q4)])
-@pytest.mark.parametrize("page", [1, 16, 64])
+@pytest.mark.parametrize("page", [8, 16, 64])
 def test_gather(kt, vt, page):
     """Kept positions move to fresh pages in every layer; a list of none, of
     one, of all; pages that stay are not touched."""

@@ -196,7 +196,7 @@ def test_cache_bytes():
     assert c.bytes_k == 2 * 4 * 2 * 16 * 80 and c.bytes_v == 2 * 4 * 2 * 16 * 48
 
 
-@pytest.mark.parametrize("bad", [dict(page_size=24), dict(page_size=512), dict(head_dim=40), dict(head_dim=288),
+@pytest.mark.parametrize("bad", [dict(page_size=24), dict(page_size=4), dict(page_size=512), dict(head_dim=40), dict(head_dim=288),
                                  dict(type_k=b2.Q4_K), dict(n_pages=0), dict(n_layer=0), dict(n_kv=0)])
 def test_cache_refusals(bad):
     with pytest.raises(b2.B2Error):
