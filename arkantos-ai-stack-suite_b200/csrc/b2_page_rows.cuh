@@ -13,11 +13,12 @@
 // Exactness.  Cache values enter the products exactly: fp16 as they are,
 // Q8_0 / Q4_0 as their integer codes in fp16, the block scale applied in fp32
 // to K's block sums and to p for V (a row of K or V is never rounded to
-// fp16).  In the SPLIT form a row of the 16-row operand is a pair: rows 0-7
-// hold the high fp16 part of q (scaled in fp32), rows 8-15 the remainder, and
-// likewise for p, so fp32 queries keep 22 bits and the output is good to
-// fp32 accuracy at no further cost while a tile has 8 rows or fewer.  The
-// FULL form (fp16 queries and outputs) rounds p once to fp16, the size of
+// fp16).  In the SPLIT form a tile has 8 rows: rows 0-7 of q's operand hold the
+// high fp16 part of q (scaled in fp32), rows 8-15 the remainder, and the
+// weights, also as two parts, are the 8-column operand of O^T = V^T·P^T, which
+// is where the scores' lanes already hold them; so fp32 queries keep 22 bits
+// and the output is good to fp32 accuracy, with half the accumulators that
+// P·V would take.  The FULL form (fp16 queries and outputs) rounds p once to fp16, the size of
 // error the fp16 output has by itself.  Accumulators, maxima and sums are
 // fp32.
 //
@@ -33,8 +34,8 @@
 // 16-row operand and their results are joined at the end of a tile; quantized
 // rows go from their stored bytes straight into the operands' registers: the
 // order of the dims within a block is free in q·k (q is loaded in the same
-// order), and in P·V a byte permute pairs two positions' codes, a lane then
-// holding 8 consecutive dims of the result.  WM = 4: each warp has its own
+// order), and for V a byte permute pairs two positions' codes, which fixes the
+// dims a lane holds of the result.  WM = 4: each warp has its own
 // 16-row operand and runs over all 64 positions; quantized rows are unpacked
 // to fp16 codes once for all of them.
 #pragma once
@@ -81,7 +82,7 @@ __device__ __forceinline__ void ldsm4_t(uint32_t a, uint32_t (&r)[4]) {
                : "memory");
 }
 __device__ __forceinline__ void mma16816(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
-  asm volatile(
+  asm(
       "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
       : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
       : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
@@ -137,6 +138,14 @@ template <int HD, bool KQ, bool VQ, int WM>
 __host__ __device__ inline int rows_conv_bytes() {
   return WM == 1 ? 0
                  : (KQ ? RowsSmem<HD>::tile + RowsSmem<HD>::scales : 0) + (VQ ? RowsSmem<HD>::tile + RowsSmem<HD>::scales : 0);
+}
+// CTAs meant for an SM: registers and the ring are cut to fit.  Reading
+// quantized rows is bound by the latency of the code's own steps, not by HBM,
+// and gains from a third (64 sequences of 4096 over Q8_0: 167 -> 156 us);
+// fp16 rows of head_dim 128 do not (97 us against 98 for 32 of them).
+template <int HD, bool KQ, bool VQ, bool SPLIT>
+__host__ __device__ constexpr int rows_ctas() {
+  return HD == 256 ? 1 : HD == 64 || (KQ && VQ && SPLIT) ? 3 : 2;
 }
 constexpr int kRowsStagesMax = 8, kRowsCtrl = 1024;
 constexpr int kWaitPolls = 1 << 22;   // polls of a wait, each suspended by the hardware for a while
@@ -203,14 +212,14 @@ __device__ __forceinline__ void row_scales(const uint8_t* p, float (&d)[NB]) {
 }
 
 template <int HD, bool KQ, bool VQ, bool SPLIT, int WM>
-__global__ void __launch_bounds__(kRowsThreads + 32)
+__global__ void __launch_bounds__(kRowsThreads + 32, rows_ctas<HD, KQ, VQ, SPLIT>())
     page_rows_kernel(const PageRowsArgs a, int stages, const __grid_constant__ CUtensorMap k_map,
                      const __grid_constant__ CUtensorMap v_map) {
   using L = RowsSmem<HD>;
   constexpr int WK = 4 / WM;                   // warps along the positions
   constexpr int KEYS = kRowsBk / WK;           // positions of a warp in a unit
   constexpr int NC = WM == 1 ? 16 : 32;        // positions per softmax step
-  constexpr int NT = NC / 8, KS = HD / 16, NB = HD / 32, DT = HD / 8;
+  constexpr int NT = NC / 8, KS = HD / 16, NB = HD / 32, OT = SPLIT ? HD / 16 : HD / 8;   // OT: tiles of the result
   constexpr int WROWS = SPLIT ? 8 : 16;        // rows of a warp's operand
   constexpr bool KD = KQ && WM == 1, VD = VQ && WM == 1;   // stored bytes straight into registers
   extern __shared__ __align__(1024) uint8_t smem_raw[];
@@ -453,13 +462,27 @@ __global__ void __launch_bounds__(kRowsThreads + 32)
       }
     }
 
-    float o[DT][4];
+    float o[OT][4];
 #pragma unroll
-    for (int d = 0; d < DT; ++d)
+    for (int d = 0; d < OT; ++d)
 #pragma unroll
       for (int e = 0; e < 4; ++e) o[d][e] = 0.f;
-    // dim of o[d][e] and o[d][e + 2]
-    auto dim_of = [&](int d, int e) { return VD ? (d >> 2) * 32 + 8 * j + 4 * e + (d & 3) : d * 8 + 2 * j + e; };
+    // the row (of the warp's) and the dim that o[d][e] belongs to
+    auto o_row = [&](int e) { return SPLIT ? 2 * j + (e & 1) : g + 8 * (e >> 1); };
+    auto o_dim = [&](int d, int e) {
+      if constexpr (SPLIT) return VD ? (d >> 1) * 32 + 4 * g + 2 * (d & 1) + (e >> 1) : d * 16 + g + 8 * (e >> 1);
+      return VD ? (d >> 2) * 32 + 8 * j + 4 * (e & 1) + (d & 3) : d * 8 + 2 * j + (e & 1);
+    };
+    // a value of rows g and g + 8 (x0, x1), for the row of o[.][e]
+    auto by_row = [&](float x0, float x1, float (&f)[4]) {
+      if constexpr (SPLIT) {
+        f[0] = f[2] = __shfl_sync(0xffffffffu, x0, 8 * j);
+        f[1] = f[3] = __shfl_sync(0xffffffffu, x0, 8 * j + 4);
+      } else {
+        f[0] = f[1] = x0;
+        f[2] = f[3] = x1;
+      }
+    };
     float m0 = -INFINITY, m1 = -INFINITY, l0 = 0.f, l1 = 0.f;   // rows g and g + 8 (SPLIT: row g)
     // positions every live row sees need no mask
     const int p_min = at.first + w.G.div(row0), p_max = at.first + w.G.div(row0 + rows - 1);
@@ -524,44 +547,63 @@ __global__ void __launch_bounds__(kRowsThreads + 32)
 #pragma unroll
         for (int n = 0; n < NT; ++n) {
           float acc[4] = {0.f, 0.f, 0.f, 0.f};
-          const uint8_t* kr = Kt + (kw + n * 8 + g) * c.rb_k;   // KD: the row of operand column g
-          float da[NB], db[NB];                                 // KD: scales of positions 2j, 2j + 1
           if constexpr (KD) {
+            // the row of operand column g; scales of positions 2j, 2j + 1
+            const uint8_t* kr = Kt + (kw + n * 8 + g) * c.rb_k;
             const uint8_t* sr = Kt + (kw + n * 8 + 2 * j) * c.rb_k + (c.type_k == B2_Q8_0 ? HD : HD / 2);
-            row_scales<NB>(sr, da);
-            row_scales<NB>(sr + c.rb_k, db);
-          }
+            uint32_t x[NB][2];
+            if (c.type_k == B2_Q8_0) {
 #pragma unroll
-          for (int b = 0; b < NB; ++b) {
-            uint32_t kf[4];   // 8 positions x 32 dims
-            if constexpr (KD) {
-              if (c.type_k == B2_Q8_0) {
-                s8x4_to_h2(*reinterpret_cast<const uint32_t*>(kr + b * 32 + 4 * j), kf[0], kf[1]);
-                s8x4_to_h2(*reinterpret_cast<const uint32_t*>(kr + b * 32 + 16 + 4 * j), kf[2], kf[3]);
-              } else {
-                const uint32_t x = *reinterpret_cast<const uint32_t*>(kr + b * 16 + 4 * j);
-                n4x4_to_h2(x & 0x0F0F0F0Fu, kf[0], kf[1]);
-                n4x4_to_h2((x >> 4) & 0x0F0F0F0Fu, kf[2], kf[3]);
+              for (int b = 0; b < NB; ++b) {
+                x[b][0] = *reinterpret_cast<const uint32_t*>(kr + b * 32 + 4 * j);
+                x[b][1] = *reinterpret_cast<const uint32_t*>(kr + b * 32 + 16 + 4 * j);
               }
             } else {
-              ldsm4(ks_base + L::at(kw + n * 8 + (lane & 7), b * 4 + (lane >> 3)), kf);
+#pragma unroll
+              for (int b = 0; b < NB; ++b) {
+                const uint32_t v = *reinterpret_cast<const uint32_t*>(kr + b * 16 + 4 * j);
+                x[b][0] = (uint32_t)nib_lo_s8(v);
+                x[b][1] = (uint32_t)nib_hi_s8(v);
+              }
             }
-            if constexpr (KQ) {
-              float t[4] = {0.f, 0.f, 0.f, 0.f};
-              mma16816(t, qf[2 * b], kf[0], kf[1]);
-              mma16816(t, qf[2 * b + 1], kf[2], kf[3]);
-              float2 d;
-              if constexpr (KD)
-                d = make_float2(da[b], db[b]);
-              else
-                d = *reinterpret_cast<const float2*>(scale_k + b * kRowsBk + kw + n * 8 + 2 * j);
-              acc[0] = fmaf(t[0], d.x, acc[0]);
-              acc[1] = fmaf(t[1], d.y, acc[1]);
-              acc[2] = fmaf(t[2], d.x, acc[2]);
-              acc[3] = fmaf(t[3], d.y, acc[3]);
-            } else {
-              mma16816(acc, qf[2 * b], kf[0], kf[1]);
-              mma16816(acc, qf[2 * b + 1], kf[2], kf[3]);
+            float da[NB], db[NB];
+            row_scales<NB>(sr, da);
+            row_scales<NB>(sr + c.rb_k, db);
+            float t[NB][4];
+#pragma unroll
+            for (int b = 0; b < NB; ++b) {
+              uint32_t kf[4];
+              s8x4_to_h2(x[b][0], kf[0], kf[1]);
+              s8x4_to_h2(x[b][1], kf[2], kf[3]);
+              t[b][0] = t[b][1] = t[b][2] = t[b][3] = 0.f;
+              mma16816(t[b], qf[2 * b], kf[0], kf[1]);
+              mma16816(t[b], qf[2 * b + 1], kf[2], kf[3]);
+            }
+#pragma unroll
+            for (int b = 0; b < NB; ++b) {
+              acc[0] = fmaf(t[b][0], da[b], acc[0]);
+              acc[1] = fmaf(t[b][1], db[b], acc[1]);
+              acc[2] = fmaf(t[b][2], da[b], acc[2]);
+              acc[3] = fmaf(t[b][3], db[b], acc[3]);
+            }
+          } else {
+#pragma unroll
+            for (int b = 0; b < NB; ++b) {
+              uint32_t kf[4];   // 8 positions x 32 dims
+              ldsm4(ks_base + L::at(kw + n * 8 + (lane & 7), b * 4 + (lane >> 3)), kf);
+              if constexpr (KQ) {
+                float t[4] = {0.f, 0.f, 0.f, 0.f};
+                mma16816(t, qf[2 * b], kf[0], kf[1]);
+                mma16816(t, qf[2 * b + 1], kf[2], kf[3]);
+                const float2 d = *reinterpret_cast<const float2*>(scale_k + b * kRowsBk + kw + n * 8 + 2 * j);
+                acc[0] = fmaf(t[0], d.x, acc[0]);
+                acc[1] = fmaf(t[1], d.y, acc[1]);
+                acc[2] = fmaf(t[2], d.x, acc[2]);
+                acc[3] = fmaf(t[3], d.y, acc[3]);
+              } else {
+                mma16816(acc, qf[2 * b], kf[0], kf[1]);
+                mma16816(acc, qf[2 * b + 1], kf[2], kf[3]);
+              }
             }
           }
           if constexpr (SPLIT) {
@@ -581,6 +623,37 @@ __global__ void __launch_bounds__(kRowsThreads + 32)
             }
           }
         }
+        // VD: this step's words of V, on their way while the weights are formed
+        uint32_t vw[VD ? NB : 1][4];
+        float sc[VD ? 4 : 1][NB];   // scales of positions 2j, 2j+1, 2j+8, 2j+9
+        if constexpr (VD) {
+          const uint8_t* vr = Vt + (kw + 2 * j) * c.rb_v;
+          const bool q8 = c.type_v == B2_Q8_0;
+#pragma unroll
+          for (int b = 0; b < NB; ++b) {
+            const uint8_t* q = vr + (q8 ? b * 32 + 4 * g : b * 16 + 4 * (g & 3));
+            vw[b][0] = *reinterpret_cast<const uint32_t*>(q);
+            vw[b][1] = *reinterpret_cast<const uint32_t*>(q + c.rb_v);
+            vw[b][2] = *reinterpret_cast<const uint32_t*>(q + 8 * c.rb_v);
+            vw[b][3] = *reinterpret_cast<const uint32_t*>(q + 9 * c.rb_v);
+          }
+          const uint8_t* sr = vr + (q8 ? HD : HD / 2);
+          row_scales<NB>(sr, sc[0]);
+          row_scales<NB>(sr + c.rb_v, sc[1]);
+          row_scales<NB>(sr + 8 * c.rb_v, sc[2]);
+          row_scales<NB>(sr + 9 * c.rb_v, sc[3]);
+          if (edge) {
+#pragma unroll
+            for (int r = 0; r < 4; ++r) {
+              const int key = kw + 2 * j + (r & 1) + (r >> 1) * 8;
+#pragma unroll
+              for (int b = 0; b < NB; ++b) {
+                if (key < v_lo || key >= v_hi) sc[r][b] = 0.f;
+                if (guard && !(fabsf(sc[r][b]) <= 65504.f)) sc[r][b] = 0.f, found = 1;
+              }
+            }
+          }
+        }
         // ---- running maximum and sum ----
         float n0 = m0, n1 = m1;
 #pragma unroll
@@ -595,17 +668,16 @@ __global__ void __launch_bounds__(kRowsThreads + 32)
         }
         // a row that has seen nothing keeps m = -inf; its exponents are taken from 0
         const float r0 = (n0 == -INFINITY ? 0.f : n0) - off, r1 = (n1 == -INFINITY ? 0.f : n1) - off;
-        if (n0 != m0 || (!SPLIT && n1 != m1)) {
+        if (__any_sync(0xffffffffu, n0 != m0 || (!SPLIT && n1 != m1))) {
           const float f0 = m0 == -INFINITY ? 0.f : ex2(m0 - n0), f1 = m1 == -INFINITY ? 0.f : ex2(m1 - n1);
           l0 *= f0;
           l1 *= f1;
+          float f[4];
+          by_row(f0, f1, f);
 #pragma unroll
-          for (int d = 0; d < DT; ++d) {
-            o[d][0] *= f0;
-            o[d][1] *= f0;
-            o[d][2] *= SPLIT ? f0 : f1;
-            o[d][3] *= SPLIT ? f0 : f1;
-          }
+          for (int d = 0; d < OT; ++d)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) o[d][e] *= f[e];
           m0 = n0;
           m1 = n1;
         }
@@ -626,6 +698,7 @@ __global__ void __launch_bounds__(kRowsThreads + 32)
           uint32_t pf[4];
           const float* x = s[2 * k];
           const float* y = s[2 * k + 1];
+          // FULL: rows g and g + 8; SPLIT: high parts pf[0], pf[2], the others' pf[1], pf[3]
           auto operand = [&](float a0, float a1, float b0, float b1) {   // scales of positions 2j, 2j+1, 2j+8, 2j+9
             if constexpr (SPLIT) {
               h2_split(x[0] * a0, x[1] * a1, pf[0], pf[1]);
@@ -638,47 +711,30 @@ __global__ void __launch_bounds__(kRowsThreads + 32)
             }
           };
           if constexpr (!VQ) operand(1.f, 1.f, 1.f, 1.f);
-          const uint8_t* vr = Vt + (kw + k * 16 + 2 * j) * c.rb_v;   // VD: the row of position 2j
-          float sc[4][NB];                                           // VD: scales of positions 2j, 2j+1, 2j+8, 2j+9
-          if constexpr (VD) {
-            const uint8_t* sr = vr + (c.type_v == B2_Q8_0 ? HD : HD / 2);
-            row_scales<NB>(sr, sc[0]);
-            row_scales<NB>(sr + c.rb_v, sc[1]);
-            row_scales<NB>(sr + 8 * c.rb_v, sc[2]);
-            row_scales<NB>(sr + 9 * c.rb_v, sc[3]);
-            if (edge) {
-#pragma unroll
-              for (int r = 0; r < 4; ++r) {
-                const int key = kw + k * 16 + 2 * j + (r & 1) + (r >> 1) * 8;
-#pragma unroll
-                for (int b = 0; b < NB; ++b) {
-                  if (key < v_lo || key >= v_hi) sc[r][b] = 0.f;
-                  if (guard && !(fabsf(sc[r][b]) <= 65504.f)) sc[r][b] = 0.f, found = 1;
-                }
-              }
-            }
-          }
 #pragma unroll
           for (int b = 0; b < NB; ++b) {
             if constexpr (VD) {
               operand(sc[0][b], sc[1][b], sc[2][b], sc[3][b]);
               uint32_t v0[4], v1[4];   // positions 2j, 2j+1 and 2j+8, 2j+9 of dims 4g + t of the block
               if (c.type_v == B2_Q8_0) {
-                const uint8_t* q = vr + b * 32 + 4 * g;
-                pair_to_h2(*reinterpret_cast<const uint32_t*>(q) ^ 0x80808080u,
-                           *reinterpret_cast<const uint32_t*>(q + c.rb_v) ^ 0x80808080u, 0x64806480u, v0);
-                pair_to_h2(*reinterpret_cast<const uint32_t*>(q + 8 * c.rb_v) ^ 0x80808080u,
-                           *reinterpret_cast<const uint32_t*>(q + 9 * c.rb_v) ^ 0x80808080u, 0x64806480u, v1);
+                pair_to_h2(vw[b][0] ^ 0x80808080u, vw[b][1] ^ 0x80808080u, 0x64806480u, v0);
+                pair_to_h2(vw[b][2] ^ 0x80808080u, vw[b][3] ^ 0x80808080u, 0x64806480u, v1);
               } else {
-                const uint8_t* q = vr + b * 16 + 4 * (g & 3);
                 const int sf = g & 4;   // values 16..31 are the high nibbles
-                pair_to_h2((*reinterpret_cast<const uint32_t*>(q) >> sf) & 0x0F0F0F0Fu,
-                           (*reinterpret_cast<const uint32_t*>(q + c.rb_v) >> sf) & 0x0F0F0F0Fu, 0x64086408u, v0);
-                pair_to_h2((*reinterpret_cast<const uint32_t*>(q + 8 * c.rb_v) >> sf) & 0x0F0F0F0Fu,
-                           (*reinterpret_cast<const uint32_t*>(q + 9 * c.rb_v) >> sf) & 0x0F0F0F0Fu, 0x64086408u, v1);
+                pair_to_h2((vw[b][0] >> sf) & 0x0F0F0F0Fu, (vw[b][1] >> sf) & 0x0F0F0F0Fu, 0x64086408u, v0);
+                pair_to_h2((vw[b][2] >> sf) & 0x0F0F0F0Fu, (vw[b][3] >> sf) & 0x0F0F0F0Fu, 0x64086408u, v1);
               }
+              if constexpr (SPLIT) {
 #pragma unroll
-              for (int t = 0; t < 4; ++t) mma16816(o[b * 4 + t], pf, v0[t], v1[t]);
+                for (int t = 0; t < 2; ++t) {
+                  const uint32_t av[4] = {v0[2 * t], v0[2 * t + 1], v1[2 * t], v1[2 * t + 1]};
+                  mma16816(o[b * 2 + t], av, pf[0], pf[2]);
+                  mma16816(o[b * 2 + t], av, pf[1], pf[3]);
+                }
+              } else {
+#pragma unroll
+                for (int t = 0; t < 4; ++t) mma16816(o[b * 4 + t], pf, v0[t], v1[t]);
+              }
             } else {
               if constexpr (VQ) {
                 const float* q = scale_v + b * kRowsBk + kw + k * 16 + 2 * j;
@@ -688,9 +744,15 @@ __global__ void __launch_bounds__(kRowsThreads + 32)
 #pragma unroll
               for (int d = 0; d < 2; ++d) {
                 uint32_t vf[4];   // 16 positions x 16 dims
-                ldsm4_t(vs_base + L::at(kw + k * 16 + (lane & 15), b * 4 + 2 * d + (lane >> 4)), vf);
-                mma16816(o[b * 4 + 2 * d], pf, vf[0], vf[1]);
-                mma16816(o[b * 4 + 2 * d + 1], pf, vf[2], vf[3]);
+                if constexpr (SPLIT) {
+                  ldsm4_t(vs_base + L::at(kw + k * 16 + (lane & 7) + (lane >> 4) * 8, b * 4 + 2 * d + ((lane >> 3) & 1)), vf);
+                  mma16816(o[b * 2 + d], vf, pf[0], pf[2]);
+                  mma16816(o[b * 2 + d], vf, pf[1], pf[3]);
+                } else {
+                  ldsm4_t(vs_base + L::at(kw + k * 16 + (lane & 15), b * 4 + 2 * d + (lane >> 4)), vf);
+                  mma16816(o[b * 4 + 2 * d], pf, vf[0], vf[1]);
+                  mma16816(o[b * 4 + 2 * d + 1], pf, vf[2], vf[3]);
+                }
               }
             }
           }
@@ -702,19 +764,19 @@ __global__ void __launch_bounds__(kRowsThreads + 32)
       if (bad) {
         // infinite and NaN values of V, to the rows that see them (their
         // weight is positive, so the value itself decides the sum)
+        float pos[4];
+        by_row(__int_as_float(p0), __int_as_float(p1), pos);
         for (int key = wk * KEYS; key < (wk + 1) * KEYS; ++key) {
           const int t = key0 + key;
           if (t < at.lo || t >= at.hi) continue;
           const int64_t row = page_row(w.b, c, at.s, at.h, t);
           if (row < 0) continue;
           const uint8_t* vr = c.v + row * c.rb_v;
-          const bool see0 = t <= p0 && !(w.window > 0 && t <= p0 - w.window);
-          const bool see1 = !SPLIT && t <= p1 && !(w.window > 0 && t <= p1 - w.window);
 #pragma unroll
-          for (int d = 0; d < DT; ++d)
+          for (int d = 0; d < OT; ++d)
 #pragma unroll
-            for (int e = 0; e < 2; ++e) {
-              const int i = dim_of(d, e);
+            for (int e = 0; e < 4; ++e) {
+              const int i = o_dim(d, e), p = __float_as_int(pos[e]);
               float v;
               if constexpr (VQ) {
                 const float sc = h2f(*reinterpret_cast<const uint16_t*>(
@@ -726,9 +788,7 @@ __global__ void __launch_bounds__(kRowsThreads + 32)
               } else {
                 v = h2f(reinterpret_cast<const uint16_t*>(vr)[i]);
               }
-              if (fabsf(v) <= 3.4e38f) continue;
-              if (see0) o[d][e] += v;
-              if (see1) o[d][2 + e] += v;
+              if (!(fabsf(v) <= 3.4e38f) && t <= p && !(w.window > 0 && t <= p - w.window)) o[d][e] += v;
             }
         }
       }
@@ -740,25 +800,17 @@ __global__ void __launch_bounds__(kRowsThreads + 32)
       l0 += __shfl_xor_sync(0xffffffffu, l0, x);
       if constexpr (!SPLIT) l1 += __shfl_xor_sync(0xffffffffu, l1, x);
     }
-    if constexpr (SPLIT) {
-#pragma unroll
-      for (int d = 0; d < DT; ++d) {
-        o[d][0] += o[d][2];
-        o[d][1] += o[d][3];
-      }
-    }
     const Split split = split_of(sh, blockIdx.x, u_hi);
     const bool whole = split.n == 0;
     float* part = a.slots + (int64_t)split.slot * slot_floats(w.rows(), HD);
     float* part_ml = part + w.rows() * HD;
-    auto put2 = [&](int r, int d, float x, float y) {   // values d, d + 1 of row r, normalized, or a partial result
-      if (!whole) {
-        *reinterpret_cast<float2*>(part + r * HD + d) = make_float2(x, y);
-      } else if (a.q_f32) {
-        *reinterpret_cast<float2*>(static_cast<float*>(a.out) + place(r) + d) = make_float2(x, y);
-      } else {
-        *reinterpret_cast<uint32_t*>(static_cast<__half*>(a.out) + place(r) + d) = h2(x, y);
-      }
+    auto put = [&](int r, int d, float x) {   // value d of row r, normalized, or a partial result
+      if (!whole)
+        part[r * HD + d] = x;
+      else if (a.q_f32)
+        static_cast<float*>(a.out)[place(r) + d] = x;
+      else
+        static_cast<__half*>(a.out)[place(r) + d] = __float2half_rn(x);
     };
 
     if constexpr (WM == 1) {
@@ -773,39 +825,34 @@ __global__ void __launch_bounds__(kRowsThreads + 32)
       auto top = [&](int r) {
         return fmaxf(fmaxf(ml[r].x, ml[16 + r].x), fmaxf(ml[32 + r].x, ml[48 + r].x));
       };
-      const float t0 = top(g), f0 = m0 == -INFINITY ? 0.f : ex2(m0 - t0);
-      float f1 = 0.f;
-      if constexpr (!SPLIT) f1 = m1 == -INFINITY ? 0.f : ex2(m1 - top(g + 8));
       // a warp that saw nothing of a row contributes nothing, not 0·NaN
+      float f[4];
 #pragma unroll
-      for (int d = 0; d < DT; ++d)
+      for (int e = 0; e < 4; ++e) {
+        const float2 x = ml[warp * 16 + o_row(e)];
+        f[e] = x.y == 0.f ? 0.f : x.x == -INFINITY ? 1.f : ex2(x.x - top(o_row(e)));
+      }
 #pragma unroll
-        for (int e = 0; e < 2; ++e) {
-          const int i = dim_of(d, e);
-          so[(warp * WROWS + g) * HD + i] = l0 != 0.f ? o[d][e] * f0 : 0.f;
-          if constexpr (!SPLIT) so[(warp * WROWS + g + 8) * HD + i] = l1 != 0.f ? o[d][2 + e] * f1 : 0.f;
-        }
+      for (int d = 0; d < OT; ++d)
+#pragma unroll
+        for (int e = 0; e < 4; ++e)
+          so[(warp * WROWS + o_row(e)) * HD + o_dim(d, e)] = f[e] != 0.f ? o[d][e] * f[e] : 0.f;
       bar_compute();
-      for (int i = tid; i < rows * (HD / 2); i += kRowsThreads) {
-        const int r = i / (HD / 2), d = 2 * (i - r * (HD / 2));
+      for (int i = tid; i < rows * HD; i += kRowsThreads) {
+        const int r = i / HD, d = i - r * HD;
         const float t = top(r);
-        float x = 0.f, y = 0.f, l = 0.f;
+        float x = 0.f, l = 0.f;
 #pragma unroll
         for (int q = 0; q < 4; ++q) {
-          const float2 v = *reinterpret_cast<const float2*>(so + (q * WROWS + r) * HD + d);
           const float2 e = ml[q * 16 + r];
-          x += v.x;
-          y += v.y;
+          x += so[(q * WROWS + r) * HD + d];
           l += e.x == -INFINITY ? e.y : e.y * ex2(e.x - t);
         }
-        if (whole) {
-          const float inv = l != 0.f ? 1.f / l : 0.f;
-          x *= inv;
-          y *= inv;
-        } else if (d == 0) {
+        if (whole)
+          x *= l != 0.f ? 1.f / l : 0.f;
+        else if (d == 0)
           *reinterpret_cast<float2*>(part_ml + 2 * r) = make_float2(t, l);
-        }
-        put2(r, d, x, y);
+        put(r, d, x);
       }
       if (!whole) {
         // all warps' shares of the rows are written before one counts the part
@@ -826,15 +873,15 @@ __global__ void __launch_bounds__(kRowsThreads + 32)
       }
       bar_compute();   // the join's space is free for the next tile
     } else {
-      const float i0 = !whole ? 1.f : l0 != 0.f ? 1.f / l0 : 0.f, i1 = !whole ? 1.f : l1 != 0.f ? 1.f / l1 : 0.f;
       const int r = wm * WROWS + g;
+      float f[4];
+      by_row(!whole ? 1.f : l0 != 0.f ? 1.f / l0 : 0.f, !whole ? 1.f : l1 != 0.f ? 1.f / l1 : 0.f, f);
 #pragma unroll
-      for (int d = 0; d < DT; ++d) {
-        const int i = d * 8 + 2 * j;
-        if (r < rows) put2(r, i, o[d][0] * i0, o[d][1] * i0);
-        if constexpr (!SPLIT)
-          if (r + 8 < rows) put2(r + 8, i, o[d][2] * i1, o[d][3] * i1);
-      }
+      for (int e = 0; e < 4; ++e)
+        if (wm * WROWS + o_row(e) < rows) {
+#pragma unroll
+          for (int d = 0; d < OT; ++d) put(wm * WROWS + o_row(e), o_dim(d, e), o[d][e] * f[e]);
+        }
       if (!whole && wm * WROWS < rows) {
         if (j == 0) {
           if (r < rows) *reinterpret_cast<float2*>(part_ml + 2 * r) = make_float2(m0, l0);
@@ -876,11 +923,8 @@ inline int rows_smem_bytes(const PageRowsArgs& a, int stages) {
 
 template <int HD, bool KQ, bool VQ, bool SPLIT, int WM>
 int launch_page_rows_one(PageRowsArgs a, cudaStream_t s) {
-  // The deepest ring that leaves two CTAs on an SM where it can (head_dim 256
-  // with fp16 rows: one).
-  const int stage = rows_stage_bytes<HD, KQ, VQ>(a.c.rb_k, a.c.rb_v);
   int stages = kRowsStagesMax;
-  while (stages > 2 && rows_smem_bytes<HD, KQ, VQ, SPLIT, WM>(a, stages) > (stage > 40 * 1024 ? 226 : 112) * 1024) --stages;
+  while (stages > 2 && rows_smem_bytes<HD, KQ, VQ, SPLIT, WM>(a, stages) > (227 / rows_ctas<HD, KQ, VQ, SPLIT>() - 1) * 1024) --stages;
   const int smem = rows_smem_bytes<HD, KQ, VQ, SPLIT, WM>(a, stages);
   auto kern = page_rows_kernel<HD, KQ, VQ, SPLIT, WM>;
   // looked up once per device and cache type pair
