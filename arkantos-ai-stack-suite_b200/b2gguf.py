@@ -216,7 +216,7 @@ class DeviceBuffer:
     def __init__(self, nbytes: int):
         p = ctypes.c_void_p()
         check(lib.b2_malloc(ctypes.byref(p), max(1, int(nbytes))), "b2_malloc")
-        self.ptr = p.value
+        self.ptr = self._as_parameter_ = p.value   # a DeviceBuffer is a pointer argument as it is
         self.nbytes = int(nbytes)
 
     @classmethod
@@ -247,7 +247,7 @@ class DeviceBuffer:
     def free(self) -> None:
         if getattr(self, "ptr", None):
             lib.b2_free(self.ptr)
-            self.ptr = None
+            self.ptr = self._as_parameter_ = None
 
     def __del__(self):
         try:
@@ -467,7 +467,7 @@ class PageCache:
     def __init__(self, n_layer: int, n_pages: int, page_size: int, n_kv: int, head_dim: int, type_k: int = F16,
                  type_v: int = F16, k=None, v=None):
         self.c = _PageCacheC(None, None, n_layer, n_pages, page_size, n_kv, head_dim, type_k, type_v)
-        self.ref = ctypes.byref(self.c)
+        self.ref = ctypes.addressof(self.c)
         bk, bv = ctypes.c_size_t(), ctypes.c_size_t()
         check(lib.b2_page_cache_bytes(self.ref, ctypes.byref(bk), ctypes.byref(bv)), "page_cache_bytes")
         self.bytes_k, self.bytes_v = bk.value, bv.value
@@ -491,7 +491,7 @@ class PageBatch:
                                       for a in (q_start, kv_len, table))
         self.q_start, self.kv_len, self.table = q_start, kv_len, table
         self.c = _PageBatchC(_addr(q_start), _addr(kv_len), _addr(table), n_seq, max_pages, n_tok, max_q)
-        self.ref = ctypes.byref(self.c)
+        self.ref = ctypes.addressof(self.c)
 
 
 def rope_sections(sections, interleave: bool = False) -> np.ndarray:
@@ -502,12 +502,19 @@ def rope_sections(sections, interleave: bool = False) -> np.ndarray:
     return out
 
 
+# The per-step calls.  Device arrays are DeviceBuffers or addresses; a decode
+# step makes these calls once per layer, so they hand their arguments on as
+# they are (the library checks them).
+_page_rope_store, _page_attn = lib.b2_page_rope_store, lib.b2_page_attn
+_page_copy, _page_gather = lib.b2_page_copy, lib.b2_page_gather
+
+
 def page_rope_store(cache: PageCache, layer: int, batch: PageBatch, n_head: int, qkv, type_x: int, q_out, type_q: int,
                     pos, n_axes: int, axis, rope, n_pos: int, n_rot: int, style: int = ROPE_ADJACENT,
                     stream: int | None = None) -> None:
     """Rotary positions (one or several axes) on q and k, q to q_out, k and v to their pages."""
-    rc = lib.b2_page_rope_store(cache.ref, layer, batch.ref, n_head, _addr(qkv), type_x, _addr(q_out), type_q,
-                                _addr(pos), n_axes, _addr(axis), _addr(rope), n_pos, n_rot, style, stream)
+    rc = _page_rope_store(cache.ref, layer, batch.ref, n_head, qkv, type_x, q_out, type_q, pos, n_axes, axis, rope,
+                          n_pos, n_rot, style, stream)
     if rc:
         check(rc, "page_rope_store")
 
@@ -519,24 +526,38 @@ def page_attn_workspace_bytes(cache: PageCache, batch: PageBatch, n_head: int, t
     return v.value
 
 
+def page_attn_workspace(cache: PageCache, batch: PageBatch, n_head: int, type_q: int) -> DeviceBuffer:
+    """A workspace for calls of this batch's shapes and smaller ones, set to zero as its first use needs."""
+    w = DeviceBuffer(page_attn_workspace_bytes(cache, batch, n_head, type_q))
+    w.zero()
+    return w
+
+
 def page_attn(cache: PageCache, layer: int, batch: PageBatch, n_head: int, q, out, type_q: int,
               scale: float | None = None, window: int = 0, workspace: DeviceBuffer | None = None,
               status: DeviceBuffer | None = None, stream: int | None = None) -> None:
     """Attention of each sequence's new tokens over its pages; scale defaults to 1/sqrt(head_dim)."""
     if scale is None:
         scale = cache.c.head_dim ** -0.5
-    rc = lib.b2_page_attn(cache.ref, layer, batch.ref, n_head, _addr(q), _addr(out), type_q, scale, window,
-                          workspace.ptr if workspace else None, workspace.nbytes if workspace else 0,
-                          status.ptr if status else None, stream)
+    rc = _page_attn(cache.ref, layer, batch.ref, n_head, q, out, type_q, scale, window, workspace,
+                    workspace.nbytes if workspace is not None else 0, status, stream)
     if rc:
         check(rc, "page_attn")
 
 
+def _host_int32(a):
+    """An int32 array and its address."""
+    a = np.ascontiguousarray(a, np.int32)
+    return a, a.__array_interface__["data"][0]
+
+
 def page_copy(cache: PageCache, src, dst, stream: int | None = None) -> None:
     """Pages src[i] -> dst[i] (host lists) in every layer."""
-    src, dst = np.ascontiguousarray(src, np.int32), np.ascontiguousarray(dst, np.int32)
-    assert src.size == dst.size
-    rc = lib.b2_page_copy(cache.ref, src.ctypes.data, dst.ctypes.data, src.size, stream)
+    src, ps = _host_int32(src)
+    dst, pd = _host_int32(dst)
+    if src.size != dst.size:
+        raise ValueError("page_copy: src and dst differ in length")
+    rc = _page_copy(cache.ref, ps, pd, src.size, stream)
     if rc:
         check(rc, "page_copy")
 
@@ -544,8 +565,7 @@ def page_copy(cache: PageCache, src, dst, stream: int | None = None) -> None:
 def page_gather(cache: PageCache, n_seq: int, keep_start, keep, n_keep: int, old_table, new_table, max_pages: int,
                 stream: int | None = None) -> None:
     """Kept positions of the old tables' pages gathered into the new tables' pages, in every layer."""
-    rc = lib.b2_page_gather(cache.ref, n_seq, _addr(keep_start), _addr(keep), n_keep, _addr(old_table),
-                            _addr(new_table), max_pages, stream)
+    rc = _page_gather(cache.ref, n_seq, keep_start, keep, n_keep, old_table, new_table, max_pages, stream)
     if rc:
         check(rc, "page_gather")
 

@@ -4,7 +4,15 @@
 namespace b2 {
 namespace {
 
-// Which kernel takes a call, by the most rows a sequence has per kv head.
+// Which kernel takes a call, by the most rows a sequence has per kv head (new
+// tokens times the query heads that share it).  Up to kFewRows: the few-row
+// kernel with its warps along the positions.  More: the tensor-core kernel
+// where it reads the cache, else the few-row kernel with its warps along the
+// rows.  One kernel takes all sequences of a call: running both, each on the
+// sequences of its kind, was slower (a step of 12 single tokens and 4 chunks
+// of 129 over 300-2049 positions: 81 us against 47 with fp16 queries, 84
+// against 64 with fp32), since the second begins when the first has ended.
+constexpr int kFewRows = 16;
 struct Plan {
   bool tc, split;
   int wm, rows, bk, max_ctas;
@@ -13,7 +21,7 @@ Plan plan_of(const PageAttnArgs& a) {
   const int64_t rows = (int64_t)a.b.max_q * (a.n_head / a.c.n_kv);
   const bool f32 = a.type_q == B2_F32;
   Plan p;
-  p.tc = rows > 32 && page_tc_ok(a.c, a.hd);
+  p.tc = rows > kFewRows && page_tc_ok(a.c, a.hd);
   p.split = f32 || (!p.tc && rows <= 8);
   if (p.tc) {
     p.wm = 0;
@@ -21,7 +29,7 @@ Plan plan_of(const PageAttnArgs& a) {
     p.bk = kTcBk;
     p.max_ctas = sm_count();
   } else {
-    p.wm = rows <= (p.split ? 8 : 16) ? 1 : 4;
+    p.wm = rows <= kFewRows ? 1 : 4;
     p.rows = (p.split ? 8 : 16) * p.wm;
     p.bk = kRowsBk;
     p.max_ctas = kPageMaxCtasPerSm * sm_count();

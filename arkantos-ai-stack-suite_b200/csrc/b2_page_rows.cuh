@@ -955,11 +955,15 @@ int launch_page_rows_one(PageRowsArgs a, cudaStream_t s) {
 template <int HD>
 int launch_page_rows_hd(const PageRowsArgs& a, bool split, int wm, cudaStream_t s) {
   const bool kq = a.c.type_k != B2_F16, vq = a.c.type_v != B2_F16;
+  // many rows over fp16 pages of these head sizes go to the tensor-core kernel
+  constexpr bool kTc = HD == 64 || HD == 128;
 #define B2_ROWS(KQ, VQ)                                                                             \
   if (kq == KQ && vq == VQ) {                                                                       \
-    if (split) return wm == 1 ? launch_page_rows_one<HD, KQ, VQ, true, 1>(a, s)                     \
-                              : launch_page_rows_one<HD, KQ, VQ, true, 4>(a, s);                    \
-    return wm == 1 ? launch_page_rows_one<HD, KQ, VQ, false, 1>(a, s)                               \
+    if (wm == 1)                                                                                    \
+      return split ? launch_page_rows_one<HD, KQ, VQ, true, 1>(a, s)                                \
+                   : launch_page_rows_one<HD, KQ, VQ, false, 1>(a, s);                              \
+    if constexpr (KQ || VQ || !kTc)                                                                 \
+      return split ? launch_page_rows_one<HD, KQ, VQ, true, 4>(a, s)                                \
                    : launch_page_rows_one<HD, KQ, VQ, false, 4>(a, s);                              \
   }
   B2_ROWS(false, false)

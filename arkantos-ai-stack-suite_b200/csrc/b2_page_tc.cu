@@ -29,17 +29,18 @@ int encode_map(CUtensorMap* map, const void* base, int rank, const cuuint64_t* d
   return B2_OK;
 }
 
-// Queries [n_tok][n_head][hd], copied as the 128 rows (token, head of the
-// group) of half a tile x 64 dims.
-int query_map(const void* q, int hd, int n_head, int n_tok, int G, CUtensorMap* map) {
+// Queries or results [n_tok][n_head][hd], copied as `rows` rows (token, head of
+// the group) x 64 dims.
+int rows_map(const void* q, int hd, int n_head, int n_tok, int G, int rows, CUtensorMap* map) {
   const cuuint64_t dims[3] = {(cuuint64_t)hd, (cuuint64_t)n_head, (cuuint64_t)n_tok};
   const cuuint64_t strides[2] = {(cuuint64_t)hd * 2, (cuuint64_t)n_head * hd * 2};
-  const cuuint32_t box[3] = {64, (cuuint32_t)G, (cuuint32_t)(128 / G)};
+  const cuuint32_t box[3] = {64, (cuuint32_t)G, (cuuint32_t)(rows / G)};
   return encode_map(map, q, 3, dims, strides, box);
 }
 
 template <int HD, bool SPLIT>
-int launch(const PageTcArgs& a, const CUtensorMap& km, const CUtensorMap& vm, const CUtensorMap& qm, cudaStream_t s) {
+int launch(const PageTcArgs& a, const CUtensorMap& km, const CUtensorMap& vm, const CUtensorMap& qm,
+           const CUtensorMap& om, cudaStream_t s) {
   auto kern = page_tc_kernel<HD, SPLIT>;
   static std::atomic<int> ready[kMaxDevices];
   int dev = 0;
@@ -50,7 +51,7 @@ int launch(const PageTcArgs& a, const CUtensorMap& km, const CUtensorMap& vm, co
     ready[dev].store(1, std::memory_order_relaxed);
   }
   const int ctas = sm_count();   // one per SM: the kernel takes all of TMEM
-  return launch_pdl(kern, dim3(ctas), dim3(kTcThreads), (size_t)TcSmem<HD, SPLIT>::bytes, s, a, km, vm, qm);
+  return launch_pdl(kern, dim3(ctas), dim3(kTcThreads), (size_t)TcSmem<HD, SPLIT>::bytes, s, a, km, vm, qm, om);
 }
 
 }  // namespace
@@ -65,15 +66,17 @@ int launch_page_tc(PageTcArgs a, int hd, bool split, int page_size, cudaStream_t
   const int box = std::min(page_size, kTcBk);
   a.box_rows_log2 = 0;
   while ((1 << a.box_rows_log2) < box) ++a.box_rows_log2;
-  CUtensorMap km, vm, qm = {};
+  CUtensorMap km, vm, qm = {}, om = {};
   int rc = page_pool_map(a.c.k, hd, a.pool_rows, box, &km);
   if (rc == B2_OK) rc = page_pool_map(a.c.v, hd, a.pool_rows, box, &vm);
   const int G = (int)a.w.G.d;
   a.q_map = !split && 128 % G == 0;
-  if (rc == B2_OK && a.q_map) rc = query_map(a.q, hd, a.n_head, a.w.b.n_tok, G, &qm);
+  a.o_map = !split && 32 % G == 0;
+  if (rc == B2_OK && a.q_map) rc = rows_map(a.q, hd, a.n_head, a.w.b.n_tok, G, 128, &qm);
+  if (rc == B2_OK && a.o_map) rc = rows_map(a.out, hd, a.n_head, a.w.b.n_tok, G, 32, &om);
   if (rc != B2_OK) return rc;
-  if (hd == 128) return split ? launch<128, true>(a, km, vm, qm, s) : launch<128, false>(a, km, vm, qm, s);
-  return split ? launch<64, true>(a, km, vm, qm, s) : launch<64, false>(a, km, vm, qm, s);
+  if (hd == 128) return split ? launch<128, true>(a, km, vm, qm, om, s) : launch<128, false>(a, km, vm, qm, om, s);
+  return split ? launch<64, true>(a, km, vm, qm, om, s) : launch<64, false>(a, km, vm, qm, om, s);
 }
 
 }  // namespace b2

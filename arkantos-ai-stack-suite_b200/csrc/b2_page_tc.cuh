@@ -72,6 +72,7 @@ struct PageTcArgs {
   float scale_log2;
   int box_rows_log2;      // rows of a tensor copy: min(page_size, 128)
   int q_map;              // FULL: Q comes by tensor copies (G divides 128)
+  int o_map;              // FULL: results leave by tensor copies (G divides 32)
   int64_t pool_rows;      // rows of the layer's pool
   unsigned* counters;
   float* slots;
@@ -229,6 +230,17 @@ __device__ __forceinline__ void tma_3d(uint32_t dst, const CUtensorMap* map, int
       "l"(reinterpret_cast<uint64_t>(map)), "r"(smem_u32(bar)), "r"(x), "r"(y), "r"(z)
       : "memory");
 }
+// Shared memory to a tensor, and the waits for a thread's stores: until their
+// shared memory has been read, until they are done.
+__device__ __forceinline__ void tma_store_3d(const CUtensorMap* map, int x, int y, int z, uint32_t src) {
+  asm volatile("cp.async.bulk.tensor.3d.global.shared::cta.bulk_group [%0, {%2, %3, %4}], [%1];\n\t"
+               "cp.async.bulk.commit_group;" ::"l"(reinterpret_cast<uint64_t>(map)),
+               "r"(src), "r"(x), "r"(y), "r"(z)
+               : "memory");
+}
+__device__ __forceinline__ void tma_store_read() { asm volatile("cp.async.bulk.wait_group.read 0;" ::: "memory"); }
+__device__ __forceinline__ void tma_store_done() { asm volatile("cp.async.bulk.wait_group 0;" ::: "memory"); }
+
 // A tile of the CTA's share as the warps see it.
 struct TcTile {
   int h, s, q0, first;            // kv head, sequence; its first new token's row and position
@@ -248,7 +260,8 @@ __device__ __forceinline__ bool tc_edge(const TcTile& t, int key0, int window) {
 template <int HD, bool SPLIT>
 __global__ void __launch_bounds__(kTcThreads, 1)
     page_tc_kernel(const PageTcArgs a, const __grid_constant__ CUtensorMap k_map,
-                   const __grid_constant__ CUtensorMap v_map, const __grid_constant__ CUtensorMap q_map) {
+                   const __grid_constant__ CUtensorMap v_map, const __grid_constant__ CUtensorMap q_map,
+                   const __grid_constant__ CUtensorMap o_map) {
   using L = TcSmem<HD, SPLIT>;
   constexpr int NS = L::stages, PARTS = SPLIT ? 2 : 1;
   extern __shared__ __align__(1024) uint8_t smem_raw[];
@@ -307,8 +320,11 @@ __global__ void __launch_bounds__(kTcThreads, 1)
                  : "memory");
     asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
   }
-  if (warp == 9 && lane < 3)
-    asm volatile("prefetch.tensormap [%0];" ::"l"(reinterpret_cast<uint64_t>(lane == 0 ? &k_map : lane == 1 ? &v_map : &q_map))
+  if (warp == 9 && lane < 4)
+    asm volatile("prefetch.tensormap [%0];" ::"l"(reinterpret_cast<uint64_t>(lane == 0   ? &k_map
+                                                                              : lane == 1 ? &v_map
+                                                                              : lane == 2 ? &q_map
+                                                                                          : &o_map))
                  : "memory");
   pdl_wait();
   const PageWork& w = a.w;
@@ -785,12 +801,38 @@ __global__ void __launch_bounds__(kTcThreads, 1)
       // moved so that neither side meets a bank conflict, then segments of rows.
       uint8_t* stage = SPLIT ? Qs + half * 2 * L::half_q + (warp & 3) * 4096 : Ts + NS * L::tile + warp * 4096;
       const bool wide = SPLIT || !whole;   // fp32 out
+      // Whole warps of rows of a whole tile leave as a tensor copy of 32/G
+      // tokens x G heads x 64 dims.
+      const int warp_row = (half * 4 + (warp & 3)) * 32;
+      const bool by_copy = !SPLIT && whole && a.o_map && warp_row + 32 <= t.rows;
+      if (by_copy) {
 #pragma unroll 1
-      for (int i = 0; i < HD / 32; ++i) {
+        for (int blk = 0; blk < HD / 64; ++blk) {
+          if (lane == 0) tma_store_read();   // the space is free again
+          __syncwarp();
+#pragma unroll
+          for (int i = 0; i < 2; ++i) {
+            float o[32];
+            tmem_ld32(to + blk * 64 + i * 32, o);
+#pragma unroll
+            for (int ch = 0; ch < 4; ++ch)
+              *reinterpret_cast<uint4*>(stage + lane * 128 + (((i * 4 + ch) ^ (lane & 7)) << 4)) =
+                  make_uint4(h2(o[8 * ch] * inv, o[8 * ch + 1] * inv), h2(o[8 * ch + 2] * inv, o[8 * ch + 3] * inv),
+                             h2(o[8 * ch + 4] * inv, o[8 * ch + 5] * inv), h2(o[8 * ch + 6] * inv, o[8 * ch + 7] * inv));
+          }
+          fence_async_proxy();
+          __syncwarp();
+          if (lane == 0)
+            tma_store_3d(&o_map, blk * 64, t.h * (int)w.G.d, t.q0 + token_of(warp_row), smem_u32(stage));
+        }
+      }
+#pragma unroll 1
+      for (int i = by_copy ? HD / 32 : 0; i < HD / 32; ++i) {
         float o[32];
         tmem_ld32(to + i * 32, o);
 #pragma unroll
         for (int e = 0; e < 32; ++e) o[e] *= inv;
+        if (!SPLIT && lane == 0) tma_store_read();   // an earlier tile's copy may still read the space
         __syncwarp();
         if (wide) {
 #pragma unroll
@@ -830,6 +872,7 @@ __global__ void __launch_bounds__(kTcThreads, 1)
       if (*reinterpret_cast<volatile int*>(bad_seen) > nt) {
         // infinite and NaN values that were taken out of V, to the rows that
         // see them: their weight is positive, so the value decides the sum
+        if (lane == 0) tma_store_done();
         __syncwarp();
         for (int u = 0; u < t.units && on; ++u) {
           const int key0 = t.key0 + u * kTcBk;
@@ -855,7 +898,6 @@ __global__ void __launch_bounds__(kTcThreads, 1)
           }
         }
       }
-      const int warp_row = (half * 4 + (warp & 3)) * 32;
       if (!whole && warp_row < t.rows) {
         if (part_arrives(a.counters + t.split.cta0 * 8 + half * 4 + (warp & 3), t.split.n)) {
           constexpr int R = 16;
@@ -868,6 +910,7 @@ __global__ void __launch_bounds__(kTcThreads, 1)
       tc_before();
       leave_tile();
     }
+    if (!SPLIT && lane == 0) tma_store_done();   // results are out before the CTA ends
   }
   tc_before();
   __syncthreads();

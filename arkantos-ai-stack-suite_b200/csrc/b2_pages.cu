@@ -6,7 +6,7 @@
 // All three move bytes and do next to no arithmetic: what bounds them is HBM at
 // large sizes and the latency of one launch at small ones.
 #include "b2_common.cuh"
-#include "b2_pages.hpp"
+#include "b2_page_work.cuh"
 
 namespace b2 {
 namespace {
@@ -20,13 +20,16 @@ namespace {
 // (j, j + rot/2) of a head whose halves are paired.  Values past `rot` and
 // the v heads pass unchanged.
 //
-// One CTA takes a share of one token's heads.  Its rot/2 (cos, sin) pairs are
-// the same for every head, so they are gathered through the axis map into
-// shared memory once.  A thread makes 4 consecutive values (a half-split pair
-// reads its partner's 4 through L1): 16-byte loads, 8- or 16-byte stores, and
-// the 8 threads of a 32-value block share its scale by shuffles when the
-// cache is quantized.
-constexpr int kStoreThreads = 256;
+// A CTA takes a few tokens (of a decode step: a share of one token's heads).
+// Where they go is looked up once, and their rot/2 (cos, sin) pairs, the same
+// for every head, are gathered through the axis map into shared memory.  A
+// thread makes 8 values, two runs of 4 half a head apart (or one run, see the
+// launch): 16-byte loads, 8- or 16-byte stores, and the 8 threads of a
+// 32-value block share its scale by shuffles when the cache is quantized.
+// With 4 values a thread and one token a CTA the instructions bound it: 118 us
+// for 14192 tokens of 48 heads of 128 whether they came as fp32 or fp16.
+// 4 tokens by 128 threads: 86 us (94 % of a plain copy's rate); 1 by 256: 99, 8 by 128: 95.
+constexpr int kStoreThreads = 128, kStoreTokens = 4;
 
 template <typename T>
 __device__ __forceinline__ float4 load4(const T* p) {
@@ -108,80 +111,106 @@ __device__ __forceinline__ void store_row4(uint8_t* row, int type, int hd, int i
   if (sub == 0) *reinterpret_cast<uint16_t*>(row + hd / 2 + 2 * (i >> 5)) = f2h_rn(d);
 }
 
-template <typename TX, typename TQ>
-__global__ void __launch_bounds__(kStoreThreads) page_rope_store_kernel(const RopeStoreArgs a) {
-  __shared__ float2 cs[128];   // rot <= 256
-  __shared__ int s_seq, s_bad;
+template <typename TX, typename TQ, bool PAIR>
+__global__ void __launch_bounds__(kStoreThreads)
+    page_rope_store_kernel(const RopeStoreArgs a, const int n_here, const FastDiv row_div, const FastDiv head_div) {
+  __shared__ __align__(16) float2 cs[kStoreTokens][128];   // rot <= 256
+  __shared__ int s_seq[kStoreTokens], s_bad[kStoreTokens];
+  __shared__ int64_t s_row[kStoreTokens];    // the position's row of kv head 0; -1: nothing stored, -2: not a token
   pdl_wait();
   pdl_launch_dependents();
-  const int tok = blockIdx.x, tid = threadIdx.x;
-  if (tid == 0) {
-    s_seq = -1;
-    s_bad = 0;
+  const int tok0 = blockIdx.x * n_here, n = min(n_here, a.b.n_tok - tok0), tid = threadIdx.x;
+  const int hd = a.hd, g4 = hd / 4, heads = a.n_head + 2 * a.c.n_kv, half = a.rot / 2, total = heads * g4;
+  if (tid < kStoreTokens) {
+    s_seq[tid] = -1;
+    s_bad[tid] = 0;
   }
   __syncthreads();
-  // the token's sequence: one parallel look at the boundaries
-  for (int s = tid; s < a.b.n_seq; s += kStoreThreads)
-    if (a.b.q_start[s] <= tok && tok < a.b.q_start[s + 1]) s_seq = s;
-  for (int j = tid; j < a.rot / 2; j += kStoreThreads) {
+  // the tokens' sequences: one parallel look at the boundaries
+  for (int s = tid; s < a.b.n_seq; s += kStoreThreads) {
+    const int lo = a.b.q_start[s] - tok0, hi = a.b.q_start[s + 1] - tok0;
+    for (int t = max(lo, 0); t < min(hi, n); ++t) s_seq[t] = s;
+  }
+  for (int i = tid; i < n * half; i += kStoreThreads) {
+    const int t = i / half, j = i - t * half;
     const int ax = a.axis ? a.axis[j] : 0;
-    const int p = ax < a.n_axes ? a.pos[(int64_t)ax * a.b.n_tok + tok] : -1;
+    const int p = ax < a.n_axes ? a.pos[(int64_t)ax * a.b.n_tok + tok0 + t] : -1;
     if (p >= 0 && p < a.n_pos)
-      cs[j] = reinterpret_cast<const float2*>(a.rope)[(int64_t)p * (a.rot / 2) + j];
+      cs[t][j] = reinterpret_cast<const float2*>(a.rope)[(int64_t)p * half + j];
     else
-      s_bad = 1;
+      s_bad[t] = 1;
   }
   __syncthreads();
-  const int seq = s_seq, hd = a.hd, g4 = hd / 4, heads = a.n_head + 2 * a.c.n_kv;
-  if (seq < 0) return;   // a row past the last sequence
-  const SeqSpan sp = seq_span(a.b, a.c.ps_log2, seq);
-  const int p = sp.first + (tok - sp.q0);
-  const bool ok = p >= 0 && !s_bad;               // otherwise: a zero q row, nothing stored
-  int64_t row0 = -1;                              // the position's row of kv head 0
-  if (ok) row0 = page_row(a.b, a.c, seq, 0, p);
-  const bool live = ok && row0 >= 0;
-  const TX* x = static_cast<const TX*>(a.x) + (int64_t)tok * heads * hd;
-  TQ* q = static_cast<TQ*>(a.q) + (int64_t)tok * a.n_head * hd;
-  const int half = a.rot / 2, total = heads * g4;
-  // hd is a multiple of 32, so the 8 threads of a block always run together
-  for (int g = blockIdx.y * kStoreThreads + tid; g < total; g += gridDim.y * kStoreThreads) {
-    const int head = g / g4, i = 4 * (g - head * g4);
-    const TX* xr = x + head * hd;
-    float4 y = load4(xr + i);
-    if (head < a.n_head + a.c.n_kv && i < a.rot) {
+  if (tid < n) {
+    int64_t row = -2;
+    if (s_seq[tid] >= 0) {
+      const SeqSpan sp = seq_span(a.b, a.c.ps_log2, s_seq[tid]);
+      const int p = sp.first + (tok0 + tid - sp.q0);
+      row = p >= 0 && !s_bad[tid] ? page_row(a.b, a.c, s_seq[tid], 0, p) : -1;
+    }
+    s_row[tid] = row;
+  }
+  __syncthreads();
+  // 4 values at i: both of a pair's sides here (style 0), rotated
+  auto turn_adjacent = [&](const float2* c, int i, float4 y) {
+    const float4 r = *reinterpret_cast<const float4*>(c + i / 2);
+    return make_float4(__fsub_rn(__fmul_rn(y.x, r.x), __fmul_rn(y.y, r.y)),
+                       __fadd_rn(__fmul_rn(y.x, r.y), __fmul_rn(y.y, r.x)),
+                       __fsub_rn(__fmul_rn(y.z, r.z), __fmul_rn(y.w, r.w)),
+                       __fadd_rn(__fmul_rn(y.z, r.w), __fmul_rn(y.w, r.z)));
+  };
+  auto low = [](float a, float b, float c, float n) { return __fsub_rn(__fmul_rn(a, c), __fmul_rn(b, n)); };
+  auto high = [](float a, float b, float c, float n) { return __fadd_rn(__fmul_rn(a, n), __fmul_rn(b, c)); };
+  const int per_row = PAIR ? total / 2 : total, gw = PAIR ? g4 / 2 : g4;
+  for (int i0 = blockIdx.y * kStoreThreads + tid; i0 < n * per_row; i0 += gridDim.y * kStoreThreads) {
+    // hd is a multiple of 32 (PAIR: 64), so the 8 threads of a block always run together
+    const int t = row_div.div(i0), g = i0 - t * per_row, head = head_div.div(g), i = 4 * (g - head * gw);
+    const int64_t row0 = s_row[t];
+    if (row0 == -2) continue;   // a row past the last sequence
+    const bool live = row0 >= 0;
+    const TX* xr = static_cast<const TX*>(a.x) + ((int64_t)(tok0 + t) * heads + head) * hd;
+    const int i2 = i + hd / 2;   // PAIR: this thread's other 4 values
+    float4 y = load4(xr + i), z = make_float4(0.f, 0.f, 0.f, 0.f);
+    if constexpr (PAIR) z = load4(xr + i2);
+    if (head < a.n_head + a.c.n_kv) {
       if (a.style == 0) {
-        const float2 r0 = cs[i / 2], r1 = cs[i / 2 + 1];
-        y = make_float4(__fsub_rn(__fmul_rn(y.x, r0.x), __fmul_rn(y.y, r0.y)),
-                        __fadd_rn(__fmul_rn(y.x, r0.y), __fmul_rn(y.y, r0.x)),
-                        __fsub_rn(__fmul_rn(y.z, r1.x), __fmul_rn(y.w, r1.y)),
-                        __fadd_rn(__fmul_rn(y.z, r1.y), __fmul_rn(y.w, r1.x)));
-      } else {
+        if (i < a.rot) y = turn_adjacent(cs[t], i, y);
+        if (PAIR && i2 < a.rot) z = turn_adjacent(cs[t], i2, z);
+      } else if (PAIR) {   // rot = hd: (y, z) are the pairs
+        const float4 r0 = *reinterpret_cast<const float4*>(&cs[t][i]), r1 = *reinterpret_cast<const float4*>(&cs[t][i + 2]);
+        const float4 u = y;
+        y = make_float4(low(u.x, z.x, r0.x, r0.y), low(u.y, z.y, r0.z, r0.w), low(u.z, z.z, r1.x, r1.y),
+                        low(u.w, z.w, r1.z, r1.w));
+        z = make_float4(high(u.x, z.x, r0.x, r0.y), high(u.y, z.y, r0.z, r0.w), high(u.z, z.z, r1.x, r1.y),
+                        high(u.w, z.w, r1.z, r1.w));
+      } else if (i < a.rot) {
         const bool lo = i < half;
         const int j = lo ? i : i - half;
-        const float4 z = load4(xr + (lo ? i + half : j));
-        const float yv[4] = {y.x, y.y, y.z, y.w}, zv[4] = {z.x, z.y, z.z, z.w};
-        float o[4];
-#pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          const float2 r = cs[j + e];
-          o[e] = lo ? __fsub_rn(__fmul_rn(yv[e], r.x), __fmul_rn(zv[e], r.y))
-                    : __fadd_rn(__fmul_rn(zv[e], r.y), __fmul_rn(yv[e], r.x));
-        }
-        y = make_float4(o[0], o[1], o[2], o[3]);
+        const float4 o = load4(xr + (lo ? i + half : j));
+        const float4 r0 = *reinterpret_cast<const float4*>(&cs[t][j]), r1 = *reinterpret_cast<const float4*>(&cs[t][j + 2]);
+        y = lo ? make_float4(low(y.x, o.x, r0.x, r0.y), low(y.y, o.y, r0.z, r0.w), low(y.z, o.z, r1.x, r1.y),
+                             low(y.w, o.w, r1.z, r1.w))
+               : make_float4(high(o.x, y.x, r0.x, r0.y), high(o.y, y.y, r0.z, r0.w), high(o.z, y.z, r1.x, r1.y),
+                             high(o.w, y.w, r1.z, r1.w));
       }
     }
     if (head < a.n_head) {
-      if (!live) y = make_float4(0.f, 0.f, 0.f, 0.f);
-      if constexpr (sizeof(TQ) == 4)
-        *reinterpret_cast<float4*>(q + head * hd + i) = y;
-      else
-        *reinterpret_cast<uint2*>(q + head * hd + i) = half4(y);
+      TQ* q = static_cast<TQ*>(a.q) + ((int64_t)(tok0 + t) * a.n_head + head) * hd + i;
+      if (!live) y = z = make_float4(0.f, 0.f, 0.f, 0.f);   // no place in the cache, or no angle: a zero q row
+      if constexpr (sizeof(TQ) == 4) {
+        *reinterpret_cast<float4*>(q) = y;
+        if constexpr (PAIR) *reinterpret_cast<float4*>(q + hd / 2) = z;
+      } else {
+        *reinterpret_cast<uint2*>(q) = half4(y);
+        if constexpr (PAIR) *reinterpret_cast<uint2*>(q + hd / 2) = half4(z);
+      }
     } else {
       const bool is_v = head >= a.n_head + a.c.n_kv;
       const int kh = head - a.n_head - (is_v ? a.c.n_kv : 0);
-      const int rb = is_v ? a.c.rb_v : a.c.rb_k;
+      const int rb = is_v ? a.c.rb_v : a.c.rb_k, type = is_v ? a.c.type_v : a.c.type_k;
       uint8_t* row = live ? (is_v ? a.c.v : a.c.k) + (row0 + ((int64_t)kh << a.c.ps_log2)) * rb : nullptr;
-      store_row4(row, is_v ? a.c.type_v : a.c.type_k, hd, i, y);
+      store_row4(row, type, hd, i, y);
+      if constexpr (PAIR) store_row4(row, type, hd, i2, z);
     }
   }
 }
@@ -286,15 +315,26 @@ __global__ void __launch_bounds__(kGatherThreads)
 
 int launch_page_rope_store(const RopeStoreArgs& a, cudaStream_t s) {
   // Few tokens: a token's heads are split over up to one CTA per 256 vectors,
-  // so that a decode step still covers the SMs.
-  const int most = ((a.n_head + 2 * a.c.n_kv) * a.hd / 4 + kStoreThreads - 1) / kStoreThreads;
-  const int want = (2 * kSMs + a.b.n_tok - 1) / a.b.n_tok;
-  const dim3 grid(a.b.n_tok, std::max(1, std::min(most, want))), block(kStoreThreads);
-  if (a.type_x == B2_F32)
-    return a.type_q == B2_F32 ? launch_pdl(page_rope_store_kernel<float, float>, grid, block, 0, s, a)
-                              : launch_pdl(page_rope_store_kernel<float, __half>, grid, block, 0, s, a);
-  return a.type_q == B2_F32 ? launch_pdl(page_rope_store_kernel<__half, float>, grid, block, 0, s, a)
-                            : launch_pdl(page_rope_store_kernel<__half, __half>, grid, block, 0, s, a);
+  // so that a decode step still covers the SMs.  Many: a CTA takes several
+  // tokens and looks their places up at once.
+  const int row = (a.n_head + 2 * a.c.n_kv) * a.hd / 4;   // vectors of a token
+  const int n_here = a.b.n_tok >= 4 * kStoreTokens * kSMs ? kStoreTokens : 1;
+  const int most = (row + kStoreThreads - 1) / kStoreThreads, want = (2 * kSMs + a.b.n_tok - 1) / a.b.n_tok;
+  const dim3 grid((a.b.n_tok + n_here - 1) / n_here, std::max(1, std::min(most, want))), block(kStoreThreads);
+  // 8 values a thread, a half head apart, where those are whole blocks and hold
+  // both sides of a half-split pair; else 4
+  const bool pair = a.hd % 64 == 0 && (a.style == 0 || a.rot == a.hd);
+  const FastDiv rd = FastDiv::of(pair ? row / 2 : row), hdv = FastDiv::of(pair ? a.hd / 8 : a.hd / 4);
+#define B2_STORE(TX, TQ)                                                                                       \
+  return pair ? launch_pdl(page_rope_store_kernel<TX, TQ, true>, grid, block, 0, s, a, n_here, rd, hdv)        \
+              : launch_pdl(page_rope_store_kernel<TX, TQ, false>, grid, block, 0, s, a, n_here, rd, hdv);
+  if (a.type_x == B2_F32) {
+    if (a.type_q == B2_F32) B2_STORE(float, float)
+    B2_STORE(float, __half)
+  }
+  if (a.type_q == B2_F32) B2_STORE(__half, float)
+  B2_STORE(__half, __half)
+#undef B2_STORE
 }
 
 int launch_page_copy(uint8_t* k, uint8_t* v, int n_layer, int64_t n_pages, int64_t page_k, int64_t page_v,

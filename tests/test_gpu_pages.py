@@ -24,12 +24,6 @@ def dev(a):
     return b2.DeviceBuffer.from_array(np.ascontiguousarray(a))
 
 
-def workspace_for(nbytes):
-    ws = b2.DeviceBuffer(nbytes)
-    ws.zero()
-    return ws
-
-
 # ---- the cache in numpy ------------------------------------------------------------------------
 def rows_of(x, t):
     """Values [..., hd] -> stored rows (uint8 [..., row bytes])."""
@@ -124,7 +118,7 @@ class Setup:
         q, out = dev(self.Q), dev(np.full(self.Q.shape, 77, NP[self.qt]))
         ws = None
         if workspace:
-            ws = workspace_for(b2.page_attn_workspace_bytes(c, b, self.n_head, self.qt))
+            ws = b2.page_attn_workspace(c, b, self.n_head, self.qt)
         status = dev(np.zeros(1, np.int32))
         b2.synchronize()
         b2.page_attn(c, self.layer, b, self.n_head, q, out, self.qt, scale=scale, window=window, workspace=ws,
@@ -307,7 +301,7 @@ def test_attn_layer_workspace_stream_and_graph():
     assert np.array_equal(a, s.run(stream=st.h).astype(np.float64))
     c, b = s.cache(), s.batch()
     q, out = dev(s.Q), dev(np.zeros(s.Q.shape, np.float16))
-    ws = workspace_for(b2.page_attn_workspace_bytes(c, b, 8, F16))
+    ws = b2.page_attn_workspace(c, b, 8, F16)
     b2.page_attn(c, 2, b, 8, q, out, F16, workspace=ws, stream=st.h)
     st.synchronize()
     g = b2.Graph(st, lambda h: b2.page_attn(c, 2, b, 8, q, out, F16, workspace=ws, stream=h))
