@@ -147,6 +147,11 @@ template <int HD, bool KQ, bool VQ, bool SPLIT>
 __host__ __device__ constexpr int rows_ctas() {
   return HD == 256 ? 1 : HD == 64 || (KQ && VQ && SPLIT) ? 3 : 2;
 }
+// Room for a tile's queries (WM = 1).
+template <int HD, bool SPLIT, int WM>
+__host__ __device__ constexpr int rows_q_bytes() {
+  return WM == 1 ? (SPLIT ? 8 * HD * 4 : 16 * HD * 2) : 0;
+}
 constexpr int kRowsStagesMax = 8, kRowsCtrl = 1024;
 constexpr int kWaitPolls = 1 << 22;   // polls of a wait, each suspended by the hardware for a while
 
@@ -226,9 +231,14 @@ __global__ void __launch_bounds__(kRowsThreads + 32, rows_ctas<HD, KQ, VQ, SPLIT
   uint8_t* smem = smem_raw + ((1024 - (smem_u32(smem_raw) & 1023)) & 1023);
   uint64_t* full = reinterpret_cast<uint64_t*>(smem);      // [stages]
   uint64_t* empty = full + kRowsStagesMax;                 // [stages]
+  uint64_t* t_full = empty + kRowsStagesMax;               // a tile and its queries have come,
+  uint64_t* t_empty = t_full + 1;                          // and been taken
   int* abort_flag = reinterpret_cast<int*>(smem + 256);
   int* last_part = abort_flag + 1;
-  uint8_t* ring = smem + kRowsCtrl;
+  TileAt* tile = reinterpret_cast<TileAt*>(smem + 320);
+  constexpr int kQRows = rows_q_bytes<HD, SPLIT, WM>();
+  uint8_t* q_rows = smem + kRowsCtrl;                      // WM = 1: the tile's queries as they are in q
+  uint8_t* ring = q_rows + kQRows;
 
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   if (tid == 0) {
@@ -236,7 +246,11 @@ __global__ void __launch_bounds__(kRowsThreads + 32, rows_ctas<HD, KQ, VQ, SPLIT
       mbar_init(&full[i], 1);
       mbar_init(&empty[i], 4);
     }
+    mbar_init(t_full, 1);
+    mbar_init(t_empty, 4);
     *abort_flag = 0;
+    *tile = TileAt{};   // what the warps would read if the first one never came
+    tile->units = 1;
     fence_mbar_init();
   }
   if (warp == 4 && lane < 2 && !(lane ? VQ : KQ))
@@ -290,12 +304,31 @@ __global__ void __launch_bounds__(kRowsThreads + 32, rows_ctas<HD, KQ, VQ, SPLIT
     };
     look_up(next_y);
     bool ok = true, wrote = false;
-    int n = 0;
-    for (; n < n_units; ++n) {
+    int n = 0, n_tiles = 0;
+    // hands the tile at sh.at to the computing warps
+    auto send_tile = [&]() {
+      if (n_tiles > 0) ok = __all_sync(0xffffffffu, wait(t_empty, (n_tiles - 1) & 1, 53));
+      ++n_tiles;
+      if (!ok) return;
+      const TileAt& at = sh.at;
+      const int row0 = at.t << w.rows_log2, rows = min(w.rows(), at.rows_total - row0);
+      const int es = a.q_f32 ? 4 : 2;
+      if (lane == 0) {
+        *tile = at;
+        mbar_arrive_expect_tx(t_full, WM == 1 ? rows * HD * es : 0);
+      }
+      __syncwarp();
+      if (WM == 1 && lane < rows) {
+        const int rr = row0 + lane, tok = w.G.div(rr);
+        const int64_t e = ((int64_t)(at.q0 + tok) * a.n_head + at.h * G + rr - tok * G) * HD;
+        bulk_g2s(q_rows + lane * HD * es, static_cast<const uint8_t*>(a.q) + e * es, HD * es, t_full);
+      }
+    };
+    send_tile();
+    for (; n < n_units && ok; ++n) {
       uint8_t* st = ring + (n % stages) * stage_bytes;
       uint64_t* bar = &full[n % stages];
-      const TileAt& at = sh.at;
-      const int key0 = (at.lo_unit + sh.off) * kRowsBk, lo = at.lo, hi = at.hi;
+      const int key0 = (sh.at.lo_unit + sh.off) * kRowsBk, lo = sh.at.lo, hi = sh.at.hi;
       uint32_t bytes = 0;
 #pragma unroll
       for (int e = 0; e < PER; ++e) {
@@ -313,6 +346,7 @@ __global__ void __launch_bounds__(kRowsThreads + 32, rows_ctas<HD, KQ, VQ, SPLIT
         }
         look_up(next_y);
       }
+      const bool new_tile = n + 1 < n_units && sh.off == 0;
       if (n >= stages) ok = __all_sync(0xffffffffu, wait(&empty[n % stages], (n / stages - 1) & 1, 50));
       if (!ok) break;
       if (wrote) fence_async_proxy();   // a stage may hold rows zeroed by hand
@@ -351,7 +385,9 @@ __global__ void __launch_bounds__(kRowsThreads + 32, rows_ctas<HD, KQ, VQ, SPLIT
             bulk_g2s(st + k_bytes + first * c.rb_v, c.v + (int64_t)y[e] * c.rb_v, run * c.rb_v, bar);
         }
       }
+      if (new_tile) send_tile();
     }
+    if (n_tiles > 0) mbar_wait_bounded(t_full, (n_tiles - 1) & 1, a.status, 54);
     // every copy issued has landed before the CTA may end
     for (int i = max(0, n - stages); i < n; ++i) mbar_wait_bounded(&full[i % stages], (i / stages) & 1, a.status, 51);
     return;
@@ -412,8 +448,10 @@ __global__ void __launch_bounds__(kRowsThreads + 32, rows_ctas<HD, KQ, VQ, SPLIT
   };
 
   int done = 0;   // units of the share so far
-  while (sh.u < sh.u_end) {
-    const TileAt at = sh.at;
+  for (int n_tile = 0; sh.u < sh.u_end; ++n_tile) {
+    wait(t_full, n_tile & 1, 55);
+    const TileAt at = *tile;
+    sh.at.units = at.units;
     const int u_lo = sh.off, u_hi = min(at.units, u_lo + (sh.u_end - sh.u));
     const int row0 = at.t << w.rows_log2;
     const int rows = min(w.rows(), at.rows_total - row0);
@@ -432,7 +470,16 @@ __global__ void __launch_bounds__(kRowsThreads + 32, rows_ctas<HD, KQ, VQ, SPLIT
       const bool on0 = r < rows, on1 = !SPLIT && r1 < rows;
       if (on0) p0 = at.first + w.G.div(row0 + r);
       if (on1) p1 = at.first + w.G.div(row0 + r1);
-      const int64_t e0 = place(on0 ? r : 0), e1 = place(on1 ? r1 : 0);
+      // WM = 1: from shared memory, else from q itself
+      const uint8_t* x0;
+      const uint8_t* x1;
+      if constexpr (WM == 1) {
+        x0 = q_rows + (on0 ? r : 0) * HD * (a.q_f32 ? 4 : 2);
+        x1 = q_rows + (on1 ? r1 : 0) * HD * (a.q_f32 ? 4 : 2);
+      } else {
+        x0 = static_cast<const uint8_t*>(a.q) + place(on0 ? r : 0) * (a.q_f32 ? 4 : 2);
+        x1 = static_cast<const uint8_t*>(a.q) + place(on1 ? r1 : 0) * (a.q_f32 ? 4 : 2);
+      }
 #pragma unroll
       for (int ks = 0; ks < KS; ++ks) {
         // dims of operand columns 2j, 2j + 1 and 2j + 8, 2j + 9
@@ -441,25 +488,24 @@ __global__ void __launch_bounds__(kRowsThreads + 32, rows_ctas<HD, KQ, VQ, SPLIT
           float2 x = make_float2(0.f, 0.f), y = x;
           if (on0) {
             if (a.q_f32) {
-              const float* q = static_cast<const float*>(a.q) + e0;
-              x = *reinterpret_cast<const float2*>(q + d0);
-              y = *reinterpret_cast<const float2*>(q + d1);
+              x = *reinterpret_cast<const float2*>(x0 + 4 * d0);
+              y = *reinterpret_cast<const float2*>(x0 + 4 * d1);
             } else {
-              const __half* q = static_cast<const __half*>(a.q) + e0;
-              x = __half22float2(*reinterpret_cast<const __half2*>(q + d0));
-              y = __half22float2(*reinterpret_cast<const __half2*>(q + d1));
+              x = __half22float2(*reinterpret_cast<const __half2*>(x0 + 2 * d0));
+              y = __half22float2(*reinterpret_cast<const __half2*>(x0 + 2 * d1));
             }
           }
           h2_split(x.x * a.scale_log2, x.y * a.scale_log2, qf[ks][0], qf[ks][1]);
           h2_split(y.x * a.scale_log2, y.y * a.scale_log2, qf[ks][2], qf[ks][3]);
         } else {
-          const __half* q = static_cast<const __half*>(a.q);
-          qf[ks][0] = on0 ? *reinterpret_cast<const uint32_t*>(q + e0 + d0) : 0u;
-          qf[ks][1] = on1 ? *reinterpret_cast<const uint32_t*>(q + e1 + d0) : 0u;
-          qf[ks][2] = on0 ? *reinterpret_cast<const uint32_t*>(q + e0 + d1) : 0u;
-          qf[ks][3] = on1 ? *reinterpret_cast<const uint32_t*>(q + e1 + d1) : 0u;
+          qf[ks][0] = on0 ? *reinterpret_cast<const uint32_t*>(x0 + 2 * d0) : 0u;
+          qf[ks][1] = on1 ? *reinterpret_cast<const uint32_t*>(x1 + 2 * d0) : 0u;
+          qf[ks][2] = on0 ? *reinterpret_cast<const uint32_t*>(x0 + 2 * d1) : 0u;
+          qf[ks][3] = on1 ? *reinterpret_cast<const uint32_t*>(x1 + 2 * d1) : 0u;
         }
       }
+      __syncwarp();
+      if (lane == 0) mbar_arrive(t_empty);
     }
 
     float o[OT][4];
@@ -899,7 +945,6 @@ __global__ void __launch_bounds__(kRowsThreads + 32, rows_ctas<HD, KQ, VQ, SPLIT
 
     sh.u += u_hi - u_lo;
     sh.off = 0;
-    if (sh.u < sh.u_end) next_tile(w, sh.at);
   }
 }
 
@@ -918,7 +963,7 @@ template <int HD, bool KQ, bool VQ, bool SPLIT, int WM>
 inline int rows_smem_bytes(const PageRowsArgs& a, int stages) {
   const int ring = stages * rows_stage_bytes<HD, KQ, VQ>(a.c.rb_k, a.c.rb_v) + rows_conv_bytes<HD, KQ, VQ, WM>();
   const int join = WM == 1 ? 64 * 8 + 4 * (SPLIT ? 8 : 16) * HD * 4 : 0, sums = kPageMaxSeq * 4;
-  return 1024 + kRowsCtrl + std::max(ring + join, sums);   // the first for alignment
+  return 1024 + kRowsCtrl + rows_q_bytes<HD, SPLIT, WM>() + std::max(ring + join, sums);   // the first for alignment
 }
 
 template <int HD, bool KQ, bool VQ, bool SPLIT, int WM>

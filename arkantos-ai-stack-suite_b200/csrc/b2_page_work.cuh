@@ -323,15 +323,26 @@ __device__ __forceinline__ void join_parts(const float* slots, int tile_rows, co
     return i < p.n ? __ldcg(reinterpret_cast<const float2*>(part(i) + tile_rows * HD + 2 * at)) : make_float2(-INFINITY, 0.f);
   };
   float top[R], sum[R], acc[R][V];
+  float2 kept[R];   // the first 32 parts'
 #pragma unroll
   for (int r = 0; r < R; ++r) {
-    top[r] = -INFINITY;
+    kept[r] = stat(lane, r);
+    top[r] = kept[r].x;
     sum[r] = 0.f;
 #pragma unroll
     for (int v = 0; v < V; ++v) acc[r][v] = 0.f;
   }
+  float x[U][R][V];
+  auto fetch = [&](int i0) {
+#pragma unroll
+    for (int u = 0; u < U; ++u)
+#pragma unroll
+      for (int r = 0; r < R; ++r)
+        load_part<V>(part(min(i0 + u, p.n - 1)) + (row + min(r, n_rows - 1)) * HD + lane * V, x[u][r]);
+  };
+  fetch(0);   // on their way with the statistics
 #pragma unroll 1
-  for (int i0 = 0; i0 < p.n; i0 += 32) {
+  for (int i0 = 32; i0 < p.n; i0 += 32) {
 #pragma unroll
     for (int r = 0; r < R; ++r) top[r] = fmaxf(top[r], stat(i0 + lane, r).x);
   }
@@ -342,19 +353,14 @@ __device__ __forceinline__ void join_parts(const float* slots, int tile_rows, co
     float wt[R];
 #pragma unroll
     for (int r = 0; r < R; ++r) {
-      const float2 ml = stat(i0 + lane, r);
+      const float2 ml = i0 == 0 ? kept[r] : stat(i0 + lane, r);
       wt[r] = part_weight(ml.x, ml.y, top[r]);
       sum[r] += wt[r] * ml.y;
     }
     const int m = min(32, p.n - i0);
 #pragma unroll 1
     for (int i1 = 0; i1 < m; i1 += U) {
-      float x[U][R][V];
-#pragma unroll
-      for (int u = 0; u < U; ++u)
-#pragma unroll
-        for (int r = 0; r < R; ++r)
-          load_part<V>(part(i0 + min(i1 + u, m - 1)) + (row + min(r, n_rows - 1)) * HD + lane * V, x[u][r]);
+      if (i0 + i1 > 0) fetch(i0 + i1);
 #pragma unroll
       for (int u = 0; u < U; ++u)
 #pragma unroll
