@@ -54,7 +54,9 @@ size_t page_attn_counters(const PageAttnArgs&) { return counter_bytes(kPageMaxCt
 
 size_t page_attn_workspace(const PageAttnArgs& a) {
   const Plan p = plan_of(a);
-  return page_attn_counters(a) + 2 * (size_t)p.max_ctas * slot_floats(p.rows, a.hd) * 4;
+  size_t floats = 2 * (size_t)p.max_ctas * slot_floats(p.rows, a.hd);
+  if (p.tc && p.split) floats += (size_t)p.max_ctas * p.rows * a.hd;   // the running sums
+  return page_attn_counters(a) + floats * 4;
 }
 
 int launch_page_attn(const PageAttnArgs& a, cudaStream_t s) {
@@ -78,6 +80,7 @@ int launch_page_attn(const PageAttnArgs& a, cudaStream_t s) {
     t.scale_log2 = scale_log2;
     t.counters = counters;
     t.slots = slots;
+    t.sums = slots + 2 * (size_t)p.max_ctas * slot_floats(p.rows, a.hd);
     t.status = a.status;
     t.pool_rows = pool_rows;
     return launch_page_tc(t, a.hd, p.split, 1 << a.c.ps_log2, s);

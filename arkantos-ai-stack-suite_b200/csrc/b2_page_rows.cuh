@@ -792,8 +792,19 @@ __global__ void __launch_bounds__(kRowsThreads + 32, rows_ctas<HD, KQ, VQ, SPLIT
                 uint32_t vf[4];   // 16 positions x 16 dims
                 if constexpr (SPLIT) {
                   ldsm4_t(vs_base + L::at(kw + k * 16 + (lane & 7) + (lane >> 4) * 8, b * 4 + 2 * d + ((lane >> 3) & 1)), vf);
-                  mma16816(o[b * 2 + d], vf, pf[0], pf[2]);
-                  mma16816(o[b * 2 + d], vf, pf[1], pf[3]);
+                  if constexpr (WM == 4) {
+                    // the tensor pipe cuts its sums to fp32; over a chunk's many
+                    // positions in one warp that would show, so 16 positions at
+                    // a time are added with rounding
+                    float t[4] = {0.f, 0.f, 0.f, 0.f};
+                    mma16816(t, vf, pf[1], pf[3]);
+                    mma16816(t, vf, pf[0], pf[2]);
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) o[b * 2 + d][e] += t[e];
+                  } else {
+                    mma16816(o[b * 2 + d], vf, pf[0], pf[2]);
+                    mma16816(o[b * 2 + d], vf, pf[1], pf[3]);
+                  }
                 } else {
                   ldsm4_t(vs_base + L::at(kw + k * 16 + (lane & 15), b * 4 + 2 * d + (lane >> 4)), vf);
                   mma16816(o[b * 4 + 2 * d], pf, vf[0], vf[1]);

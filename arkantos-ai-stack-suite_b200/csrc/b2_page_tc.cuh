@@ -38,6 +38,10 @@
 //
 // SPLIT (fp32 queries): q and p as two fp16 parts each, high and remainder,
 // two products instead of one; both parts of p take exactly S's columns.
+// The tensor pipe cuts its sums to fp32 at every step of 16, so an O that runs
+// over all positions loses accuracy with their number (7.8e-6 of the result
+// at 8192); after every 3 units SPLIT therefore adds it, rounded, to a sum in
+// the workspace and begins anew.
 // FULL rounds p once to fp16, the error of the fp16 output itself.
 //
 // V rows that a tile must not see are zeroed in shared memory before the
@@ -76,11 +80,16 @@ struct PageTcArgs {
   int64_t pool_rows;      // rows of the layer's pool
   unsigned* counters;
   float* slots;
+  float* sums;            // SPLIT: [ctas][2 halves][hd / 4][128 rows] float4
   int* status;
 };
 
 constexpr int kTcRows = 256, kTcBk = 128, kTcThreads = 384;
 constexpr float kTcOffset = 7.f, kTcRaise = 8.f;
+// SPLIT: units between two additions of O to its fp32 sum.  2, 3, 4, 8 and
+// never give 1.0, 1.2, 1.5, 2.0 and 2.3e-6 on a mixed step over 300-2049
+// positions, where fp32 arithmetic gives 0.9e-6, in 81, 78, 76, 73 and 65 us.
+constexpr int kTcFlush = 3;
 
 template <int HD, bool SPLIT>
 struct TcSmem {
@@ -551,12 +560,14 @@ __global__ void __launch_bounds__(kTcThreads, 1)
       bool ok = true;
       auto qk = [&](int i, uint32_t kd) {          // in the elected lane
         const uint32_t qd = q_desc + i * PARTS * (L::half_q >> 4);
+        // the remainders first: the sum is cut to fp32 at every step, and these
+        // steps' sums are small
 #pragma unroll
-        for (int part = 0; part < PARTS; ++part)
+        for (int part = PARTS - 1; part >= 0; --part)
 #pragma unroll
           for (int ks = 0; ks < HD / 16; ++ks) {
             const uint32_t off = ((ks / 4) * (128 * 128) + (ks % 4) * 32) >> 4;
-            tc_mma_ss(tm + i * 128, qd + part * (L::half_q >> 4) + off, kd + off, id_s, (part | ks) != 0);
+            tc_mma_ss(tm + i * 128, qd + part * (L::half_q >> 4) + off, kd + off, id_s, part != PARTS - 1 || ks != 0);
           }
         tc_commit(&s_full[i]);
       };
@@ -599,7 +610,7 @@ __global__ void __launch_bounds__(kTcThreads, 1)
           const int sv = n % NS, sk = (n + 1) % NS;
           const bool more = u + 1 < t.units;
           const uint32_t vd = uniform(v_desc + sv * (L::tile >> 4)), kd = uniform(k_desc + sk * (L::tile >> 4)),
-                         add = uniform(u > 0);
+                         add = uniform(SPLIT ? u % kTcFlush != 0 : u > 0);
           // K of the next unit and V of this one came while the softmax ran:
           // these waits are not on its path
           ok = wait(&v_ok[(n / 2) % NS], (n / 2 / NS) & 1, 62) &&
@@ -641,7 +652,7 @@ __global__ void __launch_bounds__(kTcThreads, 1)
   } else {
     asm volatile("setmaxnreg.inc.sync.aligned.u32 200;");
     // ---------------- softmax: a thread owns row 128·half + its lane of TMEM ----------------
-    const int half = warp >> 2, r = tid;   // row of the tile
+    const int half = warp >> 2, r = tid, r_in = tid & 127;   // row of the tile, of the half
     const uint32_t tm = tmem + ((uint32_t)((warp & 3) * 32) << 16);
     const uint32_t ts = tm + half * 128, to = tm + 256 + half * 128;
     const float c = SPLIT ? 1.f : fmaxf(fabsf(a.scale_log2), 1e-30f);   // the product takes the sign
@@ -703,7 +714,8 @@ __global__ void __launch_bounds__(kTcThreads, 1)
         fence_async_proxy();
         mbar_arrive(&q_full[half]);
       }
-      float m = -INFINITY, l = 0.f;
+      float m = -INFINITY, l = 0.f, m_sum = -INFINITY;   // m_sum: the maximum that the sum is relative to
+      float4* sum_row = SPLIT ? reinterpret_cast<float4*>(a.sums) + ((int64_t)blockIdx.x * 2 + half) * (HD / 4) * 128 + r_in : nullptr;
       for (int u = 0; u < units; ++u) {
         const int key0 = tile_key0 + u * kTcBk;
         const bool edge = tc_edge(t, key0, w.window);
@@ -711,6 +723,27 @@ __global__ void __launch_bounds__(kTcThreads, 1)
         ok = __all_sync(0xffffffffu, ok);
         if (!ok) break;
         tc_after();
+        if (SPLIT && u > 0 && u % kTcFlush == 0) {   // O of the last units is complete
+          const float f = m_sum == -INFINITY ? 0.f : ex2(m_sum - m);
+#pragma unroll 1
+          for (int i = 0; i < HD / 32; ++i) {
+            float o[32];
+            tmem_ld32(to + i * 32, o);
+            float4 x[8];
+            if (u > kTcFlush) {
+#pragma unroll
+              for (int e = 0; e < 8; ++e) x[e] = __ldcg(sum_row + (i * 8 + e) * 128);
+            }
+#pragma unroll
+            for (int e = 0; e < 8; ++e) {
+              float4 y = make_float4(o[4 * e], o[4 * e + 1], o[4 * e + 2], o[4 * e + 3]);
+              if (u > kTcFlush)
+                y = make_float4(fmaf(x[e].x, f, y.x), fmaf(x[e].y, f, y.y), fmaf(x[e].z, f, y.z), fmaf(x[e].w, f, y.w));
+              __stcg(sum_row + (i * 8 + e) * 128, y);
+            }
+          }
+          m_sum = m;
+        }
         float s[128];
         tmem_ld128(ts, s);
         // this row sees columns [lo, hi)
@@ -830,6 +863,17 @@ __global__ void __launch_bounds__(kTcThreads, 1)
       for (int i = by_copy ? HD / 32 : 0; i < HD / 32; ++i) {
         float o[32];
         tmem_ld32(to + i * 32, o);
+        if (SPLIT && units > kTcFlush) {
+          const float f = m_sum == -INFINITY ? 0.f : ex2(m_sum - m);
+#pragma unroll
+          for (int e = 0; e < 8; ++e) {
+            const float4 x = __ldcg(sum_row + (i * 8 + e) * 128);
+            o[4 * e] = fmaf(x.x, f, o[4 * e]);
+            o[4 * e + 1] = fmaf(x.y, f, o[4 * e + 1]);
+            o[4 * e + 2] = fmaf(x.z, f, o[4 * e + 2]);
+            o[4 * e + 3] = fmaf(x.w, f, o[4 * e + 3]);
+          }
+        }
 #pragma unroll
         for (int e = 0; e < 32; ++e) o[e] *= inv;
         if (!SPLIT && lane == 0) tma_store_read();   // an earlier tile's copy may still read the space

@@ -477,3 +477,52 @@ def test_gather_skips_positions_outside_the_tables():
     want = s.K.copy()
     want[:, free[0], :, 1] = s.K[:, s.table[0, 1], :, 3]
     assert np.array_equal(s.k.download(np.uint8).reshape(want.shape), want)
+
+
+# ---- together -----------------------------------------------------------------------------------------
+def test_example_conversations():
+    """examples/paged_chat.py: a forked conversation decoded token by token
+    gives the hidden states of the same tokens fed alone in one piece.  The
+    two differ by the order of fp32 sums and by Q8_0 codes of activations that
+    such differences move across a rounding boundary (one code is 1/127 of a
+    block's largest value, in one of 512 products)."""
+    import importlib.util
+    import os
+    path = os.path.join(os.path.dirname(os.path.dirname(os.path.abspath(__file__))), "examples", "paged_chat.py")
+    spec = importlib.util.spec_from_file_location("paged_chat", path)
+    mod = importlib.util.module_from_spec(spec)
+    spec.loader.exec_module(mod)
+    for users, steps in ((2, 3), (4, 20)):
+        difference, size = mod.main(n_users=users, steps=steps, seed=users)
+        assert difference < 2e-2 * size
+
+
+@pytest.mark.parametrize("qt", [F32, F16])
+def test_attn_nonfinite_values_in_whole_tiles(qt):
+    """As above, with enough sequences that tiles are finished by one CTA."""
+    n_seq, q_len, n = 24, 70, 90
+    s = Setup([q_len] * n_seq, [n] * n_seq, 16, 4, 64, 16, qt=qt, seed=2)
+    for i in range(n_seq):
+        p = n - 1 - (i % 40)
+        s.V[0, s.table[i, p // 16], :, p % 16, 6:8] = np.frombuffer(np.uint16(0x7C00 if i % 2 else 0x7E00).tobytes(), np.uint8)
+    got = s.run().astype(np.float64).reshape(n_seq, q_len, 16, 64)
+    clean = Setup([q_len] * n_seq, [n] * n_seq, 16, 4, 64, 16, qt=qt, seed=2)
+    want, vmax = (x.reshape(n_seq, q_len, 16, -1) for x in clean.want())
+    tol = 2e-5 * vmax + (2.0 ** -10 * vmax if qt == F16 else 0)
+    for i in range(n_seq):
+        first = q_len - 1 - (i % 40)          # the first row that sees the value, in dim 3
+        assert np.all(~np.isfinite(got[i, first:, :, 3]))
+        got[i, first:, :, 3] = want[i, first:, :, 3]
+    assert np.all(np.abs(got - want) <= tol)
+
+
+def test_attn_fp32_accuracy_does_not_fall_with_length():
+    """A chunk's fp32 sums over many positions, held to 4e-6 of the result in
+    the 2-norm: a score's products keep 22 bits of q (2^-23 each, of terms that
+    add like a random walk) and sums of at most 48 steps of 16 that the tensor
+    pipe cuts at 2^-24 each, 48 · 2^-24 = 2.9e-6 if every cut fell alike."""
+    for n in (2000, 12000):
+        s = Setup([24], [n], 4, 1, 128, 64, qt=F32, seed=n)
+        got = s.run().astype(np.float64)
+        want, _ = s.want()
+        assert np.linalg.norm(got - want) <= 4e-6 * np.linalg.norm(want)
