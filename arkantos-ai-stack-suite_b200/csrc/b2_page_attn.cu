@@ -10,8 +10,8 @@ namespace {
 // where it reads the cache, else the few-row kernel with its warps along the
 // rows.  One kernel takes all sequences of a call: running both, each on the
 // sequences of its kind, was slower (a step of 12 single tokens and 4 chunks
-// of 129 over 300-2049 positions: 81 us against 47 with fp16 queries, 84
-// against 64 with fp32), since the second begins when the first has ended.
+// of 129 over 300-2049 positions: 81 us against 47 with fp16 queries), since
+// the second begins when the first has ended.
 constexpr int kFewRows = 16;
 // Quantized pages under fp16 queries and more than kFewRows rows: the positions
 // that the call attends to are first written to the workspace as fp16 rows,
@@ -53,6 +53,13 @@ Plan plan_of(const PageAttnArgs& a) {
   }
   return p;
 }
+// Units' time that a warp takes to join a part of a split tile (see find_share).
+// One sequence's 8 tokens over 512, 4096 and 16384 fp16 positions: 22, 74 and
+// 65 us when every CTA gets some of them, 19, 33 and 56 with 0.4; 0.25 gives
+// 22, 43, 64, 0.6 19, 37, 59 and 1.5 24, 36, 56.  The few-row kernel's units and
+// tiles are smaller: fp32 queries over Q8_0 20, 54, 76 against 20, 41, 76 with
+// 0.1; 0.4 gives 24, 45, 80.
+constexpr float kJoinTc = 0.4f, kJoinRows = 0.1f;
 PageWork work_of(const PageAttnArgs& a, const Plan& p) {
   PageWork w = {};
   w.b = a.b;
@@ -62,6 +69,10 @@ PageWork work_of(const PageAttnArgs& a, const Plan& p) {
   w.window = a.window;
   while (w.rows() < p.rows) ++w.rows_log2;
   while (w.bk() < p.bk) ++w.bk_log2;
+  if (p.wm != 1) {   // one warp joins 32 rows; with few rows the join is spread over lanes and parts, and cheap
+    const int64_t tiles = (int64_t)a.c.n_kv * (a.b.n_seq + (((int64_t)a.b.n_tok * (a.n_head / a.c.n_kv)) >> w.rows_log2));
+    w.join_per_tile = (p.tc ? kJoinTc : kJoinRows) / (float)tiles;
+  }
   return w;
 }
 

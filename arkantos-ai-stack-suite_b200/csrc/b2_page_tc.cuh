@@ -11,8 +11,13 @@
 // thread owns a row: no exchange between lanes), the other half's products
 // run.  Both products of a unit cost 128·128·hd multiply-adds a half, 2048
 // tensor cycles for hd 128 and both halves; its 32768 exponentials take as
-// many cycles of the special-function pipe, so the two bound the kernel
-// together.
+// many cycles of the special-function pipe.  Neither is reached: a unit takes
+// some 3500 cycles, the length of a half's own chain of score product,
+// maximum, exponentials and second product, of which two run side by side
+// (TMEM holds no third half).  2048 tokens over 16384 positions, 32 heads of
+// 128: 437 us or 1180 TFLOP/s, the tensor pipe 57 % busy; SPLIT 905 us.  Two
+// threads a row (16 softmax warps) shorten the chain less than their exchange
+// of maxima costs: eight prompts 274 us against 267.
 //
 //   warps 0-3, 4-7  softmax of halves 0, 1, and their results
 //   warp 8          issues the products from one thread

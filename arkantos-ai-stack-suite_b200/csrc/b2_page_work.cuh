@@ -43,6 +43,7 @@ struct PageWork {
   PageSeqs b;
   FastDiv G;                                     // query heads of a kv head
   int ps_log2, n_kv, window, rows_log2, bk_log2;   // rows of a tile, positions of a unit
+  float join_per_tile;                             // see find_share
   __host__ __device__ int rows() const { return 1 << rows_log2; }
   __host__ __device__ int bk() const { return 1 << bk_log2; }
 };
@@ -135,7 +136,10 @@ __device__ __forceinline__ void sum_units(const PageWork& w, int* sums) {
 }
 
 // Warp-wide, from the sums: the share of CTA `cta` of `ctas`.  Returns false
-// for a CTA without work.
+// for a CTA without work.  A tile of U units in shares of k takes k units' time
+// and that of joining U/k parts; with j the units' time that a part takes to
+// join, k = sqrt(j U) is best, U the mean over the tiles (join_per_tile is j
+// over the number of tiles), and no CTA gets fewer.
 __device__ __forceinline__ bool find_share(const PageWork& w, int cta, int ctas, const int* sums, Share& sh) {
   const int lane = threadIdx.x & 31;
   int per_head = 0;
@@ -146,7 +150,8 @@ __device__ __forceinline__ bool find_share(const PageWork& w, int cta, int ctas,
     per_head += v;
   }
   const int total = per_head * w.n_kv;
-  sh.deal.n = min(total, ctas);
+  const int least = max(1, (int)ceilf(sqrtf(w.join_per_tile * (float)total)));
+  sh.deal.n = min((int)((unsigned)(total + least - 1) / (unsigned)least), ctas);
   if (cta >= sh.deal.n) return false;
   sh.deal.base = (int)((unsigned)total / (unsigned)sh.deal.n);
   sh.deal.rem = total - sh.deal.base * sh.deal.n;
