@@ -971,9 +971,8 @@ __global__ void __launch_bounds__(kTcThreads, 1)
 
 int launch_page_tc(PageTcArgs a, int hd, bool split, int page_size, cudaStream_t s);
 // The caches this kernel reads.
-inline bool page_tc_hd(int hd) { return hd == 64 || hd == 128; }
 inline bool page_tc_ok(const PageView& c, int hd) {
-  return page_tc_hd(hd) && c.type_k == B2_F16 && c.type_v == B2_F16;
+  return (hd == 64 || hd == 128) && c.type_k == B2_F16 && c.type_v == B2_F16;
 }
 
 }  // namespace b2

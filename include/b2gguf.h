@@ -410,14 +410,11 @@ B2_API int b2_rope_sections(const int32_t* sections, int32_t n_axes, int32_t n_p
  * (p - window, p], window <= 0 meaning all up to p, with n_head/n_kv query
  * heads per kv head and scores scale·q·k.  q and out [n_tok][n_head][head_dim]
  * of type_q: B2_F32 is computed to fp32 accuracy, B2_F16 rounds the softmax
- * weights to fp16, and when more than 16 rows (tokens x n_head/n_kv) of a
- * sequence attend to quantized pages of head_dim 64 or 128, K and V as well
- * (|k| up to 65504 then), through up to 1 GiB of the workspace.  A token that
- * sees no position gets a zero row; no value outside the positions a token
- * sees reaches its row, infinite and NaN ones included.  Results do not depend
- * on timing: the same call gives the same bits.  Unlike b2_attn_decode the
- * sums are not in the reference's sequential order.  |scale·q| and |v| up to
- * 65504 (fp16's range).
+ * weights to fp16.  A token that sees no position gets a zero row; no value
+ * outside the positions a token sees reaches its row, infinite and NaN ones
+ * included.  Results do not depend on timing: the same call gives the same
+ * bits.  Unlike b2_attn_decode the sums are not in the reference's sequential
+ * order.  |scale·q| and |v| up to 65504 (fp16's range).
  * workspace: device, 16-byte aligned, of at least
  * b2_page_attn_workspace_bytes for the call's shapes, set to zero (b2_memset)
  * before its first use; every call leaves it fit for the next, of any shape

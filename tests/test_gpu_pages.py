@@ -526,84 +526,3 @@ def test_attn_fp32_accuracy_does_not_fall_with_length():
         got = s.run().astype(np.float64)
         want, _ = s.want()
         assert np.linalg.norm(got - want) <= 4e-6 * np.linalg.norm(want)
-
-
-# ---- many rows of fp16 queries over quantized pages: the positions are expanded to fp16 first -------------
-def check_expanded(s, **kw):
-    """K and V rounded to fp16 once, like the weights and the result: each a
-    relative error of 2^-11 at most, uniform, so 2^-12.8 in the 2-norm; those
-    of K's products add like a random walk to about as much of a score of unit
-    variance as of a value.  Four of them are 2^-11.8, held to 2^-10.  Of the
-    largest value a row sees, one result: 2^-10 for V and the result, and twice
-    the change of a score, 2^-11 of sum |q k| (at most 2 sqrt(hd) for these
-    unit normal values), and the weights' 2^-11."""
-    got = s.run(**kw).astype(np.float64)
-    kw.pop("workspace", None)
-    want, vmax = s.want(**kw)
-    assert np.all(np.isfinite(got))
-    assert np.all(np.abs(got - want) <= (2.0 ** -10 + 2.0 ** -11 + 2.0 ** -10 * 2 * s.hd ** 0.5) * vmax)
-    assert np.linalg.norm(got - want) <= 2.0 ** -10 * np.linalg.norm(want)
-    return got
-
-
-@pytest.mark.parametrize("kt,vt", [(Q8, Q8), (Q4, Q4), (F16, Q8), (Q4, F16)])
-@pytest.mark.parametrize("hd,n_head,n_kv,page", [(64, 8, 2, 8), (128, 4, 1, 32), (128, 6, 2, 256), (64, 5, 5, 128)])
-def test_attn_expanded_pages(kt, vt, hd, n_head, n_kv, page):
-    s = Setup([130, 1, 0, 45, 3], [130, 257, 12, 300, 3], n_head, n_kv, hd, page, kt, vt, qt=F16, seed=hd + page)
-    check_expanded(s)
-
-
-@pytest.mark.parametrize("window", [1, 50, 300])
-@pytest.mark.parametrize("page", [16, 256])
-def test_attn_expanded_pages_window(window, page):
-    s = Setup([140, 64, 1], [700, 64, 513], 4, 2, 64, page, Q8, Q4, qt=F16, seed=window)
-    check_expanded(s, window=window)
-
-
-def test_attn_expanded_pages_layer_table_and_workspace():
-    """Another layer, table entries outside the pool, more new tokens than
-    positions, a workspace that holds anything past its counters."""
-    s = Setup([128, 150, 30], [200, 140, 90], 4, 2, 128, 16, Q8, Q8, qt=F16, seed=9, n_layer=3, layer=1)
-    s.table[0, 3], s.table[2, 0] = -7, s.n_pages + 1
-    a = check_expanded(s)
-    assert np.all(a[128:138] == 0)             # rows before the first position
-    assert np.array_equal(a, s.run(workspace=False).astype(np.float64))
-    c, b = s.cache(), s.batch()
-    ws = b2.page_attn_workspace(c, b, s.n_head, F16)
-    x = np.full(ws.nbytes, 0x7E, np.uint8)
-    x[:1 << 16] = 0                            # the counters
-    ws.upload(x)
-    out = dev(np.full(s.Q.shape, 77, np.float16))
-    q = dev(s.Q)
-    for _ in range(2):
-        b2.page_attn(c, s.layer, b, s.n_head, q, out, F16, workspace=ws)
-    b2.synchronize()
-    assert np.array_equal(out.download(np.float16).reshape(s.Q.shape).astype(np.float64), a)
-
-
-@pytest.mark.parametrize("bits", [0x7C00, 0xFC00, 0x7E00])
-def test_attn_expanded_pages_nonfinite_scales(bits):
-    """Infinite and NaN scales reach the rows that see them and no others."""
-    q_len, n, at = 140, 200, 150
-    s = Setup([q_len], [n], 4, 2, 64, 16, Q8, Q8, qt=F16, seed=3)
-    want, vmax = s.want()
-    for pool in (s.K, s.V):
-        pool[0, s.table[0, at // 16], :, at % 16, 64:66] = np.frombuffer(np.uint16(bits).tobytes(), np.uint8)
-    got = s.run().astype(np.float64)
-    first = at - (n - q_len)
-    assert np.all(~np.isfinite(got[first:]).all(-1))
-    assert np.linalg.norm((got - want)[:first]) <= 2.0 ** -10 * np.linalg.norm(want[:first])
-
-
-def test_attn_expanded_pages_capacity():
-    """A table whose capacity is past what a workspace may take: the pages are
-    read as they are, to the accuracy of exact codes."""
-    s = Setup([130], [600], 16, 8, 128, 256, Q8, Q8, qt=F16, seed=5)
-    small = s.run()
-    wide = np.full((1, 1100), -1, np.int32)    # 281600 positions of 4 KB each
-    wide[:, :s.max_pages] = s.table
-    narrow_bytes = b2.page_attn_workspace_bytes(s.cache(), s.batch(), s.n_head, F16)
-    s.table, s.max_pages = wide, 1100
-    assert b2.page_attn_workspace_bytes(s.cache(), s.batch(), s.n_head, F16) < narrow_bytes + (64 << 20)
-    got = s.check()
-    assert np.linalg.norm(got - small.astype(np.float64)) <= 2.0 ** -10 * np.linalg.norm(got)
