@@ -578,6 +578,8 @@ __global__ void __launch_bounds__(kRowsThreads + 32, rows_ctas<HD, KQ, VQ, SPLIT
             if (changed) *q = x, found = 1;
           }
         }
+        // a later copy into this stage must not be overtaken by these stores
+        fence_async_proxy();
       }
       if constexpr (WM == 4) {
         if (edge)
