@@ -62,7 +62,9 @@
 // every role it was 160 KB, and its fetches showed at every change of tiles.
 //
 // Every wait is bounded: an expired one records a code in *status and ends
-// the other waits.
+// the other waits; warps leave whole, copies in flight are waited for and TMEM
+// is given back.  Parts of split tiles may then never be counted: the
+// workspace's counters have to be cleared again.
 #pragma once
 
 #include <cuda.h>
@@ -350,6 +352,8 @@ __global__ void __launch_bounds__(kTcThreads, 1)
   pdl_launch_dependents();   // only now: a later kernel must not take the TMEM before this CTA has it
 
   // A wait of one thread; after one in the CTA has expired all others return.
+  // Lanes may learn of that at different polls, so a warp votes before any of
+  // them leaves a loop: what follows asks for all 32.
   auto wait = [&](uint64_t* bar, uint32_t parity, int code) -> bool {
     for (int i = 0; !mbar_try_wait(bar, parity); ++i)
       if (i == kWaitPolls || *reinterpret_cast<volatile int*>(abort_flag)) {
@@ -359,9 +363,12 @@ __global__ void __launch_bounds__(kTcThreads, 1)
       }
     return true;
   };
+  auto warp_wait = [&](uint64_t* bar, uint32_t parity, int code) -> bool {
+    return __all_sync(0xffffffffu, wait(bar, parity, code));
+  };
   // The n-th tile of the share, copied out of the ring (whole warps).
   auto take_tile = [&](int n, TcTile& t) -> bool {
-    if (!wait(&t_full[n % kTcTiles], (n / kTcTiles) & 1, 90)) return false;
+    if (!warp_wait(&t_full[n % kTcTiles], (n / kTcTiles) & 1, 90)) return false;
     const int4* src = reinterpret_cast<const int4*>(&tiles[n % kTcTiles]);
     int4* dst = reinterpret_cast<int4*>(&t);
 #pragma unroll
@@ -402,8 +409,7 @@ __global__ void __launch_bounds__(kTcThreads, 1)
           for (int kv = 0; kv < 2; ++kv, ++n) {
             const int st = n % NS;
             uint64_t* full = (kv ? v_full : k_full) + (n / 2) % NS;
-            if (n >= NS) ok = ok && wait(&kv_empty[st], ((n / NS) - 1) & 1, 50);
-            ok = __all_sync(0xffffffffu, ok);
+            if (n >= NS) ok = warp_wait(&kv_empty[st], ((n / NS) - 1) & 1, 50);
             if (!ok) break;
             if (lane == 0) mbar_arrive_expect_tx(full, L::tile);
             __syncwarp();
@@ -429,7 +435,7 @@ __global__ void __launch_bounds__(kTcThreads, 1)
       int fills[2] = {0, 0};
       bool ok = true;
       for (int nt = 0; ok; ++nt) {
-        if (nt >= kTcTiles) ok = __all_sync(0xffffffffu, wait(&t_empty[nt % kTcTiles], (nt / kTcTiles - 1) & 1, 91));
+        if (nt >= kTcTiles) ok = warp_wait(&t_empty[nt % kTcTiles], (nt / kTcTiles - 1) & 1, 91);
         if (!ok) break;
         TcTile t = {};
         const bool more = sh.u < sh.u_end;
@@ -464,9 +470,9 @@ __global__ void __launch_bounds__(kTcThreads, 1)
             // Rows past the sequence are other tokens' and are not written.
             const int z = t.q0 + w.G.div(t.row0), dz = w.G.div(128);
             for (int i = 0; i < halves && ok; ++i) {
-              if (fills[i] > 0) ok = __all_sync(0xffffffffu, wait(&q_empty[i], (fills[i] - 1) & 1, 80));
-              ++fills[i];
+              if (fills[i] > 0) ok = warp_wait(&q_empty[i], (fills[i] - 1) & 1, 80);
               if (!ok) break;
+              ++fills[i];
               if (lane == 0) mbar_arrive_expect_tx(&q_full[i], L::half_q);
               __syncwarp();
               if (lane < HD / 64)
@@ -476,9 +482,9 @@ __global__ void __launch_bounds__(kTcThreads, 1)
             const __half* src = static_cast<const __half*>(a.q) + ((int64_t)t.q0 * a.n_head + t.h * G) * HD + ch * 8;
             int tok = w.G.div(t.row0 + rl), g = (t.row0 + rl) - tok * G;
             for (int i = 0; i < halves && ok; ++i) {
-              if (fills[i] > 0) ok = __all_sync(0xffffffffu, wait(&q_empty[i], (fills[i] - 1) & 1, 80));
-              ++fills[i];
+              if (fills[i] > 0) ok = warp_wait(&q_empty[i], (fills[i] - 1) & 1, 80);
               if (!ok) break;
+              ++fills[i];
               const uint32_t qd = smem_u32(Qs) + i * L::half_q + (ch / 8) * (128 * 128);
 #pragma unroll 2
               for (int r = rl; r < 128; r += RI) {
@@ -512,7 +518,8 @@ __global__ void __launch_bounds__(kTcThreads, 1)
       for (int nt = 0; ok && take_tile(nt, t); ++nt) {
         for (int u = 0; ok && u < t.units; ++u, ++n) {
           const int key0 = t.key0 + u * kTcBk;
-          ok = wait(&v_full[n % NS], (n / NS) & 1, 71);
+          ok = warp_wait(&v_full[n % NS], (n / NS) & 1, 71);
+          if (!ok) break;
           if (tc_edge(t, key0, w.window)) {
             // zeros where the tile sees nothing; of the others only positions
             // that some row does not see are looked over
@@ -604,6 +611,7 @@ __global__ void __launch_bounds__(kTcThreads, 1)
         if (elect_one()) tc_commit(&kv_empty[n % NS]);
         __syncwarp();
         ++n;
+        ok = __all_sync(0xffffffffu, ok);
       };
       TcTile t;
       int nt = 0;
@@ -647,7 +655,7 @@ __global__ void __launch_bounds__(kTcThreads, 1)
           if (!ok) break;
         }
         if (!ok) break;
-        have = __all_sync(0xffffffffu, take_tile(nt++, t));
+        have = take_tile(nt++, t);
         if (have) open_tile(t);
       }
       if (elect_one()) tc_commit(done);   // every product has completed before TMEM is given back
@@ -666,7 +674,7 @@ __global__ void __launch_bounds__(kTcThreads, 1)
     for (int nt = 0; ok; ++nt) {
       // The tile stays in the ring until its results are out: what the units
       // need is in registers, the rest is read where it is used.
-      ok = __all_sync(0xffffffffu, wait(&t_full[nt % kTcTiles], (nt / kTcTiles) & 1, 90));
+      ok = warp_wait(&t_full[nt % kTcTiles], (nt / kTcTiles) & 1, 90);
       if (!ok) break;
       const TcTile& t = tiles[nt % kTcTiles];
       auto leave_tile = [&]() {
@@ -724,8 +732,7 @@ __global__ void __launch_bounds__(kTcThreads, 1)
       for (int u = 0; u < units; ++u) {
         const int key0 = tile_key0 + u * kTcBk;
         const bool edge = tc_edge(t, key0, w.window);
-        ok = wait(&s_full[half], n_s++ & 1, 70);
-        ok = __all_sync(0xffffffffu, ok);
+        ok = warp_wait(&s_full[half], n_s++ & 1, 70);
         if (!ok) break;
         tc_after();
         if (SPLIT && u > 0 && u % kTcFlush == 0) {   // O of the last units is complete
@@ -827,8 +834,7 @@ __global__ void __launch_bounds__(kTcThreads, 1)
         l += (sum[0].x + sum[0].y) + (sum[1].x + sum[1].y);
       }
       // ---- the result ----
-      if (ok) ok = wait(&o_full[half], n_o++ & 1, 72);
-      ok = __all_sync(0xffffffffu, ok);
+      if (ok) ok = warp_wait(&o_full[half], n_o++ & 1, 72);
       if (!ok) break;
       tc_after();
       const bool whole = t.split.n == 0;

@@ -420,7 +420,9 @@ B2_API int b2_rope_sections(const int32_t* sections, int32_t n_axes, int32_t n_p
  * before its first use; every call leaves it fit for the next, of any shape
  * that it is large enough for, and one call at a time may use it.  NULL: the
  * call allocates stream-ordered scratch.  status (device int,
- * may be NULL) receives a nonzero code if a pipeline wait expired. */
+ * may be NULL) receives a nonzero code if a pipeline wait expired; the call's
+ * results are then undefined, and the workspace is to be set to zero again
+ * before its next use. */
 B2_API int b2_page_attn_workspace_bytes(const b2_page_cache* cache, const b2_page_batch* batch, int32_t n_head,
                                         int type_q, size_t* bytes);
 B2_API int b2_page_attn(const b2_page_cache* cache, int32_t layer, const b2_page_batch* batch, int32_t n_head,
