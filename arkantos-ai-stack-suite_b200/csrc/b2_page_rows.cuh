@@ -115,11 +115,16 @@ __device__ __forceinline__ void s8x4_to_h2(uint32_t w, uint32_t& a, uint32_t& b)
   b = *reinterpret_cast<const uint32_t*>(&q);
 }
 
-// p is carried times 2^offset so that its fp16 parts stay normal; the sum
-// carries the same factor.  With a quantized V the operand is p·d, d the
-// block scale: |v| <= 65504 bounds d by 516 (Q8_0) and 8188 (Q4_0), which
-// leaves room for 2^6 and 2^3.
-__host__ __device__ inline float p_offset(int type_v) { return type_v == B2_F16 ? 10.f : type_v == B2_Q8_0 ? 6.f : 3.f; }
+// p is carried times 2^offset so that its fp16 parts stay normal; the sum of
+// the weights carries the same factor.  With a quantized V the operand is p·d,
+// d the block scale, and the offset is 15 + e, 2^e the power of two that brings
+// the largest |d| so far into [1/2, 1): the operand uses fp16's whole range
+// whatever the size of V (error of the result for V of size 1e-3 over Q8_0:
+// 4.3e-7, with one offset for all sizes 4.5e-5).  When a larger d comes, e falls
+// and the sums with it, exactly.
+constexpr float kOffset = 10.f, kOffsetQ = 15.f;
+constexpr int kFitMost = 23;   // e for the smallest fp16 scale, 2^-24
+__device__ __forceinline__ float pow2(int e) { return __int_as_float((e + 127) << 23); }
 
 // An fp16 (or unpacked) operand: [dims / 64][64 rows][128 bytes], 16-byte
 // chunk c of row r at c ^ (r % 8).
@@ -239,6 +244,7 @@ __global__ void __launch_bounds__(kRowsThreads + 32, rows_ctas<HD, KQ, VQ, SPLIT
   uint64_t* t_empty = t_full + 1;                          // and been taken
   int* abort_flag = reinterpret_cast<int*>(smem + 256);
   int* last_part = abort_flag + 1;
+  uint32_t* v_top = reinterpret_cast<uint32_t*>(smem + 264);   // [2] by unit (WM = 4): largest scale of V, as bits, if the offset must fall
   TileAt* tile = reinterpret_cast<TileAt*>(smem + 320);
   constexpr int kQRows = rows_q_bytes<HD, SPLIT, WM>();
   uint8_t* q_rows = smem + kRowsCtrl;                      // WM = 1: the tile's queries as they are in q
@@ -253,6 +259,7 @@ __global__ void __launch_bounds__(kRowsThreads + 32, rows_ctas<HD, KQ, VQ, SPLIT
     mbar_init(t_full, 1);
     mbar_init(t_empty, 4);
     *abort_flag = 0;
+    v_top[0] = v_top[1] = 0;
     *tile = TileAt{};   // what the warps would read if the first one never came
     tile->units = 1;
     fence_mbar_init();
@@ -401,12 +408,12 @@ __global__ void __launch_bounds__(kRowsThreads + 32, rows_ctas<HD, KQ, VQ, SPLIT
   float* scale_k = reinterpret_cast<float*>(conv_k + L::tile);
   uint8_t* conv_v = conv_k + (KQ ? L::tile + L::scales : 0);
   float* scale_v = reinterpret_cast<float*>(conv_v + L::tile);
-  const float off = p_offset(c.type_v);
 
   // Quantized rows of a stage -> fp16 codes and fp32 scales [block][position] (WM = 4).
   auto unpack = [&](const uint8_t* raw, int type, int rb, uint8_t* dst, float* sc, const FastDiv& cpr, int lo, int hi,
-                    bool guard) {
+                    bool guard, float& top) {
     int found = 0;   // infinite or NaN scales, taken out when guarded; rows outside [lo, hi) count as zeros
+    top = 0.f;       // the largest scale
     const int cb = type == B2_Q8_0 ? HD : HD / 2;
     const int cpk = (int)cpr.d - 1, total = kRowsBk * (int)cpr.d;   // a row: code chunks, then the scales'
 #pragma unroll 2
@@ -420,6 +427,7 @@ __global__ void __launch_bounds__(kRowsThreads + 32, rows_ctas<HD, KQ, VQ, SPLIT
         for (int b = 0; b < NB; ++b) {
           if (key < lo || key >= hi) d[b] = 0.f;
           if (guard && !(fabsf(d[b]) <= 65504.f)) d[b] = 0.f, found = 1;
+          top = fmaxf(top, fabsf(d[b]));
           sc[b * kRowsBk + key] = d[b];
         }
         continue;
@@ -534,6 +542,21 @@ __global__ void __launch_bounds__(kRowsThreads + 32, rows_ctas<HD, KQ, VQ, SPLIT
       }
     };
     float m0 = -INFINITY, m1 = -INFINITY, l0 = 0.f, l1 = 0.f;   // rows g and g + 8 (SPLIT: row g)
+    float off = VQ ? kOffsetQ + kFitMost : kOffset, fit = VQ ? pow2(kFitMost) : 1.f;   // fit: 2^e of the offset
+    auto fit_scales = [&](float top) {   // top: the same in every lane
+      top = fminf(top, 65504.f);         // what an infinite scale does to its rows needs no room
+      if (top * fit < 1.f) return;
+      const int e_old = (__float_as_int(fit) >> 23) - 127, e = 126 - (__float_as_int(top) >> 23);
+      const float r = pow2(e - e_old);
+#pragma unroll
+      for (int d = 0; d < OT; ++d)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) o[d][i] *= r;
+      l0 *= r;
+      l1 *= r;
+      fit = pow2(e);
+      off = kOffsetQ + e;
+    };
     // positions every live row sees need no mask
     const int p_min = at.first + w.G.div(row0), p_max = at.first + w.G.div(row0 + rows - 1);
 
@@ -554,8 +577,12 @@ __global__ void __launch_bounds__(kRowsThreads + 32, rows_ctas<HD, KQ, VQ, SPLIT
       const int v_lo = edge ? at.lo - key0 : 0, v_hi = edge ? at.hi - key0 : kRowsBk;   // rows of V the tile sees
       if constexpr (WM == 4) {
         if constexpr (KQ || VQ) bar_compute();   // the last unit's operands are done with
-        if constexpr (KQ) unpack(st, c.type_k, c.rb_k, conv_k, scale_k, a.cpr_k, 0, kRowsBk, false);
-        if constexpr (VQ) found = unpack(st + k_bytes, c.type_v, c.rb_v, conv_v, scale_v, a.cpr_v, v_lo, v_hi, guard);
+        float top;
+        if constexpr (KQ) unpack(st, c.type_k, c.rb_k, conv_k, scale_k, a.cpr_k, 0, kRowsBk, false, top);
+        if constexpr (VQ) {
+          found = unpack(st + k_bytes, c.type_v, c.rb_v, conv_v, scale_v, a.cpr_v, v_lo, v_hi, guard, top);
+          if (top * fit >= 1.f) atomicMax(&v_top[done & 1], __float_as_uint(top));   // the offset must fall
+        }
       }
       if (!VQ && edge) {
         // WM = 1: a warp looks over its own positions
@@ -586,6 +613,10 @@ __global__ void __launch_bounds__(kRowsThreads + 32, rows_ctas<HD, KQ, VQ, SPLIT
           bad = bar_compute_or(found);
         else if (KQ || VQ)
           bar_compute();
+        if constexpr (VQ) {
+          fit_scales(__uint_as_float(*reinterpret_cast<volatile uint32_t*>(&v_top[done & 1])));
+          if (tid == 0) v_top[(done + 1) & 1] = 0;   // read before the barrier above, used after the next unit's first
+        }
       } else if (!VQ && edge) {
         __syncwarp();
         bad = __any_sync(0xffffffffu, found);
@@ -705,6 +736,13 @@ __global__ void __launch_bounds__(kRowsThreads + 32, rows_ctas<HD, KQ, VQ, SPLIT
               }
             }
           }
+          float top = 0.f;
+#pragma unroll
+          for (int r = 0; r < 4; ++r)
+#pragma unroll
+            for (int b = 0; b < NB; ++b) top = fmaxf(top, fabsf(sc[r][b]));
+          top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
+          fit_scales(fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2)));   // lanes of the same j hold the same
         }
         // ---- running maximum and sum ----
         float n0 = m0, n1 = m1;
@@ -857,6 +895,15 @@ __global__ void __launch_bounds__(kRowsThreads + 32, rows_ctas<HD, KQ, VQ, SPLIT
       }
     }
 
+    if constexpr (VQ) {   // warps and parts meet with the same offset
+      const float r = pow2(127 - (__float_as_int(fit) >> 23));
+#pragma unroll
+      for (int d = 0; d < OT; ++d)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) o[d][e] *= r;
+      l0 *= r;
+      l1 *= r;
+    }
     // ---- join the lanes' sums, and for WM = 1 the warps ----
 #pragma unroll
     for (int x = 1; x < 4; x <<= 1) {

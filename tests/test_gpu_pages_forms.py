@@ -84,3 +84,51 @@ def test_attn_stages_used_again_after_masked_units(n_head, n_kv, hd, q_len, n_se
     r = np.random.default_rng(hd)
     kv = [int(x) for x in r.integers(q_len, 260, n_seq)]
     check_sampled(Setup([q_len] * n_seq, kv, n_head, n_kv, hd, 16, qt=qt, seed=hd + q_len), 400)
+
+
+# ---- values of every size ------------------------------------------------------------------------
+FORMS = {"tokens": (1, 8, 4), "tokens of 12 heads": (1, 12, 1), "chunk": (40, 4, 2)}   # new tokens, heads, kv heads
+
+
+def check_norm(s, blocks=1, n_rows=200, **kw):
+    """The 2-norm's bound, for every run of hd / blocks values on its own."""
+    got = s.run(**kw)
+    a, w, _ = sampled(s, got, n_rows, **kw)
+    for x, y in zip(np.split(a, blocks, 1), np.split(w, blocks, 1)):
+        tol = 4e-6 * np.linalg.norm(y) if s.qt == F32 else 2.0 ** -11 * np.linalg.norm(y) + 2.0 ** -25 * y.size ** 0.5
+        err = np.linalg.norm(x - y)
+        assert err <= tol, f"{err / np.linalg.norm(y):.3g} of the result, {err / tol:.3g} of the tolerance"
+
+
+@pytest.mark.parametrize("form", FORMS)
+@pytest.mark.parametrize("qt", [F32, F16])
+@pytest.mark.parametrize("t", [Q8, Q4])
+@pytest.mark.parametrize("size", [1, 1e-2, 1e-3, 1e-4, 300])
+def test_attn_quantized_values_of_any_size(form, qt, t, size):
+    q_len, n_head, n_kv = FORMS[form]
+    check_norm(shared(3, 1500, n_head, n_kv, 128, 32, t, t, qt, 11, q_len, v=lambda x: size * x))
+
+
+@pytest.mark.parametrize("form", FORMS)
+@pytest.mark.parametrize("t", [Q8, Q4])
+def test_attn_quantized_values_of_mixed_size(form, t):
+    """Blocks of one row whose sizes differ: each is good on its own."""
+    q_len, n_head, n_kv = FORMS[form]
+    f = np.repeat(np.array([1, 1e-3, 30, 1e-2], np.float32), 32)
+    check_norm(shared(3, 1500, n_head, n_kv, 128, 32, t, t, F32, 12, q_len, v=lambda x: f * x), blocks=4)
+
+
+@pytest.mark.parametrize("form", FORMS)
+@pytest.mark.parametrize("t", [Q8, Q4])
+@pytest.mark.parametrize("hd", [64, 128, 256])
+@pytest.mark.parametrize("grow", [1, -1])
+def test_attn_quantized_values_growing_along_the_positions(form, t, hd, grow):
+    """The largest block scale rises (or falls) by six decades along a sequence, and some blocks are zero."""
+    q_len, n_head, n_kv = FORMS[form]
+    s = shared(300, 900, n_head, n_kv, hd, 16, t, t, F32, 16, q_len)
+    p = np.arange(900)
+    size = 10.0 ** (grow * (p - 450) / 150)
+    size[100:170] = 0
+    v = np.random.default_rng(1).standard_normal((900, n_kv, hd)) * size[:, None, None]
+    s.V[0, s.table[0, p // 16], :, p % 16] = rows_of(v.astype(np.float32), t)
+    check_norm(s)
