@@ -1,4 +1,6 @@
 // Page attention: the choice of kernel and its launch.
+#include <math.h>
+
 #include "b2_page_tc.cuh"
 
 namespace b2 {
@@ -79,6 +81,9 @@ int launch_page_attn(const PageAttnArgs& a, cudaStream_t s) {
   const int64_t pool_rows = ((int64_t)a.c.n_pages * a.c.n_kv) << a.c.ps_log2;
   B2_CHECK_ARG(pool_rows < ((int64_t)1 << 31), "page_attn: rows of a layer's pool below 2^31");
   const float scale_log2 = (float)((double)a.scale * 1.4426950408889634);
+  int c_exp;
+  const float q_mul = 2.f * frexpf(scale_log2, &c_exp);
+  --c_exp;
   unsigned* counters = reinterpret_cast<unsigned*>(a.ws);
   float* slots = reinterpret_cast<float*>(a.ws + page_attn_counters(a));
   if (p.tc) {
@@ -89,6 +94,8 @@ int launch_page_attn(const PageAttnArgs& a, cudaStream_t s) {
     t.out = a.out;
     t.n_head = a.n_head;
     t.scale_log2 = scale_log2;
+    t.q_mul = q_mul;
+    t.c_exp = c_exp;
     t.counters = counters;
     t.slots = slots;
     t.sums = slots + 2 * (size_t)p.max_ctas * slot_floats(p.rows, a.hd);
@@ -104,6 +111,8 @@ int launch_page_attn(const PageAttnArgs& a, cudaStream_t s) {
   r.n_head = a.n_head;
   r.q_f32 = a.type_q == B2_F32;
   r.scale_log2 = scale_log2;
+  r.q_mul = q_mul;
+  r.c_exp = c_exp;
   r.counters = counters;
   r.pool_rows = pool_rows;
   r.status = a.status;

@@ -14,7 +14,10 @@
 // Q8_0 / Q4_0 as their integer codes in fp16, the block scale applied in fp32
 // to K's block sums and to p for V (a row of K or V is never rounded to
 // fp16).  In the SPLIT form a tile has 8 rows: rows 0-7 of q's operand hold the
-// high fp16 part of q (scaled in fp32), rows 8-15 the remainder, and the
+// high fp16 part of q, rows 8-15 the remainder (each row times the scale's
+// mantissa and a power of two that brings its largest value near 2^14, so the
+// parts are good for any size of q; another power of two makes the scores
+// exponents), and the
 // weights, also as two parts, are the 8-column operand of O^T = V^T·P^T, which
 // is where the scores' lanes already hold them; so fp32 queries keep 22 bits
 // and the output is good to fp32 accuracy, with half the accumulators that
@@ -60,6 +63,8 @@ struct PageRowsArgs {
   void* out;
   int n_head, q_f32;
   float scale_log2;          // scale · log2(e)
+  float q_mul;               // the same as q_mul · 2^c_exp, 1 <= |q_mul| < 2 or 0
+  int c_exp;
   FastDiv cpr_k, cpr_v;      // 16-byte chunks of a row
   int64_t pool_rows;
   int* status;
@@ -103,6 +108,11 @@ __device__ __forceinline__ void h2_split(float lo, float hi, uint32_t& head, uin
   rest = h2(lo - f.x, hi - f.y);
 }
 
+// The exponent that brings a largest magnitude (as bits; zeros, infinities and
+// NaNs too) to [2^13, 2^14), as far as 2^e stays normal.
+__device__ __forceinline__ int q_fit(uint32_t bits) { return min(140 - (int)(bits >> 23), 100); }
+__device__ __forceinline__ float pow2(int e) { return __int_as_float((e + 127) << 23); }
+
 // Bytes 0-3 of w (signed codes) as four exact fp16 values: a byte b + 128 in
 // the low bits of 0x6400 is 1024 + b + 128.
 __device__ __forceinline__ void s8x4_to_h2(uint32_t w, uint32_t& a, uint32_t& b) {
@@ -124,7 +134,6 @@ __device__ __forceinline__ void s8x4_to_h2(uint32_t w, uint32_t& a, uint32_t& b)
 // and the sums with it, exactly.
 constexpr float kOffset = 10.f, kOffsetQ = 15.f;
 constexpr int kFitMost = 23;   // e for the smallest fp16 scale, 2^-24
-__device__ __forceinline__ float pow2(int e) { return __int_as_float((e + 127) << 23); }
 
 // An fp16 (or unpacked) operand: [dims / 64][64 rows][128 bytes], 16-byte
 // chunk c of row r at c ^ (r % 8).
@@ -473,10 +482,11 @@ __global__ void __launch_bounds__(kRowsThreads + 32, rows_ctas<HD, KQ, VQ, SPLIT
       return ((int64_t)(at.q0 + tok) * a.n_head + at.h * G + rr - tok * G) * HD;
     };
 
-    // ---- queries: registers, scaled in fp32 and split, or as they are; in
+    // ---- queries: registers, split in two parts, or as they are; in
     // the dims' order within a block of 32 that the K operand is loaded in ----
     uint32_t qf[KS][4];
     int p0 = -1, p1 = -1;   // positions of rows g and g + 8 (-1: sees nothing)
+    float cs = 1.f;   // SPLIT: from scores to exponents, a power of two of the row
     {
       const int r = wm * WROWS + g, r1 = r + 8;
       const bool on0 = r < rows, on1 = !SPLIT && r1 < rows;
@@ -507,13 +517,31 @@ __global__ void __launch_bounds__(kRowsThreads + 32, rows_ctas<HD, KQ, VQ, SPLIT
               y = __half22float2(*reinterpret_cast<const __half2*>(x0 + 2 * d1));
             }
           }
-          h2_split(x.x * a.scale_log2, x.y * a.scale_log2, qf[ks][0], qf[ks][1]);
-          h2_split(y.x * a.scale_log2, y.y * a.scale_log2, qf[ks][2], qf[ks][3]);
+          qf[ks][0] = __float_as_uint(x.x), qf[ks][1] = __float_as_uint(x.y);
+          qf[ks][2] = __float_as_uint(y.x), qf[ks][3] = __float_as_uint(y.y);
         } else {
           qf[ks][0] = on0 ? *reinterpret_cast<const uint32_t*>(x0 + 2 * d0) : 0u;
           qf[ks][1] = on1 ? *reinterpret_cast<const uint32_t*>(x1 + 2 * d0) : 0u;
           qf[ks][2] = on0 ? *reinterpret_cast<const uint32_t*>(x0 + 2 * d1) : 0u;
           qf[ks][3] = on1 ? *reinterpret_cast<const uint32_t*>(x1 + 2 * d1) : 0u;
+        }
+      }
+      if constexpr (SPLIT) {
+        uint32_t top = 0;
+#pragma unroll
+        for (int ks = 0; ks < KS; ++ks)
+#pragma unroll
+          for (int e = 0; e < 4; ++e) top = max(top, qf[ks][e] & 0x7FFFFFFFu);
+        top = max(top, __shfl_xor_sync(0xffffffffu, top, 1));
+        top = max(top, __shfl_xor_sync(0xffffffffu, top, 2));
+        const int fit = q_fit(top);
+        const float f = a.q_mul * pow2(fit);
+        cs = pow2(min(max(a.c_exp - fit, -120), 120));
+#pragma unroll
+        for (int ks = 0; ks < KS; ++ks) {
+          const uint32_t x = qf[ks][2], y = qf[ks][3];
+          h2_split(__uint_as_float(qf[ks][0]) * f, __uint_as_float(qf[ks][1]) * f, qf[ks][0], qf[ks][1]);
+          h2_split(__uint_as_float(x) * f, __uint_as_float(y) * f, qf[ks][2], qf[ks][3]);
         }
       }
       __syncwarp();
@@ -757,9 +785,9 @@ __global__ void __launch_bounds__(kRowsThreads + 32, rows_ctas<HD, KQ, VQ, SPLIT
           if constexpr (!SPLIT) n1 = fmaxf(n1, __shfl_xor_sync(0xffffffffu, n1, x));
         }
         // a row that has seen nothing keeps m = -inf; its exponents are taken from 0
-        const float r0 = (n0 == -INFINITY ? 0.f : n0) - off, r1 = (n1 == -INFINITY ? 0.f : n1) - off;
+        const float r0 = (n0 == -INFINITY ? 0.f : SPLIT ? n0 * cs : n0) - off, r1 = (n1 == -INFINITY ? 0.f : n1) - off;
         if (__any_sync(0xffffffffu, n0 != m0 || (!SPLIT && n1 != m1))) {
-          const float f0 = m0 == -INFINITY ? 0.f : ex2(m0 - n0), f1 = m1 == -INFINITY ? 0.f : ex2(m1 - n1);
+          const float f0 = m0 == -INFINITY ? 0.f : ex2(SPLIT ? (m0 - n0) * cs : m0 - n0), f1 = m1 == -INFINITY ? 0.f : ex2(m1 - n1);
           l0 *= f0;
           l1 *= f1;
           float f[4];
@@ -773,8 +801,8 @@ __global__ void __launch_bounds__(kRowsThreads + 32, rows_ctas<HD, KQ, VQ, SPLIT
         }
 #pragma unroll
         for (int n = 0; n < NT; ++n) {
-          s[n][0] = ex2(s[n][0] - r0);
-          s[n][1] = ex2(s[n][1] - r0);
+          s[n][0] = ex2(SPLIT ? fmaf(s[n][0], cs, -r0) : s[n][0] - r0);
+          s[n][1] = ex2(SPLIT ? fmaf(s[n][1], cs, -r0) : s[n][1] - r0);
           l0 += s[n][0] + s[n][1];
           if constexpr (!SPLIT) {
             s[n][2] = ex2(s[n][2] - r1);
@@ -904,6 +932,7 @@ __global__ void __launch_bounds__(kRowsThreads + 32, rows_ctas<HD, KQ, VQ, SPLIT
       l0 *= r;
       l1 *= r;
     }
+    if constexpr (SPLIT) m0 *= cs;
     // ---- join the lanes' sums, and for WM = 1 the warps ----
 #pragma unroll
     for (int x = 1; x < 4; x <<= 1) {

@@ -80,7 +80,9 @@ struct PageTcArgs {
   const void* q;
   void* out;
   int n_head;
-  float scale_log2;
+  float scale_log2;       // FULL: scores to exponents; SPLIT: q_mul · 2^c_exp, 1 <= |q_mul| < 2 or 0
+  float q_mul;
+  int c_exp;
   int box_rows_log2;      // rows of a tensor copy: min(page_size, 128)
   int q_map;              // FULL: Q comes by tensor copies (G divides 128)
   int o_map;              // FULL: results leave by tensor copies (G divides 32)
@@ -563,7 +565,7 @@ __global__ void __launch_bounds__(kTcThreads, 1)
       }
     } else {
       // ---------------- products (a converged warp; one lane issues) ----------------
-      // a negative scale negates Q (SPLIT has it in Q already)
+      // a negative scale negates Q (SPLIT has that in Q already)
       const uint32_t id_s = tc_idesc(128, false) | (!SPLIT && a.scale_log2 < 0.f ? 1u << 13 : 0u);
       constexpr uint32_t id_o = tc_idesc(HD, true);
       const uint32_t q_desc = uniform(desc_k(smem_u32(Qs))), k_desc = uniform(desc_k(smem_u32(Ts))),
@@ -668,7 +670,6 @@ __global__ void __launch_bounds__(kTcThreads, 1)
     const int half = warp >> 2, r = tid, r_in = tid & 127;   // row of the tile, of the half
     const uint32_t tm = tmem + ((uint32_t)((warp & 3) * 32) << 16);
     const uint32_t ts = tm + half * 128, to = tm + 256 + half * 128;
-    const float c = SPLIT ? 1.f : fmaxf(fabsf(a.scale_log2), 1e-30f);   // the product takes the sign
     int n_o = 0, n_s = 0;   // tiles and units of this half so far
     bool ok = true;
     for (int nt = 0; ok; ++nt) {
@@ -695,12 +696,18 @@ __global__ void __launch_bounds__(kTcThreads, 1)
         return ((int64_t)(t.q0 + tok) * a.n_head + t.h * G + (t.row0 + row - tok * G)) * HD;
       };
       const int p = on ? t.first + token_of(r) : -1;
+      // from products to exponents: the product takes the sign, and a masked
+      // score of minus infinity must not meet a zero.  SPLIT: a power of two of
+      // each row.
+      float c = fmaxf(fabsf(a.scale_log2), 1e-30f);
       if constexpr (SPLIT) {
-        // ---- the warp's 32 rows of Q, a row (hd 64: two) per step, as two parts ----
+        // ---- the warp's 32 rows of Q, a row (hd 64: two) per step, as two
+        // parts, each row times the scale's mantissa and a power of two that
+        // brings its largest value near 2^14 ----
         constexpr int LR = HD / 4, RI = 32 / LR, B = 8;
         uint8_t* qd = Qs + half * 2 * L::half_q;
         const int ch = lane % LR;   // 4 values
-        const float f = a.scale_log2;
+        uint32_t own_top = 0;       // of the row this thread will own
         const int64_t e0 = place_of(on ? r : 0);
 #pragma unroll 1
         for (int it = 0; it < 32 / RI; it += B) {
@@ -713,9 +720,30 @@ __global__ void __launch_bounds__(kTcThreads, 1)
             x[e] = make_float4(0.f, 0.f, 0.f, 0.f);
             if (live) x[e] = __ldg(reinterpret_cast<const float4*>(static_cast<const float*>(a.q) + at_r) + ch);
           }
+          // largest magnitudes of the rows, a bound by their upper 16 bits: of two steps at once
+          uint32_t pair[B / 2];
+#pragma unroll
+          for (int e = 0; e < B; e += 2) {
+            uint32_t top[2];
+#pragma unroll
+            for (int i = 0; i < 2; ++i)
+              top[i] = max(max(__float_as_uint(fabsf(x[e + i].x)), __float_as_uint(fabsf(x[e + i].y))),
+                           max(__float_as_uint(fabsf(x[e + i].z)), __float_as_uint(fabsf(x[e + i].w))));
+            if constexpr (LR == 32) {
+              pair[e / 2] = __byte_perm(__reduce_max_sync(0xffffffffu, top[0]), __reduce_max_sync(0xffffffffu, top[1]), 0x7632);
+            } else {
+              pair[e / 2] = __byte_perm(top[0], top[1], 0x7632);
+#pragma unroll
+              for (int i = 1; i < LR; i <<= 1) pair[e / 2] = __vmaxu2(pair[e / 2], __shfl_xor_sync(0xffffffffu, pair[e / 2], i));
+            }
+            const uint32_t to_own = RI == 1 ? pair[e / 2] : __shfl_sync(0xffffffffu, pair[e / 2], (lane % RI) * LR);
+            if (lane / RI == it + e) own_top = to_own << 16;
+            if (lane / RI == it + e + 1) own_top = to_own;
+          }
 #pragma unroll
           for (int e = 0; e < B; ++e) {
             const int rl = (warp & 3) * 32 + (it + e) * RI + lane / LR;
+            const float f = a.q_mul * pow2(q_fit(e & 1 ? pair[e / 2] : pair[e / 2] << 16));
             uint2 hi, lo;
             h2_split(x[e].x * f, x[e].y * f, hi.x, lo.x);
             h2_split(x[e].z * f, x[e].w * f, hi.y, lo.y);
@@ -726,6 +754,7 @@ __global__ void __launch_bounds__(kTcThreads, 1)
         }
         fence_async_proxy();
         mbar_arrive(&q_full[half]);
+        c = pow2(min(max(a.c_exp - q_fit(own_top), -120), 120));
       }
       float m = -INFINITY, l = 0.f, m_sum = -INFINITY;   // m_sum: the maximum that the sum is relative to
       float4* sum_row = SPLIT ? reinterpret_cast<float4*>(a.sums) + ((int64_t)blockIdx.x * 2 + half) * (HD / 4) * 128 + r_in : nullptr;

@@ -414,7 +414,9 @@ B2_API int b2_rope_sections(const int32_t* sections, int32_t n_axes, int32_t n_p
  * outside the positions a token sees reaches its row, infinite and NaN ones
  * included.  Results do not depend on timing: the same call gives the same
  * bits.  Unlike b2_attn_decode the sums are not in the reference's sequential
- * order.  |scale·q| and |v| up to 65504 (fp16's range).
+ * order.  q, k and v may have any size that their types hold: fp32 queries
+ * keep 22 bits relative to the row's largest value, and the weights of
+ * quantized v are scaled by its largest block scale.
  * workspace: device, 16-byte aligned, of at least
  * b2_page_attn_workspace_bytes for the call's shapes, set to zero (b2_memset)
  * before its first use; every call leaves it fit for the next, of any shape

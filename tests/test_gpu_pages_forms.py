@@ -132,3 +132,43 @@ def test_attn_quantized_values_growing_along_the_positions(form, t, hd, grow):
     v = np.random.default_rng(1).standard_normal((900, n_kv, hd)) * size[:, None, None]
     s.V[0, s.table[0, p // 16], :, p % 16] = rows_of(v.astype(np.float32), t)
     check_norm(s)
+
+
+@pytest.mark.parametrize("form,hd", [("tokens", 64), ("tokens", 128), ("chunk", 64), ("chunk", 128), ("chunk", 96)])
+@pytest.mark.parametrize("qt,size", [(F32, 1e-4), (F32, 1e-3), (F32, 1), (F32, 1.4e4), (F32, 1e6), (F16, 1e-3), (F16, 1.4e4)])
+@pytest.mark.parametrize("kt", [F16, Q8])
+def test_attn_queries_of_any_size(form, hd, qt, size, kt):
+    """Scores of unit size from small queries and large keys and the reverse;
+    products of large ones pass fp16's range."""
+    q_len, n_head, n_kv = FORMS[form]
+    s = shared(3, 700, n_head, n_kv, hd, 16, kt, kt, qt, 13, q_len, k=lambda x: x / (size * hd ** 0.5))
+    s.Q = s.Q.astype(np.float32) * np.float32(size)
+    s.Q = (s.Q if qt == F32 else np.clip(s.Q, -65504, 65504)).astype(NP[qt])
+    check_norm(s, scale=1.0)
+    check_norm(s, scale=-1.0)
+
+
+@pytest.mark.parametrize("form,hd", [("tokens", 64), ("tokens", 128), ("chunk", 64), ("chunk", 128), ("chunk", 96)])
+def test_attn_rows_of_mixed_size(form, hd):
+    """Rows of one call between 1e-20 and 1e20 and all-zero ones: none disturbs
+    another.  Scores of the large ones only tell the largest key."""
+    q_len, n_head, n_kv = FORMS[form]
+    s = shared(3, 400, n_head, n_kv, hd, 16, F16, F16, F32, 14, q_len)
+    size = 10.0 ** np.array([0, -20, 20, 1, -3, -38])[np.arange(s.n_tok * n_head) % 6].reshape(s.n_tok, n_head, 1)
+    s.Q = (s.Q * size).astype(np.float32)
+    s.Q[0, 0] = 0
+    check_sampled(s)
+    check_sampled(s, scale=0.0)
+
+
+@pytest.mark.parametrize("form,hd", [("tokens", 128), ("chunk", 64), ("chunk", 128), ("chunk", 96)])
+@pytest.mark.parametrize("bad", [np.inf, -np.inf, np.nan])
+def test_attn_nonfinite_queries_stay_in_their_rows(form, hd, bad):
+    q_len, n_head, n_kv = FORMS[form]
+    s = shared(3, 400, n_head, n_kv, hd, 16, F16, F16, F32, 14, q_len)
+    clean = s.run()
+    s.Q[1::2, 1, 5] = bad
+    got = s.run()
+    assert np.all(np.isnan(got[1::2, 1]))
+    got[1::2, 1] = clean[1::2, 1]
+    assert np.array_equal(got, clean)
