@@ -757,6 +757,11 @@ __global__ void __launch_bounds__(kTcThreads, 1)
         c = pow2(min(max(a.c_exp - q_fit(own_top), -120), 120));
       }
       float m = -INFINITY, l = 0.f, m_sum = -INFINITY;   // m_sum: the maximum that the sum is relative to
+      // FULL: c is no power of two, so far from zero the rounding of m would be
+      // more than an exponent may be off by; there the scores in TMEM are made
+      // relative to the maximum first, as the product left both.
+      float m_raw = -INFINITY;
+      bool far = false;
       float4* sum_row = SPLIT ? reinterpret_cast<float4*>(a.sums) + ((int64_t)blockIdx.x * 2 + half) * (HD / 4) * 128 + r_in : nullptr;
       for (int u = 0; u < units; ++u) {
         const int key0 = tile_key0 + u * kTcBk;
@@ -785,7 +790,9 @@ __global__ void __launch_bounds__(kTcThreads, 1)
           }
           m_sum = m;
         }
+        bool shifted = false;   // the scores in TMEM are relative to m_raw already
         float s[128];
+      [[maybe_unused]] load_scores:
         tmem_ld128(ts, s);
         // this row sees columns [lo, hi)
         const int hi = min(p + 1, tile_hi) - key0, lo = w.window > 0 ? p - w.window + 1 - key0 : 0;
@@ -808,11 +815,12 @@ __global__ void __launch_bounds__(kTcThreads, 1)
 
 #pragma unroll
         for (int e = 0; e < 4; ++e) top[e] = max_nan(top[e], s[124 + e]);
-        const float high = max_nan(max_nan(top[0], top[1]), max_nan(top[2], top[3])) * c;
-        const bool raise = !(high <= m + kTcRaise);   // from -inf, and to NaN, always
-        if (__any_sync(0xffffffffu, raise)) {
+        const float raw = max_nan(max_nan(top[0], top[1]), max_nan(top[2], top[3])), high = raw * c;
+        bool raise = !(high <= m + kTcRaise);   // from -inf, and to NaN, always
+        if (!shifted && __any_sync(0xffffffffu, raise || far)) {
+          if (!SPLIT && far) raise = raise || raw > m_raw;
           const float nm = raise ? high : m;
-          const float f = m == -INFINITY ? 0.f : ex2(m - nm);
+          const float f = m == -INFINITY ? 0.f : ex2(SPLIT ? m - nm : (m_raw - (raise ? raw : m_raw)) * c);
           const float g = raise ? f : 1.f;            // the other rows keep their maximum
           if (u > 0) {
             float o[16];
@@ -826,8 +834,25 @@ __global__ void __launch_bounds__(kTcThreads, 1)
           }
           l *= g;
           m = nm;
+          if constexpr (!SPLIT) {
+            m_raw = raise ? raw : m_raw;
+            far = __any_sync(0xffffffffu, fabsf(m) > 4194304.f && m != -INFINITY);
+            if (far) {
+              float x[16];
+#pragma unroll 1
+              for (int i = 0; i < 8; ++i) {
+                tmem_ld16(ts + i * 16, x);
+#pragma unroll
+                for (int e = 0; e < 16; ++e) x[e] -= m_raw == -INFINITY ? 0.f : m_raw;
+                tmem_st16(ts + i * 16, reinterpret_cast<const uint32_t*>(x));
+              }
+              tmem_wait_st();
+              shifted = true;
+              goto load_scores;
+            }
+          }
         }
-        const float rs = kTcOffset - (m == -INFINITY ? 0.f : m);
+        const float rs = kTcOffset - (m == -INFINITY || shifted ? 0.f : m);
         float2 sum[2] = {make_float2(0.f, 0.f), make_float2(0.f, 0.f)};
 #pragma unroll
         for (int h = 0; h < 4; ++h) {

@@ -172,3 +172,16 @@ def test_attn_nonfinite_queries_stay_in_their_rows(form, hd, bad):
     assert np.all(np.isnan(got[1::2, 1]))
     got[1::2, 1] = clean[1::2, 1]
     assert np.array_equal(got, clean)
+
+
+@pytest.mark.parametrize("form,hd", [("tokens", 64), ("tokens of 12 heads", 128), ("chunk", 64), ("chunk", 128), ("chunk", 96)])
+@pytest.mark.parametrize("qt", [F32, F16])
+def test_attn_scores_of_any_size(form, hd, qt):
+    """Scores past 2^24, whose rounding alone is more than an exponent may be
+    off by: each row takes the value of its largest key."""
+    q_len, n_head, n_kv = FORMS[form]
+    for size in (1e2, 1e4, 6e4):
+        s = shared(3, 700, n_head, n_kv, hd, 16, F16, F16, qt, 17, q_len, k=lambda x: np.clip(x * size, -65504, 65504))
+        s.Q = np.clip(s.Q.astype(np.float32) * size, -65504, 65504).astype(NP[qt])
+        check_sampled(s, scale=1.0)
+        check_sampled(s, scale=-1.0)
