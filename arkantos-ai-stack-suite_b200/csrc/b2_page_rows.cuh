@@ -171,6 +171,11 @@ __host__ __device__ constexpr int rows_q_bytes() {
   return WM == 1 ? (SPLIT ? 8 * HD * 4 : 16 * HD * 2) : 0;
 }
 constexpr int kRowsStagesMax = 8, kRowsCtrl = 1024;
+// SPLIT, warps along the positions: units between two additions, with
+// rounding, of the result so far to an fp32 sum.  The tensor pipe cuts a sum at
+// each of the unit's two steps; over a share of 512 units that was 3.4e-5 of
+// the result, now 1.1e-6.
+constexpr int kRowsFlush = 16;
 constexpr int kWaitPolls = 1 << 22;   // polls of a wait, each suspended by the hardware for a while
 
 __device__ __forceinline__ void tma_2d(uint32_t dst, const CUtensorMap* map, int x, int y, uint64_t* bar) {
@@ -588,7 +593,39 @@ __global__ void __launch_bounds__(kRowsThreads + 32, rows_ctas<HD, KQ, VQ, SPLIT
     // positions every live row sees need no mask
     const int p_min = at.first + w.G.div(row0), p_max = at.first + w.G.div(row0 + rows - 1);
 
+    // WM = 1: [4 warps][16] (maximum, sum), then [4 warps][WROWS][HD] sums, after
+    // the ring.  Until the tile's end SPLIT keeps its fp32 sums there, a lane's
+    // own (see kRowsFlush), with the maximum and the offset they are relative to.
+    float2* ml = reinterpret_cast<float2*>(ring + stages * stage_bytes);
+    float* so = reinterpret_cast<float*>(ml + 64);
+    float4* own_sum = reinterpret_cast<float4*>(so + warp * WROWS * HD) + lane;
+    auto add_sums = [&]() {   // to o
+      const float2 rel = ml[warp * 16 + g];
+      float x = rel.x == -INFINITY ? 0.f : ex2((rel.x - m0) * cs), f[4];
+      if constexpr (VQ) x *= pow2((__float_as_int(fit) >> 23) - (__float_as_int(rel.y) >> 23));
+      by_row(x, x, f);
+#pragma unroll
+      for (int d = 0; d < OT; ++d) {
+        const float4 y = own_sum[d * 32];
+        o[d][0] = fmaf(y.x, f[0], o[d][0]);
+        o[d][1] = fmaf(y.y, f[1], o[d][1]);
+        o[d][2] = fmaf(y.z, f[2], o[d][2]);
+        o[d][3] = fmaf(y.w, f[3], o[d][3]);
+      }
+      __syncwarp();
+    };
+
     for (int u = u_lo; u < u_hi; ++u, ++done) {
+      if (SPLIT && WM == 1 && u > u_lo && (u - u_lo) % kRowsFlush == 0) {
+        if (u - u_lo > kRowsFlush) add_sums();
+#pragma unroll
+        for (int d = 0; d < OT; ++d) {
+          own_sum[d * 32] = make_float4(o[d][0], o[d][1], o[d][2], o[d][3]);
+          o[d][0] = o[d][1] = o[d][2] = o[d][3] = 0.f;
+        }
+        if (j == 0) ml[warp * 16 + g] = make_float2(m0, fit);
+        __syncwarp();
+      }
       uint8_t* st = ring + (done % stages) * stage_bytes;
       const int key0 = (at.lo_unit + u) * kRowsBk;
       const bool edge = key0 + kRowsBk > at.hi || key0 + kRowsBk - 1 > p_min ||
@@ -923,6 +960,7 @@ __global__ void __launch_bounds__(kRowsThreads + 32, rows_ctas<HD, KQ, VQ, SPLIT
       }
     }
 
+    if (SPLIT && WM == 1 && u_hi - u_lo > kRowsFlush) add_sums();
     if constexpr (VQ) {   // warps and parts meet with the same offset
       const float r = pow2(127 - (__float_as_int(fit) >> 23));
 #pragma unroll
@@ -953,9 +991,6 @@ __global__ void __launch_bounds__(kRowsThreads + 32, rows_ctas<HD, KQ, VQ, SPLIT
     };
 
     if constexpr (WM == 1) {
-      // [4 warps][16] (m, l), then [4 warps][WROWS][HD] sums, after the ring
-      float2* ml = reinterpret_cast<float2*>(ring + stages * stage_bytes);
-      float* so = reinterpret_cast<float*>(ml + 64);
       if (j == 0) {
         ml[warp * 16 + g] = make_float2(m0, l0);
         if constexpr (!SPLIT) ml[warp * 16 + g + 8] = make_float2(m1, l1);

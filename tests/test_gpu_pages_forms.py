@@ -185,3 +185,11 @@ def test_attn_scores_of_any_size(form, hd, qt):
         s.Q = np.clip(s.Q.astype(np.float32) * size, -65504, 65504).astype(NP[qt])
         check_sampled(s, scale=1.0)
         check_sampled(s, scale=-1.0)
+
+
+# ---- long shares ---------------------------------------------------------------------------------
+@pytest.mark.parametrize("t", [F16, Q8, Q4])
+@pytest.mark.parametrize("hd,page,n_seq,n", [(64, 256, 70, 32768), (128, 64, 70, 32768), (96, 16, 70, 9000), (256, 8, 90, 9000)])
+def test_attn_tokens_fp32_accuracy_does_not_fall_with_a_ctas_share(t, hd, page, n_seq, n):
+    """A CTA adds over hundreds of units of one tile; values of one sign, so that cuts of a sum add up."""
+    check_norm(shared(n_seq, n, 8, 8, hd, page, t, t, F32, 14, v=lambda x: 1 + x), n_rows=60)
