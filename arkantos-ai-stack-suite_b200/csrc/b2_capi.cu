@@ -730,7 +730,9 @@ int b2_page_attn(const b2_page_cache* cache, int32_t layer, const b2_page_batch*
   a.q = q;
   a.out = out;
   a.scale = scale;
-  a.window = window > 0 ? window : 0;
+  // a window as long as the table hides nothing; shorter ones keep position
+  // minus window within 32 bits, for positions below zero too
+  a.window = window > 0 && window < (int64_t)batch->max_pages * cache->page_size ? window : 0;
   a.status = status;
   const size_t need = page_attn_workspace(a);
   B2_CHECK_ARG(!workspace || workspace_bytes >= need, "page_attn: workspace below b2_page_attn_workspace_bytes");

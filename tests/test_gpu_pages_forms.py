@@ -193,3 +193,16 @@ def test_attn_scores_of_any_size(form, hd, qt):
 def test_attn_tokens_fp32_accuracy_does_not_fall_with_a_ctas_share(t, hd, page, n_seq, n):
     """A CTA adds over hundreds of units of one tile; values of one sign, so that cuts of a sum add up."""
     check_norm(shared(n_seq, n, 8, 8, hd, page, t, t, F32, 14, v=lambda x: 1 + x), n_rows=60)
+
+
+# ---- windows -------------------------------------------------------------------------------------
+@pytest.mark.parametrize("qt", [F32, F16])
+@pytest.mark.parametrize("q_len,hd", [(4, 64), (70, 64), (70, 128), (40, 96)])
+@pytest.mark.parametrize("window", [2 ** 31 - 1, 2 ** 30, 4096])
+def test_attn_windows_past_every_position(q_len, hd, window, qt):
+    """A window that hides nothing, with more new tokens than positions: the
+    first ones' positions lie below zero."""
+    s = Setup([q_len, 1, q_len], [q_len - 3, 0, q_len + 200], 8, 2, hd, 16, qt=qt, seed=3)
+    got = s.check(window=window)
+    assert np.all(got[:3] == 0)
+    assert np.array_equal(got, s.run().astype(np.float64))
