@@ -590,6 +590,10 @@ __global__ void __launch_bounds__(kRowsThreads + 32, rows_ctas<HD, KQ, VQ, SPLIT
       fit = pow2(e);
       off = kOffsetQ + e;
     };
+    // Where the exponents of a row with maximum m are counted from: a row that
+    // has seen nothing keeps m = -inf and counts from 0.  Rounded up, so that no
+    // weight passes 2^off where the offset is below the spacing of scores.
+    auto origin = [&](float m) { return __fsub_ru(m == -INFINITY ? 0.f : SPLIT ? m * cs : m, off); };
     // positions every live row sees need no mask
     const int p_min = at.first + w.G.div(row0), p_max = at.first + w.G.div(row0 + rows - 1);
 
@@ -601,7 +605,7 @@ __global__ void __launch_bounds__(kRowsThreads + 32, rows_ctas<HD, KQ, VQ, SPLIT
     float4* own_sum = reinterpret_cast<float4*>(so + warp * WROWS * HD) + lane;
     auto add_sums = [&]() {   // to o
       const float2 rel = ml[warp * 16 + g];
-      float x = rel.x == -INFINITY ? 0.f : ex2((rel.x - m0) * cs), f[4];
+      float x = rel.x == -INFINITY ? 0.f : ex2(origin(rel.x) - origin(m0)), f[4];
       if constexpr (VQ) x *= pow2((__float_as_int(fit) >> 23) - (__float_as_int(rel.y) >> 23));
       by_row(x, x, f);
 #pragma unroll
@@ -821,10 +825,9 @@ __global__ void __launch_bounds__(kRowsThreads + 32, rows_ctas<HD, KQ, VQ, SPLIT
           n0 = fmaxf(n0, __shfl_xor_sync(0xffffffffu, n0, x));
           if constexpr (!SPLIT) n1 = fmaxf(n1, __shfl_xor_sync(0xffffffffu, n1, x));
         }
-        // a row that has seen nothing keeps m = -inf; its exponents are taken from 0
-        const float r0 = (n0 == -INFINITY ? 0.f : SPLIT ? n0 * cs : n0) - off, r1 = (n1 == -INFINITY ? 0.f : n1) - off;
+        const float r0 = origin(n0), r1 = origin(n1);
         if (__any_sync(0xffffffffu, n0 != m0 || (!SPLIT && n1 != m1))) {
-          const float f0 = m0 == -INFINITY ? 0.f : ex2(SPLIT ? (m0 - n0) * cs : m0 - n0), f1 = m1 == -INFINITY ? 0.f : ex2(m1 - n1);
+          const float f0 = m0 == -INFINITY ? 0.f : ex2(origin(m0) - r0), f1 = m1 == -INFINITY ? 0.f : ex2(origin(m1) - r1);
           l0 *= f0;
           l1 *= f1;
           float f[4];
@@ -970,7 +973,8 @@ __global__ void __launch_bounds__(kRowsThreads + 32, rows_ctas<HD, KQ, VQ, SPLIT
       l0 *= r;
       l1 *= r;
     }
-    if constexpr (SPLIT) m0 *= cs;
+    if (m0 != -INFINITY) m0 = origin(m0) + off;
+    if (m1 != -INFINITY) m1 = origin(m1) + off;
     // ---- join the lanes' sums, and for WM = 1 the warps ----
 #pragma unroll
     for (int x = 1; x < 4; x <<= 1) {

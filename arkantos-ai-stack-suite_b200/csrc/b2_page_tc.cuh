@@ -816,7 +816,9 @@ __global__ void __launch_bounds__(kTcThreads, 1)
 #pragma unroll
         for (int e = 0; e < 4; ++e) top[e] = max_nan(top[e], s[124 + e]);
         const float raw = max_nan(max_nan(top[0], top[1]), max_nan(top[2], top[3])), high = raw * c;
-        bool raise = !(high <= m + kTcRaise);   // from -inf, and to NaN, always
+        // both roundings towards less, so that no weight passes 2^15 where the
+        // offsets are below the spacing of scores
+        bool raise = !(high <= __fadd_rd(m, kTcRaise));   // from -inf, and to NaN, always
         if (!shifted && __any_sync(0xffffffffu, raise || far)) {
           if (!SPLIT && far) raise = raise || raw > m_raw;
           const float nm = raise ? high : m;
@@ -852,7 +854,7 @@ __global__ void __launch_bounds__(kTcThreads, 1)
             }
           }
         }
-        const float rs = kTcOffset - (m == -INFINITY || shifted ? 0.f : m);
+        const float rs = __fsub_rd(kTcOffset, m == -INFINITY || shifted ? 0.f : m);
         float2 sum[2] = {make_float2(0.f, 0.f), make_float2(0.f, 0.f)};
 #pragma unroll
         for (int h = 0; h < 4; ++h) {

@@ -187,6 +187,25 @@ def test_attn_scores_of_any_size(form, hd, qt):
         check_sampled(s, scale=-1.0)
 
 
+@pytest.mark.parametrize("form,hd", [("tokens", 64), ("tokens of 12 heads", 128), ("chunk", 64), ("chunk", 128), ("chunk", 96)])
+@pytest.mark.parametrize("qt", [F32, F16])
+@pytest.mark.parametrize("vt", [F16, Q8])
+def test_attn_weights_add_up_at_any_score(form, hd, qt, vt):
+    """Scores around 2^18 to 2^44, many within a few units of the last place of
+    the largest: all values are one number, so every result is."""
+    q_len, n_head, n_kv = FORMS[form]
+    for size in (1.0, 2.0 ** -10):
+        s = shared(3, 700, n_head, n_kv, hd, 16, F16, vt, qt, 18, q_len, k=lambda x: 1 - (x > 1) * 2.0 ** -11,
+                   v=lambda x: 0 * x + size)
+        s.Q = np.abs(s.Q.astype(np.float32) * 100 + 1000).astype(NP[qt])
+        v = s.seq_values(0, 700)[1]
+        assert np.all(v == v[0, 0, 0])
+        for e in range(18, 45):
+            for sign in (1, -1):
+                got = s.run(scale=sign * 2.0 ** e / (1000 * hd)).astype(np.float64) / v[0, 0, 0]
+                assert np.all(np.abs(got - 1) <= (2e-5 if qt == F32 else 2.0 ** -10)), (e, sign)
+
+
 # ---- long shares ---------------------------------------------------------------------------------
 @pytest.mark.parametrize("t", [F16, Q8, Q4])
 @pytest.mark.parametrize("hd,page,n_seq,n", [(64, 256, 70, 32768), (128, 64, 70, 32768), (96, 16, 70, 9000), (256, 8, 90, 9000)])
