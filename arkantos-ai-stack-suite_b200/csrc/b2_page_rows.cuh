@@ -1008,7 +1008,7 @@ __global__ void __launch_bounds__(kRowsThreads + 32, rows_ctas<HD, KQ, VQ, SPLIT
 #pragma unroll
       for (int e = 0; e < 4; ++e) {
         const float2 x = ml[warp * 16 + o_row(e)];
-        f[e] = x.y == 0.f ? 0.f : x.x == -INFINITY ? 1.f : ex2(x.x - top(o_row(e)));
+        f[e] = part_weight(x.x, x.y, top(o_row(e)));
       }
 #pragma unroll
       for (int d = 0; d < OT; ++d)

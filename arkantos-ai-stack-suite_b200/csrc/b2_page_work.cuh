@@ -305,9 +305,11 @@ __device__ __forceinline__ void store_joined(void* out, bool f32, int64_t at, co
 }
 // A part's weight for a row with maximum m and sum l in it: a part that saw
 // nothing of the row adds nothing; a sum without a maximum comes from scores
-// that are all NaN.
+// that are all NaN.  Any other weight stays positive, too small for finite
+// values to count, so that an infinite or NaN value of a low score is not lost.
+constexpr float kLeastWeight = 1.17549435e-38f;
 __device__ __forceinline__ float part_weight(float m, float l, float top) {
-  return l == 0.f ? 0.f : m == -INFINITY ? 1.f : ex2(m - top);
+  return l == 0.f ? 0.f : m == -INFINITY ? 1.f : fmaxf(ex2(m - top), kLeastWeight);
 }
 
 // Rows row .. row + min(R, n_rows) - 1 of a split tile from its parts, by one

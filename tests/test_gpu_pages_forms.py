@@ -225,3 +225,27 @@ def test_attn_windows_past_every_position(q_len, hd, window, qt):
     got = s.check(window=window)
     assert np.all(got[:3] == 0)
     assert np.array_equal(got, s.run().astype(np.float64))
+
+
+# ---- values that are not finite -------------------------------------------------------------------
+@pytest.mark.parametrize("bits", [0x7C00, 0x7E00])
+@pytest.mark.parametrize("q_len,hd,kt,qt", [(1, 64, F16, F32), (1, 128, F16, F16), (1, 128, Q8, F32), (40, 64, F16, F32),
+                                            (40, 128, F16, F16), (40, 128, Q8, F16), (40, 96, F16, F32)])
+def test_attn_infinite_value_of_a_low_score(q_len, hd, kt, qt, bits):
+    """An infinite or NaN value whose weight is some e^-500, in another part of
+    a split tile than the large weights, still reaches every row that sees it."""
+    n, at = 6000, 10
+    s = Setup([q_len], [n], 4, 2, hd, 16, kt, kt, qt, seed=15)
+    p = np.arange(n)
+    k = np.random.default_rng(0).standard_normal((1, s.n_pages, 2, 16, hd), dtype=np.float32)
+    k[0, s.table[0, p // 16], :, p % 16] = np.where(p < n // 2, -20, 20)[:, None, None]
+    s.K = rows_of(k, kt)
+    s.Q = (np.abs(s.Q) + 1).astype(NP[qt])
+    clean, _ = s.want()
+    first = 0 if kt == F16 else hd           # a value, or the first block's scale
+    s.V[0, s.table[0, at // 16], :, at % 16, first:first + 2] = [0, bits >> 8]
+    got = s.run().astype(np.float64)
+    touched = 1 if kt == F16 else 32
+    assert np.all(~np.isfinite(got[..., :touched]).all(-1))
+    tol = 1e-4 if qt == F32 else 4e-3        # the rest is as it was (|v| below 5)
+    assert np.all(np.abs(got - clean)[..., touched:] <= tol)
