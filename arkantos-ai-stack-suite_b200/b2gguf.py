@@ -527,9 +527,10 @@ def page_attn_workspace_bytes(cache: PageCache, batch: PageBatch, n_head: int, t
 
 
 def page_attn_workspace(cache: PageCache, batch: PageBatch, n_head: int, type_q: int) -> DeviceBuffer:
-    """A workspace for calls of this batch's shapes and smaller ones, set to zero as its first use needs."""
+    """A workspace for calls of this batch's shapes and smaller ones, on any stream, set to zero as its first use needs."""
     w = DeviceBuffer(page_attn_workspace_bytes(cache, batch, n_head, type_q))
     w.zero()
+    check(lib.b2_stream_synchronize(None), "sync")   # its first call may be on a stream that does not wait for this one
     return w
 
 

@@ -249,3 +249,26 @@ def test_attn_infinite_value_of_a_low_score(q_len, hd, kt, qt, bits):
     assert np.all(~np.isfinite(got[..., :touched]).all(-1))
     tol = 1e-4 if qt == F32 else 4e-3        # the rest is as it was (|v| below 5)
     assert np.all(np.abs(got - clean)[..., touched:] <= tol)
+
+
+# ---- the workspace -------------------------------------------------------------------------------
+def test_workspace_is_zero_when_it_is_handed_out(monkeypatch):
+    """For calls on any stream: streams of their own do not wait for the
+    default one, which may be busy."""
+    s = Setup([1], [100], 8, 2, 64, 16)
+    c, b = s.cache(), s.batch()
+    n = b2.page_attn_workspace_bytes(c, b, 8, F32)
+    big, ws = b2.DeviceBuffer(8 << 30), b2.DeviceBuffer(n)
+    host, st = b2.PinnedArray((n,), np.uint8), b2.Stream()
+    b2.check(b2.lib.b2_memset(ws.ptr, 0xFF, n, None))
+    b2.synchronize()
+    for _ in range(20):                        # some 20 ms of work
+        b2.check(b2.lib.b2_memset(big.ptr, 1, big.nbytes, None))
+    with monkeypatch.context() as m:
+        m.setattr(b2, "DeviceBuffer", lambda size: ws)
+        assert b2.page_attn_workspace(c, b, 8, F32) is ws
+    b2.check(b2.lib.b2_memcpy_d2h(host.p, ws.ptr, n, st.h))
+    st.synchronize()
+    got = host.array.copy()
+    b2.synchronize()
+    assert not got.any()
