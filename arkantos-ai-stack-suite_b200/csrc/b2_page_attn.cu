@@ -52,6 +52,7 @@ PageWork work_of(const PageAttnArgs& a, const Plan& p) {
   w.n_kv = a.c.n_kv;
   w.G = FastDiv::of(a.n_head / a.c.n_kv);
   w.window = a.window;
+  w.fair = (int)((((int64_t)1 << 31) - 1) / ((int64_t)a.c.n_kv * a.b.n_seq));
   while (w.rows() < p.rows) ++w.rows_log2;
   while (w.bk() < p.bk) ++w.bk_log2;
   if (p.wm != 1) {   // one warp joins 32 rows; with few rows the join is spread over lanes and parts, and cheap

@@ -44,6 +44,7 @@ struct PageWork {
   FastDiv G;                                     // query heads of a kv head
   int ps_log2, n_kv, window, rows_log2, bk_log2;   // rows of a tile, positions of a unit
   float join_per_tile;                             // see find_share
+  int fair;                                        // units of a sequence that n_seq · n_kv of them keep below 2^31
   __host__ __device__ int rows() const { return 1 << rows_log2; }
   __host__ __device__ int bk() const { return 1 << bk_log2; }
 };
@@ -135,20 +136,32 @@ __device__ __forceinline__ void sum_units(const PageWork& w, int* sums) {
   }
 }
 
+// Whether a call's units are too many to count: the launcher bounds them for
+// sequences that divide the tokens, but q_start is the device's, and sequences
+// that overlap could pass 2^31.
+__device__ __forceinline__ bool too_many_units(const PageWork& w, const int* sums) {
+  int64_t total = 0;
+  for (int s = 0; s < w.b.n_seq; ++s) total += sums[s];
+  return total * w.n_kv >= ((int64_t)1 << 31);
+}
+
 // Warp-wide, from the sums: the share of CTA `cta` of `ctas`.  Returns false
-// for a CTA without work.  A tile of U units in shares of k takes k units' time
+// for a CTA without work, and for a batch with more units than can be counted.  A tile of U units in shares of k takes k units' time
 // and that of joining U/k parts; with j the units' time that a part takes to
 // join, k = sqrt(j U) is best, U the mean over the tiles (join_per_tile is j
 // over the number of tiles), and no CTA gets fewer.
 __device__ __forceinline__ bool find_share(const PageWork& w, int cta, int ctas, const int* sums, Share& sh) {
   const int lane = threadIdx.x & 31;
   int per_head = 0;
+  bool more = false;
   for (int s0 = 0; s0 < w.b.n_seq; s0 += 32) {
     int v = s0 + lane < w.b.n_seq ? sums[s0 + lane] : 0;
+    more = more || v > w.fair;
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
     per_head += v;
   }
+  if (__any_sync(0xffffffffu, more) && too_many_units(w, sums)) return false;
   const int total = per_head * w.n_kv;
   const int least = max(1, (int)ceilf(sqrtf(w.join_per_tile * (float)total)));
   sh.deal.n = min((int)((unsigned)(total + least - 1) / (unsigned)least), ctas);

@@ -364,8 +364,10 @@ typedef struct b2_page_cache {
  * p % page_size of page table[s·max_pages + p / page_size].  The three arrays
  * are device int32 and are read when the call runs, so a captured call follows
  * them.  q_start[0] = 0 and ascending; n_tok is q_start[n_seq] or more, rows
- * past it are not touched; max_q is at least every sequence's new tokens.
- * Lengths outside the arrays are clamped into them; a table entry outside
+ * past it are not touched; max_q, 1 to n_tok, is at least every sequence's new
+ * tokens.  Lengths outside the arrays are clamped into them, and a batch whose
+ * sequences overlap reads and writes nothing outside them (its results are
+ * undefined); a table entry outside
  * [0, n_pages) that a position needs reads as a row of zeros and stores
  * nothing.  n_seq <= 1024, max_pages·page_size <= 2^30. */
 typedef struct b2_page_batch {

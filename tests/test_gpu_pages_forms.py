@@ -272,3 +272,28 @@ def test_workspace_is_zero_when_it_is_handed_out(monkeypatch):
     got = host.array.copy()
     b2.synchronize()
     assert not got.any()
+
+
+# ---- malformed batches ---------------------------------------------------------------------------
+@pytest.mark.parametrize("qt,kt", [(F16, F16), (F32, F16), (F32, Q8)])
+def test_attn_overlapping_sequences_that_pass_all_counts(qt, kt):
+    """512 sequences that claim all of 65536 tokens each: more work units than
+    32 bits count.  The call does nothing, and the workspace stays fit."""
+    n, n_seq, n_kv, hd = 1 << 16, 1024, 8, 64
+    c = b2.PageCache(1, 4, 256, n_kv, hd, kt, kt)
+    start = np.where(np.arange(n_seq + 1) % 2, n, 0).astype(np.int32)
+    start[-1] = n
+    b = b2.PageBatch(start, np.full(n_seq, 1 << 20, np.int32), np.full((n_seq, 4096), -1, np.int32), n_tok=n, max_q=n)
+    q, out = b2.DeviceBuffer(n * n_kv * hd * 4), b2.DeviceBuffer(n * n_kv * hd * 4)
+    b2.check(b2.lib.b2_memset(out.ptr, 77, out.nbytes, None))
+    ws = b2.page_attn_workspace(c, b, n_kv, qt)
+    b2.page_attn(c, 0, b, n_kv, q, out, qt, workspace=ws)
+    b2.synchronize()
+    assert np.all(out.download(np.uint8) == 77)
+    s = Setup([70, 3], [200, 300], 8, 2, 64, 16, kt, kt, qt, seed=1)
+    c, b = s.cache(), s.batch()
+    x, y = b2.DeviceBuffer.from_array(s.Q), b2.DeviceBuffer(s.Q.nbytes)
+    assert b2.page_attn_workspace_bytes(c, b, 8, qt) <= ws.nbytes
+    b2.page_attn(c, 0, b, 8, x, y, qt, workspace=ws)
+    b2.synchronize()
+    assert np.array_equal(y.download(NP[qt]).reshape(s.Q.shape), s.run())
