@@ -570,7 +570,7 @@ namespace {
 
 int page_check(const b2_page_cache* c, bool pools = true) {
   B2_CHECK_ARG(c && (!pools || (c->k && c->v)), "page cache pools");
-  B2_CHECK_ARG(c->n_layer > 0 && c->n_pages > 0 && c->n_kv > 0, "page cache sizes");
+  B2_CHECK_ARG(c->n_layer > 0 && c->n_pages > 0 && c->n_kv > 0 && c->n_kv <= (1 << 20), "page cache sizes");
   B2_CHECK_ARG(c->page_size >= 8 && c->page_size <= 256 && (c->page_size & (c->page_size - 1)) == 0,
                "page_size must be a power of two from 8 to 256");
   B2_CHECK_ARG(c->head_dim > 0 && c->head_dim % 32 == 0 && c->head_dim <= 256,
@@ -663,6 +663,9 @@ int b2_page_rope_store(const b2_page_cache* cache, int32_t layer, const b2_page_
   B2_CHECK_ARG(n_pos > 0 && n_rot > 0 && n_rot % 8 == 0 && n_rot <= cache->head_dim,
                "page_rope_store: n_rot a multiple of 8 up to head_dim");
   B2_CHECK_ARG(style == B2_ROPE_ADJACENT || style == B2_ROPE_HALVES, "page_rope_store: style");
+  // a CTA counts the values of its tokens in 31 bits
+  B2_CHECK_ARG((int64_t)n_head + 2 * cache->n_kv <= (1 << 20), "page_rope_store: more than 2^20 heads");
+  B2_CHECK_ARG(batch->n_tok <= (1 << 30), "page_rope_store: n_tok up to 2^30");
   RopeStoreArgs a;
   a.c = page_view(cache, layer);
   a.b = page_seqs(batch);

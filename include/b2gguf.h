@@ -350,7 +350,7 @@ B2_API int b2_flag_wait(const uint64_t* flags, int n, uint64_t target, int* stat
  * aligned): [n_layer][n_pages][n_kv][page_size] rows of
  * b2_kv_row_bytes(type, head_dim) bytes, in the storage of the typed caches
  * above.  page_size a power of two, 8..256; head_dim a multiple of 32 up to
- * 256 (attention: 64, 96, 128 and 256). */
+ * 256 (attention: 64, 96, 128 and 256); n_kv up to 2^20. */
 typedef struct b2_page_cache {
     void*   k;
     void*   v;
@@ -393,7 +393,8 @@ B2_API int b2_page_cache_bytes(const b2_page_cache* cache, size_t* bytes_k, size
  * quantize.  With B2_F32 and one axis the results are bit-identical to
  * b2_rope_kv_store_typed.  A token with a rotary position or axis outside the
  * table, or no place in the cache, gets a zero q row and stores nothing.
- * n_rot a multiple of 8 up to head_dim.  Every device array 16-byte aligned
+ * n_rot a multiple of 8 up to head_dim, n_head + 2·n_kv up to 2^20, n_tok up
+ * to 2^30.  Every device array 16-byte aligned
  * (pos, axis and the batch: their own type). */
 #define B2_ROPE_ADJACENT 0
 #define B2_ROPE_HALVES 1
