@@ -214,6 +214,12 @@ def test_attn_tokens_fp32_accuracy_does_not_fall_with_a_ctas_share(t, hd, page, 
     check_norm(shared(n_seq, n, 8, 8, hd, page, t, t, F32, 14, v=lambda x: 1 + x), n_rows=60)
 
 
+@pytest.mark.parametrize("t,hd", [(F16, 64), (F16, 128), (F16, 96), (Q8, 64), (Q4, 128)])
+def test_attn_chunks_fp32_accuracy_does_not_fall_with_a_ctas_share(t, hd):
+    """The same with many rows: tiles of 16384 positions, two and more a CTA."""
+    check_norm(shared(50, 16384, 32, 8, hd, 64, t, t, F32, 14, 30, v=lambda x: 1 + x), n_rows=60)
+
+
 # ---- windows -------------------------------------------------------------------------------------
 @pytest.mark.parametrize("qt", [F32, F16])
 @pytest.mark.parametrize("q_len,hd", [(4, 64), (70, 64), (70, 128), (40, 96)])
@@ -297,3 +303,145 @@ def test_attn_overlapping_sequences_that_pass_all_counts(qt, kt):
     b2.page_attn(c, 0, b, 8, x, y, qt, workspace=ws)
     b2.synchronize()
     assert np.array_equal(y.download(NP[qt]).reshape(s.Q.shape), s.run())
+
+
+# ---- every form over every cache -----------------------------------------------------------------
+TYPES = [(a, b) for a in (F16, Q8, Q4) for b in (F16, Q8, Q4)]
+
+
+@pytest.mark.parametrize("kt,vt", TYPES)
+@pytest.mark.parametrize("hd", [64, 96, 128, 256])
+@pytest.mark.parametrize("qt", [F32, F16])
+@pytest.mark.parametrize("n_head,n_kv", [(4, 4), (16, 2), (12, 1), (16, 1)])
+def test_attn_single_tokens_over_every_cache(kt, vt, hd, qt, n_head, n_kv):
+    """Steps of single tokens only: 1, 8, 12 and 16 rows a kv head."""
+    kv = [1, 31, 33, 64, 130, 700]
+    Setup([1] * len(kv), kv, n_head, n_kv, hd, 32, kt, vt, qt, seed=kt * 7 + vt + hd + n_head).check()
+
+
+@pytest.mark.parametrize("kt,vt", TYPES)
+@pytest.mark.parametrize("hd", [64, 96, 128, 256])
+@pytest.mark.parametrize("qt", [F32, F16])
+def test_attn_single_tokens_many_units_and_tiles(kt, vt, hd, qt):
+    """At least 8 tiles and 60 units a CTA; fp16 queries with 12 heads a kv head and with one."""
+    n_head = 96 if qt == F16 and hd <= 128 else 8
+    check_sampled(shared(450 if hd < 256 else 150, 460, n_head, 8, hd, 16, kt, vt, qt, hd + kt, 1), 200)
+
+
+@pytest.mark.parametrize("kt,vt", TYPES)
+@pytest.mark.parametrize("hd", [64, 96, 128, 256])
+@pytest.mark.parametrize("qt", [F32, F16])
+def test_attn_chunks_many_units_and_tiles(kt, vt, hd, qt):
+    """At least 6 tiles and 40 units a CTA in either kernel for many rows."""
+    over_tc = kt == vt == F16 and hd in (64, 128)
+    q_len, n_seq = (150, 80) if over_tc else (50, 180)
+    check_sampled(shared(n_seq, 900, 16, 8, hd, 64, kt, vt, qt, hd + vt, q_len), 200)
+
+
+@pytest.mark.parametrize("kt,vt", [(F16, F16), (Q8, Q8), (Q4, Q8)])
+@pytest.mark.parametrize("hd", [64, 128])
+@pytest.mark.parametrize("qt", [F32, F16])
+@pytest.mark.parametrize("window", [0, 100])
+def test_attn_ragged_chunks_many_tiles(kt, vt, hd, qt, window):
+    """Tiles of every length in one share, most of them short."""
+    r = np.random.default_rng(hd + window)
+    q = [int(x) for x in r.integers(0, 200, 90)]
+    kv = [n + int(x) for n, x in zip(q, r.integers(0, 700, 90))]
+    q[5], kv[5], kv[7] = 40, 10, 0
+    check_sampled(Setup(q, kv, 16, 8, hd, 16, kt, vt, qt, seed=7), 300, window=window)
+
+
+@pytest.mark.parametrize("page", [8, 128, 256])
+@pytest.mark.parametrize("kt,vt", [(F16, F16), (Q8, Q8), (Q4, Q4), (F16, Q4), (Q8, F16)])
+@pytest.mark.parametrize("q_len", [1, 40])
+@pytest.mark.parametrize("hd", [96, 256])
+def test_attn_page_sizes_over_every_cache(page, kt, vt, q_len, hd):
+    Setup([q_len, q_len], [q_len + 70, q_len + 257], 4, 2, hd, page, kt, vt, F32, seed=page).check()
+
+
+@pytest.mark.parametrize("kt,vt", [(Q8, Q8), (Q4, Q4), (F16, Q8), (Q4, F16)])
+@pytest.mark.parametrize("hd,n_head,n_kv,page", [(64, 8, 2, 8), (128, 4, 1, 32), (128, 6, 2, 256), (64, 5, 5, 128)])
+@pytest.mark.parametrize("qt", [F32, F16])
+def test_attn_quantized_chunks(kt, vt, hd, n_head, n_kv, page, qt):
+    Setup([130, 1, 0, 45, 3], [130, 257, 12, 300, 3], n_head, n_kv, hd, page, kt, vt, qt, seed=hd + page).check()
+
+
+@pytest.mark.parametrize("window", [1, 50, 300])
+@pytest.mark.parametrize("page", [16, 256])
+@pytest.mark.parametrize("q_len", [[140, 64, 1], [1, 1, 1]])
+@pytest.mark.parametrize("kt,vt", [(Q8, Q4), (Q4, Q4)])
+def test_attn_quantized_windows(window, page, q_len, kt, vt):
+    Setup(q_len, [700, 64, 513], 4, 2, 64, page, kt, vt, qt=F32, seed=window).check(window=window)
+
+
+@pytest.mark.parametrize("q_len", [[128, 150, 30], [1, 150, 1], [1, 1, 1]])
+@pytest.mark.parametrize("kt,vt", [(Q8, Q8), (Q4, F16), (F16, Q4)])
+@pytest.mark.parametrize("qt", [F32, F16])
+def test_attn_quantized_layer_table_and_workspace(q_len, kt, vt, qt):
+    """Another layer, table entries outside the pool, more new tokens than
+    positions, a workspace that holds anything past its counters."""
+    s = Setup(q_len, [200, 140, 90], 4, 2, 128, 16, kt, vt, qt, seed=9, n_layer=3, layer=1)
+    s.table[0, 3], s.table[2, 0] = -7, s.n_pages + 1
+    a = s.check()
+    assert np.array_equal(a, s.run(workspace=False).astype(np.float64))
+    c, b = s.cache(), s.batch()
+    ws = b2.page_attn_workspace(c, b, s.n_head, qt)
+    x = np.full(ws.nbytes, 0x7E, np.uint8)
+    x[:1 << 16] = 0                            # the counters
+    ws.upload(x)
+    q, out = b2.DeviceBuffer.from_array(s.Q), b2.DeviceBuffer(s.Q.nbytes)
+    for _ in range(2):
+        b2.page_attn(c, s.layer, b, s.n_head, q, out, qt, workspace=ws)
+    b2.synchronize()
+    assert np.array_equal(out.download(NP[qt]).reshape(s.Q.shape).astype(np.float64), a)
+
+
+@pytest.mark.parametrize("bits", [0x7C00, 0xFC00, 0x7E00])
+@pytest.mark.parametrize("t", [Q8, Q4])
+@pytest.mark.parametrize("q_len,window", [(140, 0), (9, 0), (9, 5), (1, 0), (1, 20)])
+@pytest.mark.parametrize("hd", [64, 128])
+def test_attn_nonfinite_scales(bits, t, q_len, window, hd):
+    """Infinite and NaN block scales reach the rows that see them and no others."""
+    n = 200
+    at = n - 5 if q_len > 5 else n - 40
+    s = Setup([q_len], [n], 4, 2, hd, 16, t, t, F32, seed=3)
+    want, vmax = s.want(window=window)
+    code = hd if t == Q8 else hd // 2
+    for pool in (s.K, s.V):
+        pool[0, s.table[0, at // 16], :, at % 16, code:code + 2] = np.frombuffer(np.uint16(bits).tobytes(), np.uint8)
+    got = s.run(window=window).astype(np.float64)
+    p = np.arange(n - q_len, n)
+    sees = (p >= at) & ((p - at < window) if window else True)
+    assert np.all(~np.isfinite(got[sees]).all(-1))
+    assert np.all(np.abs(got - want)[~sees] <= 2e-5 * vmax[~sees])
+
+
+@pytest.mark.parametrize("axes", [4, 5, 8])
+@pytest.mark.parametrize("style", [0, 1])
+@pytest.mark.parametrize("hd,rot", [(128, 128), (64, 32)])
+def test_store_of_many_axes(axes, style, hd, rot):
+    """Bit for bit, as with fewer axes; and an axis past the last stores nothing."""
+    from tests.test_gpu_pages import dev, rotate
+    n_head, n_kv, n, n_pos, half = 4, 2, 29, 300, rot // 2
+    s = Setup([n], [40], n_head, n_kv, hd, 16, qt=F32, seed=axes, poison=False)
+    r = np.random.default_rng(axes)
+    x = r.standard_normal((n, n_head + 2 * n_kv, hd), dtype=np.float32)
+    pos = r.integers(0, n_pos, (axes, n)).astype(np.int32)
+    axis = r.integers(0, axes, half).astype(np.uint8)
+    table = b2.rope_table(10000.0, rot, 0, n_pos)
+    for broken in (False, True):
+        if broken:
+            axis[half // 2] = axes
+        c, q = s.cache(), dev(np.full((n, n_head, hd), 77, np.float32))
+        b2.page_rope_store(c, 0, s.batch(), n_head, dev(x), F32, q, F32, dev(pos), axes, dev(axis), dev(table), n_pos, rot,
+                           style)
+        b2.synchronize()
+        got, K = q.download(np.float32).reshape(n, n_head, hd), s.K.copy()
+        if broken:
+            assert not got.any()
+        else:
+            y = rotate(x[:, :n_head + n_kv], table.reshape(n_pos, half, 2)[pos[axis].T, np.arange(half)], style)
+            assert np.array_equal(got, y[:, :n_head])
+            p = 40 - n + np.arange(n)
+            K[0, s.table[0, p // 16], :, p % 16] = rows_of(y[:, n_head:], F16)
+        assert np.array_equal(s.k.download(np.uint8).reshape(K.shape), K)
