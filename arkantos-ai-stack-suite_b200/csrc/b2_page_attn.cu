@@ -12,8 +12,8 @@ namespace {
 // where it reads the cache, else the few-row kernel with its warps along the
 // rows.  One kernel takes all sequences of a call: running both, each on the
 // sequences of its kind, was slower (a step of 12 single tokens and 4 chunks
-// of 129 over 300-2049 positions: 81 us against 47 with fp16 queries), since
-// the second begins when the first has ended.
+// of 129 over 300-2049 positions: 81 us against 47 with fp16 queries in one
+// run; 49 now), since the second begins when the first has ended.
 constexpr int kFewRows = 16;
 struct Plan {
   bool tc, split;
@@ -39,11 +39,12 @@ Plan plan_of(const PageAttnArgs& a) {
   return p;
 }
 // Units' time that a warp takes to join a part of a split tile (see find_share).
-// One sequence's 8 tokens over 512, 4096 and 16384 fp16 positions: 22, 74 and
-// 65 us when every CTA gets some of them, 19, 33 and 56 with 0.4; 0.25 gives
-// 22, 43, 64, 0.6 19, 37, 59 and 1.5 24, 36, 56.  The few-row kernel's units and
-// tiles are smaller: fp32 queries over Q8_0 20, 54, 76 against 20, 41, 76 with
-// 0.1; 0.4 gives 24, 45, 80.
+// One sequence's 8 tokens over 512, 4096 and 16384 fp16 positions, all measured
+// in one run: 22, 74 and 65 us when every CTA gets some of them, 19, 33 and 56
+// with 0.4 (now 18, 31, 53); 0.25 gives 22, 43, 64, 0.6 19, 37, 59 and 1.5 24,
+// 36, 56.  The few-row kernel's units and tiles are smaller: fp32 queries over
+// Q8_0 20, 54, 76 against 20, 41, 76 with 0.1 (now 21, 42, 80); 0.4 gives 24,
+// 45, 80.
 constexpr float kJoinTc = 0.4f, kJoinRows = 0.1f;
 PageWork work_of(const PageAttnArgs& a, const Plan& p) {
   PageWork w = {};

@@ -17,16 +17,16 @@
 // high fp16 part of q, rows 8-15 the remainder (each row times the scale's
 // mantissa and a power of two that brings its largest value near 2^14, so the
 // parts are good for any size of q; another power of two makes the scores
-// exponents), and the
-// weights, also as two parts, are the 8-column operand of O^T = V^T·P^T, which
-// is where the scores' lanes already hold them; so fp32 queries keep 22 bits
-// and the output is good to fp32 accuracy, with half the accumulators that
-// P·V would take.  The FULL form (fp16 queries and outputs) rounds p once to fp16, the size of
-// error the fp16 output has by itself.  Accumulators, maxima and sums are
-// fp32.
+// exponents), and the weights, also as two parts, are the 8-column operand of
+// O^T = V^T·P^T, which is where the scores' lanes already hold them; so fp32
+// queries keep 22 bits and the output is good to fp32 accuracy, with half the
+// accumulators that P·V would take.  The FULL form (fp16 queries and outputs)
+// rounds p once to fp16, over a quantized V its product with the block scale,
+// an error of the size of the fp16 output's.  Accumulators, maxima and sums
+// are fp32.
 //
-// Measured: 32 sequences of 4048 over fp16 pages 93 us, 5.7 TB/s; 16 of 4096
-// over Q8_0 51 us, 2.9 TB/s, where the instructions that turn codes into
+// Measured: 32 sequences of 4048 over fp16 pages 91 us, 5.8 TB/s; 16 of 4096
+// over Q8_0 54 us, 2.8 TB/s, where the instructions that turn codes into
 // operands bound it (issue slots half used, warps waiting on their latency).
 //
 // Layout.  A unit is 64 positions.  One warp brings K and V through a ring of
@@ -159,8 +159,9 @@ __host__ __device__ inline int rows_conv_bytes() {
 }
 // CTAs meant for an SM: registers and the ring are cut to fit.  Reading
 // quantized rows is bound by the latency of the code's own steps, not by HBM,
-// and gains from a third (64 sequences of 4096 over Q8_0: 167 -> 156 us);
-// fp16 rows of head_dim 128 do not (97 us against 98 for 32 of them).
+// and gains from a third (64 sequences of 4096 over Q8_0: 167 -> 156 us when
+// that was measured, 164 now); fp16 rows of head_dim 128 do not (97 us against
+// 98 for 32 of them).
 template <int HD, bool KQ, bool VQ, bool SPLIT>
 __host__ __device__ constexpr int rows_ctas() {
   return HD == 256 ? 1 : HD == 64 || (KQ && VQ && SPLIT) ? 3 : 2;
@@ -258,7 +259,8 @@ __global__ void __launch_bounds__(kRowsThreads + 32, rows_ctas<HD, KQ, VQ, SPLIT
   uint64_t* t_empty = t_full + 1;                          // and been taken
   int* abort_flag = reinterpret_cast<int*>(smem + 256);
   int* last_part = abort_flag + 1;
-  uint32_t* v_top = reinterpret_cast<uint32_t*>(smem + 264);   // [2] by unit (WM = 4): largest scale of V, as bits, if the offset must fall
+  // [2] by unit (WM = 4): the largest scale of V, as bits, where the offset must fall
+  uint32_t* v_top = reinterpret_cast<uint32_t*>(smem + 264);
   TileAt* tile = reinterpret_cast<TileAt*>(smem + 320);
   constexpr int kQRows = rows_q_bytes<HD, SPLIT, WM>();
   uint8_t* q_rows = smem + kRowsCtrl;                      // WM = 1: the tile's queries as they are in q

@@ -15,9 +15,11 @@
 // some 3500 cycles, the length of a half's own chain of score product,
 // maximum, exponentials and second product, of which two run side by side
 // (TMEM holds no third half).  2048 tokens over 16384 positions, 32 heads of
-// 128: 437 us or 1180 TFLOP/s, the tensor pipe 57 % busy; SPLIT 905 us.  Two
-// threads a row (16 softmax warps) shorten the chain less than their exchange
-// of maxima costs: eight prompts 274 us against 267.
+// 128: 449 us or 1150 TFLOP/s, the tensor pipe 57 % busy; SPLIT 920 us.  Eight
+// prompts of 1500-2048 tokens: 276 us in a short run, 300-310 once a long one
+// has lowered the clocks.  Two threads a row (16 softmax warps) shortened the
+// chain less than their exchange of maxima cost (274 us against 267, when both
+// were measured in one short run).
 //
 //   warps 0-3, 4-7  softmax of halves 0, 1, and their results
 //   warp 8          issues the products from one thread
@@ -42,12 +44,16 @@
 // their offset of 2^7, inside fp16's range), so O is rarely rescaled.
 //
 // SPLIT (fp32 queries): q and p as two fp16 parts each, high and remainder,
-// two products instead of one; both parts of p take exactly S's columns.
+// two products instead of one; both parts of p take exactly S's columns.  A
+// row of q is brought near 2^14 by a power of two first, taken back in its
+// scores, so the parts are good for any size of q.
 // The tensor pipe cuts its sums to fp32 at every step of 16, so an O that runs
 // over all positions loses accuracy with their number (7.8e-6 of the result
 // at 8192); after every 3 units SPLIT therefore adds it, rounded, to a sum in
 // the workspace and begins anew.
-// FULL rounds p once to fp16, the error of the fp16 output itself.
+// FULL rounds p once to fp16, an error of the size of the fp16 output's, and
+// leaves its sums to the pipe (2.6e-4 of the result with 32768 positions in one
+// CTA, 1.0e-3 with 262144).
 //
 // V rows that a tile must not see are zeroed in shared memory before the
 // unit's product, and infinite or NaN values of units that only some rows see
@@ -96,8 +102,9 @@ struct PageTcArgs {
 constexpr int kTcRows = 256, kTcBk = 128, kTcThreads = 384;
 constexpr float kTcOffset = 7.f, kTcRaise = 8.f;
 // SPLIT: units between two additions of O to its fp32 sum.  2, 3, 4, 8 and
-// never give 1.0, 1.2, 1.5, 2.0 and 2.3e-6 on a mixed step over 300-2049
-// positions, where fp32 arithmetic gives 0.9e-6, in 81, 78, 76, 73 and 65 us.
+// never give 1.0, 1.2, 1.5, 2.0 and 2.2e-6 on a mixed step over 300-2049
+// positions, where fp32 arithmetic gives 0.9e-6, in 84, 81, 80, 78 and 72 us;
+// over 16384 positions in one CTA, values of one sign, never gives 8.5e-5.
 constexpr int kTcFlush = 3;
 
 template <int HD, bool SPLIT>

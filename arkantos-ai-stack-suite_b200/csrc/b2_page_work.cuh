@@ -146,10 +146,11 @@ __device__ __forceinline__ bool too_many_units(const PageWork& w, const int* sum
 }
 
 // Warp-wide, from the sums: the share of CTA `cta` of `ctas`.  Returns false
-// for a CTA without work, and for a batch with more units than can be counted.  A tile of U units in shares of k takes k units' time
-// and that of joining U/k parts; with j the units' time that a part takes to
-// join, k = sqrt(j U) is best, U the mean over the tiles (join_per_tile is j
-// over the number of tiles), and no CTA gets fewer.
+// for a CTA without work, and for a batch with more units than can be counted.
+// A tile of U units in shares of k takes k units' time and that of joining U/k
+// parts; with j the units' time that a part takes to join, k = sqrt(j U) is
+// best, U the mean over the tiles (join_per_tile is j over the number of
+// tiles), and no CTA gets fewer.
 __device__ __forceinline__ bool find_share(const PageWork& w, int cta, int ctas, const int* sums, Share& sh) {
   const int lane = threadIdx.x & 31;
   int per_head = 0;

@@ -412,19 +412,26 @@ B2_API int b2_rope_sections(const int32_t* sections, int32_t n_axes, int32_t n_p
  * token or many per sequence: the token at position p attends to positions
  * (p - window, p], window <= 0 meaning all up to p, with n_head/n_kv query
  * heads per kv head and scores scale·q·k.  q and out [n_tok][n_head][head_dim]
- * of type_q: B2_F32 is computed to fp32 accuracy, B2_F16 rounds the softmax
- * weights to fp16.  A token that sees no position gets a zero row; no value
- * outside the positions a token sees reaches its row, infinite and NaN ones
- * included.  Results do not depend on timing: the same call gives the same
+ * of type_q.  B2_F32 is computed to fp32 accuracy.  B2_F16, with more than 8
+ * rows (max_q tokens times n_head/n_kv), rounds the softmax weights to fp16,
+ * over quantized v their products with the block scales, and its sums are the
+ * tensor pipe's alone, each step cut at 2^-24: the result's error is 2.9e-4 of
+ * it where the fp16 result alone gives 2.1e-4, and where one CTA adds over very
+ * many positions the cuts show (1.0e-3 over 262144).  A token that sees no
+ * position gets a zero row; no value outside the positions a token sees reaches
+ * its row, infinite and NaN ones included.  Results do not depend on timing:
+ * the same call gives the same bits.  They do depend, within these errors, on
+ * the whole call: max_q and the other sequences decide the kernel and how tiles
+ * are divided, so a sequence replayed in another batch need not repeat its
  * bits.  Unlike b2_attn_decode the sums are not in the reference's sequential
  * order.  q, k and v may have any size that their types hold: fp32 queries
  * keep 22 bits relative to the row's largest value, and the weights of
  * quantized v are scaled by its largest block scale.
  * workspace: device, 16-byte aligned, of at least
- * b2_page_attn_workspace_bytes for the call's shapes, set to zero (b2_memset)
- * before its first use; every call leaves it fit for the next, of any shape
- * that it is large enough for, and one call at a time may use it.  NULL: the
- * call allocates stream-ordered scratch.  status (device int,
+ * b2_page_attn_workspace_bytes for the call's shapes, set to zero (b2_memset,
+ * on the call's stream or awaited) before its first use; every call leaves it
+ * fit for the next, of any shape that it is large enough for, and one call at a
+ * time may use it.  NULL: the call allocates stream-ordered scratch.  status (device int,
  * may be NULL) receives a nonzero code if a pipeline wait expired; the call's
  * results are then undefined, and the workspace is to be set to zero again
  * before its next use. */
@@ -451,6 +458,7 @@ B2_API int b2_page_gather(const b2_page_cache* cache, int32_t n_seq, const int32
 
 /* Host-side page bookkeeping (CPU only): which pages each sequence holds, in
  * order, its length, and how many sequences share a page.  Not thread-safe.
+ * page_size 1..256, a power of two (the device operators take 8 and up).
  * The pool decides, b2_page_copy and b2_page_gather move the bytes; calls on
  * one stream in the order of the decisions keep a page's old readers ahead of
  * its new writers. */
